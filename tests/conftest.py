@@ -15,6 +15,15 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (runs the CUDA library)")
 
 
+def pytest_collection_modifyitems(items):
+    """The program that test_reference_main_with_cuda_backend_links runs is built from the
+    reference's sources: without them there is nothing to link."""
+    if not (ROOT / "oracle" / "_ref" / "mg_generate_cuda").exists():
+        for item in items:
+            if item.name == "test_reference_main_with_cuda_backend_links":
+                item.add_marker(pytest.mark.skip(reason="built only where the reference tree exists"))
+
+
 @pytest.fixture(scope="session")
 def golden():
     return np.load(GOLDEN)
