@@ -21,6 +21,24 @@ I = C.c_int
 I64 = C.c_int64
 F = C.c_float
 
+
+class AttentionArgs(C.Structure):
+    """mgc_attention_args"""
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("Sq", C.c_int32), ("Sk", C.c_int32), ("Hq", C.c_int32),
+                ("Hkv", C.c_int32), ("D", C.c_int32), ("causal", C.c_int32),
+                ("q", P), ("k", P), ("v", P), ("out", P),
+                ("q_stride", I64 * 3), ("k_stride", I64 * 3), ("v_stride", I64 * 3), ("out_stride", I64 * 3),
+                ("scale", F), ("cap", F), ("slopes", P), ("dist_bias", P), ("dist_range", C.c_int32),
+                ("reserved", C.c_int32), ("prefix", P), ("k_len", P), ("q_pos", P), ("doc_q", P), ("doc_k", P),
+                ("workspace", P), ("workspace_bytes", C.c_uint64)]
+
+
+class LogitControls(C.Structure):
+    """mgc_logit_controls"""
+    _fields_ = [("repetition", F), ("frequency", F), ("presence", F), ("bias", P), ("allowed", P),
+                ("allowed_rows", C.c_int32)]
+
+
 _SIGS = {
     "mgc_last_error": (C.c_char_p, []),
     "mgc_device_error": (I, []),
@@ -37,6 +55,11 @@ _SIGS = {
     "mgc_layernorm_affine": (I, [P, P, P, I, I, F, P, P]),
     "mgc_flash_attn": (I, [P, I, I, I, I, F, P, P]),
     "mgc_embed": (I, [P, I, P, I, P, I, I, P, P]),
+    "mgc_linear": (I, [I, P, I64, P, I64, I, I, I, P, I, P, I64, P, I64, P]),
+    "mgc_attention_workspace": (I, [C.POINTER(AttentionArgs), C.POINTER(C.c_uint64)]),
+    "mgc_attention": (I, [C.POINTER(AttentionArgs), P]),
+    "mgc_logits_adjust": (I, [I, P, I64, I, I, P, I64, I, P, P, I64, P, I64, P, I64, P, I64, P]),
+    "mgc_generate_with": (I, [P, I, P, P, I, F, C.POINTER(LogitControls), P]),
     "mgc_runtime_create": (I, [C.c_char_p, I, I, C.POINTER(P)]),
     "mgc_runtime_destroy": (None, [P]),
     "mgc_tp_unique_id": (I, [P]),

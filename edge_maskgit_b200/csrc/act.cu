@@ -401,7 +401,8 @@ void launch_quant_act_tiled(const float* x, int M, int K, const ActQ& a, bool wa
 // CB - 1.  Lanes compute the exponentials, lane 0 runs the two ordered sums.
 __global__ void __launch_bounds__(128) sample_codes_kernel(const float* __restrict__ logits, int rows, int vocab,
                                                            int CB, const double* __restrict__ r,
-                                                           int32_t* __restrict__ sid, float* __restrict__ psid) {
+                                                           int32_t* __restrict__ sid, float* __restrict__ psid,
+                                                           bool masked) {
     griddep_wait();
     griddep_launch();
     extern __shared__ float e_sm[];
@@ -424,6 +425,10 @@ __global__ void __launch_bounds__(128) sample_codes_kernel(const float* __restri
         int pick = CB - 1;
         for (int v = 0; v < CB; v++) {
             acc = __dadd_rn(acc, (double)__fmul_rn(e[v], inv));
+            if (masked) {   // a forbidden code (probability 0) is never drawn, by rounding or by r = 0
+                if (e[v] == 0.0f) continue;
+                pick = v;
+            }
             if (rr <= acc) { pick = v; break; }
         }
         sid[row] = pick;
@@ -432,10 +437,10 @@ __global__ void __launch_bounds__(128) sample_codes_kernel(const float* __restri
 }
 
 void launch_sample_codes(const float* logits, int rows, int vocab, int CB, const double* r, int32_t* sid, float* psid,
-                         cudaStream_t st) {
+                         cudaStream_t st, bool masked) {
     ++g_launch_count;
     launch_k(sample_codes_kernel, (unsigned)((rows + 3) / 4), 128, (size_t)4 * CB * sizeof(float), st, logits, rows,
-             vocab, CB, r, sid, psid);
+             vocab, CB, r, sid, psid, masked);
 }
 
 }  // namespace mgc

@@ -1,0 +1,317 @@
+// attn_step.cu -- mgc_attention for few queries against long keys (a decode step), and the join of
+// split key ranges.
+//
+// Bound by the bytes of k and v, which are read once: the Sq * (Hq / Hkv) query rows that share a
+// key head sit in one 16-row tensor-core tile (mma.sync m16n8k16; with 16 rows or fewer per key the
+// tile is memory-bound by an order of magnitude, so the tcgen05 path with its 128-row tile would
+// add nothing).  The key range is split over CTAs, and inside a CTA over four warps.  Each warp has
+// its own ring of 16-key stages filled by cp.async, so the main loop has no CTA-wide barrier; the
+// online softmax keeps (max, sum, output) in registers, and warps and CTAs are joined at the end.
+#include <stdexcept>
+
+#include "attn_shaped.cuh"
+
+namespace mgc {
+namespace {
+
+constexpr int WARPS = 4, KT = 16, STAGES = 4;
+template <int DP> constexpr int row_bytes() { return DP * 2 + 16; }   // odd in 16-byte units: ldmatrix without conflicts
+template <int DP> constexpr int stage_bytes() { return 2 * KT * row_bytes<DP>(); }
+template <int DP> constexpr int ring_bytes() { return WARPS * STAGES * stage_bytes<DP>(); }
+template <int DP> constexpr int join_bytes() { return WARPS * 16 * (DP * 4 + 8); }
+template <int DP> constexpr int smem_bytes() { return ring_bytes<DP>() > join_bytes<DP>() ? ring_bytes<DP>() : join_bytes<DP>(); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes global -> shared, or zeros
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool copy) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(copy ? 16 : 0) : "memory");
+}
+
+// Writes one finished row (o = dims lane + 32 u), repairing a NaN.
+template <bool BF16>
+__device__ __forceinline__ void write_row(const AttnCall& c, int b, int h, int i, float (&o)[4]) {
+    const int lane = threadIdx.x & 31;
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < 4; u++) bad |= lane + 32 * u < c.a.D && isnan(o[u]);
+    if (__any_sync(0xffffffffu, bad)) exact_row<BF16>(c.a, c.g, b, h, i, o);
+    const long long at = b * c.a.out_stride[0] + i * c.a.out_stride[1] + h * c.a.out_stride[2];
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+        if (lane + 32 * u < c.a.D) store16<BF16>(c.a.out, at + lane + 32 * u, o[u]);
+}
+
+// grid: splits x (batch row, key head, 16-row block), splits fastest
+template <bool BF16, int DP>
+__global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_constant__ AttnCall c) {
+    constexpr int RB = row_bytes<DP>(), SB = stage_bytes<DP>(), NK = DP / 16, CH = DP / 8;
+    extern __shared__ __align__(16) uint8_t smem[];
+    griddep_wait();
+    griddep_launch();
+    const mgc_attention_args& a = c.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qr = lane >> 2, qc = (lane & 3) * 2;
+    const int split = blockIdx.x % c.nsplit;
+    long long rest = blockIdx.x / c.nsplit;
+    const int rows = a.Sq * c.g, blocks = (rows + 15) / 16;
+    const int blk = (int)(rest % blocks); rest /= blocks;
+    const int hk = (int)(rest % a.Hkv), b = (int)(rest / a.Hkv);
+    const RowBounds rb = row_bounds(a, b);
+
+    // rows of this lane's fragments: blk * 16 + qr and + 8; row = query i * g + (h - hk * g)
+    int row[2], qi[2], head[2], doc[2], end[2];
+    ScoreShape sh[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        row[u] = blk * 16 + qr + 8 * u;
+        const int rr = min(row[u], rows - 1);
+        qi[u] = rr / c.g;
+        head[u] = hk * c.g + rr % c.g;
+        sh[u] = score_shape(a, head[u]);
+        doc[u] = a.doc_q ? __ldg(a.doc_q + (long long)b * a.Sq + qi[u]) : 0;
+        end[u] = row[u] < rows && doc[u] >= 0 ? key_end(rb, rb.pos0 + qi[u]) : 0;
+    }
+    uint32_t qf[NK][4];
+#pragma unroll
+    for (int k = 0; k < NK; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int u = e & 1, d = k * 16 + qc + (e >> 1) * 8;
+            const long long at = b * a.q_stride[0] + qi[u] * a.q_stride[1] + head[u] * a.q_stride[2] + d;
+            qf[k][e] = d < a.D ? __ldg(reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(a.q) + at)) : 0u;
+        }
+
+    // this CTA's keys: the split's chunk, cut to what the block's last query sees
+    const int last_q = min(blk * 16 + 15, rows - 1) / c.g;
+    const int k_lo = split * c.chunk, k_hi = min(k_lo + c.chunk, key_end(rb, rb.pos0 + last_q));
+    const int tiles = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
+    const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
+    const uint16_t* vp = reinterpret_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
+    const uint32_t ring = smem_u32(smem) + warp * STAGES * SB;
+    const int mine = tiles > warp ? (tiles - warp + WARPS - 1) / WARPS : 0;   // tiles warp, warp + 4, ...
+
+    auto load = [&](int n) {   // stage n % STAGES <- the warp's n-th tile; keys past the end read as zeros
+        if (n < mine) {
+            const int j0 = k_lo + (warp + n * WARPS) * KT;
+            const uint32_t s = ring + (n % STAGES) * SB;
+#pragma unroll
+            for (int x = lane; x < KT * CH; x += 32) {
+                const int r = x / CH, ch = x % CH, j = j0 + r;
+                const bool in = j < k_hi && ch * 8 < a.D;
+                const long long jj = in ? j : 0;
+                const int d = in ? ch * 8 : 0;
+                cp16_or_zero(s + r * RB + ch * 16, kp + jj * a.k_stride[1] + d, in);
+                cp16_or_zero(s + KT * RB + r * RB + ch * 16, vp + jj * a.v_stride[1] + d, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[DP / 8][4];
+#pragma unroll
+    for (int d = 0; d < DP / 8; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[d][e] = 0.0f;
+    for (int n = 0; n < STAGES - 1; n++) load(n);
+    for (int n = 0; n < mine; n++) {
+        load(n + STAGES - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
+        const uint32_t s = ring + (n % STAGES) * SB;
+        const int j0 = k_lo + (warp + n * WARPS) * KT;
+        float sc[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            uint32_t kf[4];   // keys 0-7 and 8-15, d halves
+            ldsm4(kf, s + (lane & 15) * RB + k * 32 + (lane >> 4) * 16);
+            mma16816<BF16>(sc[0], qf[k], kf[0], kf[2]);
+            mma16816<BF16>(sc[1], qf[k], kf[1], kf[3]);
+        }
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int u = e >> 1, j = j0 + t * 8 + qc + (e & 1);
+                bool seen = j < end[u];
+                if (a.doc_k) seen = seen && __ldg(a.doc_k + (long long)b * a.Sk + min(j, a.Sk - 1)) == doc[u];
+                sc[t][e] = seen ? shaped(sc[t][e], sh[u], j - (rb.pos0 + qi[u])) : -INFINITY;
+                mx[u] = fmaxf(mx[u], sc[t][e]);
+            }
+        float alpha[2], base[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
+            mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
+            const float mn = fmaxf(m[u], mx[u]);
+            base[u] = mn == -INFINITY ? 0.0f : mn;   // nothing seen yet: p = 2^-inf = 0
+            alpha[u] = ex2_approx(m[u] - base[u]);
+            m[u] = mn;
+        }
+        uint32_t pf[4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float p[4];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) p[t * 2 + e] = ex2_approx(sc[t][u * 2 + e] - base[u]);
+            l[u] = l[u] * alpha[u] + ((p[0] + p[1]) + (p[2] + p[3]));
+            pf[u] = pack16<BF16>(p[0], p[1]);       // rounded to the type of v: what tensor cores multiply
+            pf[u + 2] = pack16<BF16>(p[2], p[3]);
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < DP / 8; d++) {
+                o[d][0] *= alpha[0]; o[d][1] *= alpha[0];
+                o[d][2] *= alpha[1]; o[d][3] *= alpha[1];
+            }
+        }
+        const uint32_t sv = s + KT * RB;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            uint32_t vf[4];   // keys 0-7 / 8-15 of dims 16 k .. 16 k + 7, then of the next 8 dims
+            ldsm4t(vf, sv + (lane & 15) * RB + k * 32 + (lane >> 4) * 16);
+            mma16816<BF16>(o[2 * k], pf, vf[0], vf[1]);
+            mma16816<BF16>(o[2 * k + 1], pf, vf[2], vf[3]);
+        }
+        __syncwarp();   // the stage is read before the next round refills it
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();   // the ring is free: join the warps through it
+    float* so = reinterpret_cast<float*>(smem);                    // [WARPS][16][DP]
+    float2* sml = reinterpret_cast<float2*>(so + WARPS * 16 * DP);  // [WARPS][16]
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+        if ((lane & 3) == 0) sml[warp * 16 + qr + 8 * u] = make_float2(m[u], l[u]);
+#pragma unroll
+        for (int d = 0; d < DP / 8; d++)
+            *reinterpret_cast<float2*>(so + (warp * 16 + qr + 8 * u) * DP + d * 8 + qc) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
+    }
+    __syncthreads();
+    for (int r = warp; r < 16 && blk * 16 + r < rows; r += WARPS) {
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, sml[w * 16 + r].x);
+        const float base = mm == -INFINITY ? 0.0f : mm;
+        float ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float2 ml = sml[w * 16 + r];
+            const float f = ex2_approx(ml.x - base);
+            ll += ml.y * f;
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (lane + 32 * u < DP) acc[u] += so[(w * 16 + r) * DP + lane + 32 * u] * f;
+        }
+        const int gr = blk * 16 + r, i = gr / c.g, h = hk * c.g + gr % c.g;
+        if (c.nsplit == 1) {
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+            for (int u = 0; u < 4; u++) acc[u] = ll == 0.0f ? 0.0f : acc[u] * inv;
+            write_row<BF16>(c, b, h, i, acc);
+        } else {
+            const long long all = (long long)a.B * a.Sq * a.Hq;
+            const long long id = split * all + ((long long)b * a.Sq + i) * a.Hq + h;
+            if (lane == 0) c.mlpart[id] = make_float2(mm, ll);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (lane + 32 * u < a.D) c.opart[id * a.D + lane + 32 * u] = acc[u];
+        }
+    }
+}
+
+// Joins the splits of one row per warp, in split order.
+template <bool BF16>
+__global__ void __launch_bounds__(128) attn_combine_kernel(const __grid_constant__ AttnCall c) {
+    griddep_wait();
+    griddep_launch();
+    const mgc_attention_args& a = c.a;
+    const int lane = threadIdx.x & 31;
+    const long long all = (long long)a.B * a.Sq * a.Hq, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (id >= all) return;
+    float mm = -INFINITY;
+    for (int s = lane; s < c.nsplit; s += 32) mm = fmaxf(mm, c.mlpart[s * all + id].x);
+    for (int k = 16; k; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
+    const float base = mm == -INFINITY ? 0.0f : mm;
+    float ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = 0; s < c.nsplit; s++) {
+        const float2 ml = c.mlpart[s * all + id];
+        const float f = ex2_approx(ml.x - base);
+        ll += ml.y * f;
+        const float* o = c.opart + (s * all + id) * a.D;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (lane + 32 * u < a.D) acc[u] = fmaf(o[lane + 32 * u], f, acc[u]);
+    }
+    const float inv = 1.0f / ll;
+#pragma unroll
+    for (int u = 0; u < 4; u++) acc[u] = ll == 0.0f ? 0.0f : acc[u] * inv;
+    const int h = (int)(id % a.Hq);
+    const long long bi = id / a.Hq;
+    write_row<BF16>(c, (int)(bi / a.Sq), h, (int)(bi % a.Sq), acc);
+}
+
+template <bool BF16, int DP>
+void launch_step(const AttnCall& c, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto kernel = attn_step_kernel<BF16, DP>;
+    allow_smem(kernel, smem_bytes<DP>(), done);
+    const long long blocks = (long long)c.a.B * c.a.Hkv * ((c.a.Sq * c.g + 15) / 16) * c.nsplit;
+    if (blocks > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
+    ++g_launch_count;
+    const cudaError_t e = launch_k(kernel, dim3((unsigned)blocks), dim3(WARPS * 32), smem_bytes<DP>(), st, c);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+}
+
+template <bool BF16>
+void dispatch_step(const AttnCall& c, cudaStream_t st) {
+    switch ((c.a.D + 15) / 16) {
+        case 1: launch_step<BF16, 16>(c, st); break;
+        case 2: launch_step<BF16, 32>(c, st); break;
+        case 3: launch_step<BF16, 48>(c, st); break;
+        case 4: launch_step<BF16, 64>(c, st); break;
+        case 5: launch_step<BF16, 80>(c, st); break;
+        case 6: launch_step<BF16, 96>(c, st); break;
+        case 7: launch_step<BF16, 112>(c, st); break;
+        default: launch_step<BF16, 128>(c, st); break;
+    }
+}
+
+}  // namespace
+
+void launch_attn_step(const AttnCall& c, cudaStream_t st) {
+    if (c.a.dtype == MGC_BF16) dispatch_step<true>(c, st);
+    else dispatch_step<false>(c, st);
+}
+
+void launch_attn_combine(const AttnCall& c, cudaStream_t st) {
+    const long long all = (long long)c.a.B * c.a.Sq * c.a.Hq, blocks = (all + 3) / 4;
+    if (blocks > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
+    ++g_launch_count;
+    const cudaError_t e = c.a.dtype == MGC_BF16
+                              ? launch_k(attn_combine_kernel<true>, dim3((unsigned)blocks), dim3(128), 0, st, c)
+                              : launch_k(attn_combine_kernel<false>, dim3((unsigned)blocks), dim3(128), 0, st, c);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+}
+
+}  // namespace mgc

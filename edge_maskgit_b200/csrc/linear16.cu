@@ -1,0 +1,414 @@
+// linear16.cu -- mgc_linear: y = act(x W^T + bias) + resid in f16 / bf16 on tcgen05 tensor cores.
+//
+// Both kernels compute the transposed product: W's rows are the MMA's M axis (TMEM lanes) and x's
+// rows its N axis (TMEM columns).  A warp then holds 32 consecutive outputs n of one row m in its
+// lanes, so results, residual and bias move between registers and memory in consecutive addresses
+// without a staging tile, whatever the alignment of y's rows, and a call with few rows (one token)
+// wastes columns of a narrow tile instead of 127 lanes of a wide one.
+//
+// Operands come by tensor maps with the 128-byte swizzle, 64 k at a time; what lies outside the
+// tensors reads as zero, so K, N and M need no padding.
+#include <algorithm>
+#include <atomic>
+
+#include "../../include/mgc.h"
+#include "kernels.h"
+#include "tma.cuh"
+
+namespace mgc {
+namespace {
+
+constexpr int BK = 64;         // k per stage: one 128-byte swizzle row
+constexpr int TILE_N = 128;    // outputs n per CTA (TMEM lanes)
+constexpr uint32_t A_BYTES = TILE_N * BK * 2;
+
+struct LinArgs {
+    int M, N, K;
+    const float* bias;
+    const void* resid; long long ldr;
+    void* y; long long ldy;
+    int act;
+};
+
+__device__ __forceinline__ float act16(float v, int a) {
+    if (a == 1) return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    if (a == 2) return v / (1.0f + __expf(-v));
+    return v;
+}
+
+// Columns [c0, c0 + 32) of the accumulator at TMEM address t (this warp's lanes): x rows m0 + c0 +
+// j, output n of this lane.
+template <bool BF16>
+__device__ __forceinline__ void finish_cols(const uint32_t (&acc)[32], const LinArgs& a, int m, int n, float bias) {
+    float res[32];
+    if (a.resid) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) res[j] = m + j < a.M ? load16<BF16>(a.resid, (m + j) * a.ldr + n) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j++) {
+        float v = act16(__uint_as_float(acc[j]) + bias, a.act);
+        if (a.resid) v += res[j];
+        if (m + j < a.M) store16<BF16>(a.y, (m + j) * a.ldy + n, v);
+    }
+}
+
+// ------------------------------------------------------------------ few rows or few tiles
+// One 128 n x BN m tile, its k range split over the CTAs of a cluster so that a small product
+// still reads its weight with every SM.  The partial sums meet in distributed shared memory and
+// are added in rank order: no workspace, no atomics, one launch.
+namespace ls {
+constexpr int THREADS = 192;   // warp 0 copies, warp 1 issues MMAs, warps 2-5 read the result
+template <int BN> constexpr int stages() { return BN <= 32 ? 5 : BN <= 64 ? 8 : 6; }
+template <int BN> constexpr uint32_t stage_bytes() { return A_BYTES + BN * BK * 2; }
+template <int BN> constexpr uint32_t ring() { return stages<BN>() * stage_bytes<BN>(); }
+template <int BN> constexpr uint32_t smem() { return 1024 + ring<BN>() + 256; }
+}  // namespace ls
+
+template <bool BF16, int BN>
+__global__ void __launch_bounds__(ls::THREADS) linear_split_kernel(const __grid_constant__ CUtensorMap mw,
+                                                                   const __grid_constant__ CUtensorMap mx,
+                                                                   const LinArgs a, int split) {
+    constexpr int ST = ls::stages<BN>();
+    constexpr uint32_t SB = ls::stage_bytes<BN>(), COLS = BN < 32 ? 32 : BN;
+    static_assert((uint32_t)BN * TILE_N * 4 <= ls::ring<BN>(), "the partial tile reuses the ring");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = align1024_smem(smem_raw);
+    uint64_t* full = (uint64_t*)(sm + ls::ring<BN>());
+    uint64_t* empty = full + ST;
+    uint64_t* done = empty + ST;
+    uint32_t* tmem_slot = (uint32_t*)(done + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x % split, tile = blockIdx.x / split;
+    const int ntn = (a.N + TILE_N - 1) / TILE_N;
+    const int n0 = tile % ntn * TILE_N, m0 = tile / ntn * BN;
+    const int ks = (a.K + BK - 1) / BK;
+    const int k0 = (int)((long long)ks * rank / split), nk = (int)((long long)ks * (rank + 1) / split) - k0;
+
+    if (tid == 0) {
+        for (int i = 0; i < ST; i++) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_map(&mw);
+        tma_prefetch_map(&mx);
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, COLS);
+    griddep_wait();
+    griddep_launch();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int i = 0;
+        for (; i < nk; i++) {
+            const int s = i % ST;
+            if (i >= ST && !mbar_wait(empty + s, (i / ST - 1) & 1, abort_flag, 41)) break;
+            mbar_arrive_expect_tx(full + s, SB);
+            tma_load_2d(sm + s * SB, &mw, (k0 + i) * BK, n0, full + s);
+            tma_load_2d(sm + s * SB + A_BYTES, &mx, (k0 + i) * BK, m0, full + s);
+        }
+        if (i < nk) {   // gave up: let the copies in flight land
+            volatile int never = 0;
+            for (int t = std::max(0, i - ST); t < i; t++) mbar_wait(full + t % ST, (t / ST) & 1, &never, 42);
+        }
+    } else if (warp == 1 && lane == 0) {
+        constexpr uint32_t idesc = idesc_make(1, BF16, BF16, TILE_N, BN);
+        bool ok = true;
+        for (int i = 0; i < nk; i++) {
+            const int s = i % ST;
+            if (!(ok = mbar_wait(full + s, (i / ST) & 1, abort_flag, 43))) break;
+            tc_fence_after();
+            const uint64_t da = sdesc_sw128(smem_u32(sm + s * SB)), db = sdesc_sw128(smem_u32(sm + s * SB + A_BYTES));
+#pragma unroll
+            for (int k = 0; k < BK / 16; k++) mma_f16(tmem, da + 2 * k, db + 2 * k, idesc, (i | k) != 0);
+            mma_commit(empty + s);
+        }
+        if (ok) mma_commit(done);
+    }
+    // every warp waits for the accumulator: past it nothing reads or writes the ring any more
+    __syncwarp();
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, 44));
+    tc_fence_after();
+    const int quad = warp & 3, n = n0 + quad * 32 + lane;   // warps 2-5: TMEM lanes 32 (warp % 4) ..
+    const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16);
+    const float bias = warp >= 2 && a.bias && n < a.N ? __ldg(a.bias + n) : 0.0f;
+    if (split == 1) {
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 32) {
+                if (m0 + c >= a.M) break;
+                uint32_t acc[32];
+                if (BN >= 32) tmem_ld32(t_row + c, acc);
+                else tmem_ld16(t_row + c, acc);
+                tmem_ld_wait();
+                if (BN < 32) for (int j = 16; j < 32; j++) acc[j] = 0;
+                if (n < a.N) finish_cols<BF16>(acc, a, m0 + c, n, bias);
+            }
+        }
+    } else {
+        float* part = reinterpret_cast<float*>(sm);   // [BN][128 n]
+        const int cols = min(BN, a.M - m0);
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 16) {
+                uint32_t acc[16];
+                tmem_ld16(t_row + c, acc);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; j++) part[(c + j) * TILE_N + quad * 32 + lane] = __uint_as_float(acc[j]);
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        if (warp >= 2 && ok && n < a.N) {
+#pragma unroll 1
+            for (int c = rank; c < cols; c += split) {   // this CTA finishes every split-th column
+                float v = 0.0f;
+                const int m = m0 + c;
+                float res = a.resid ? load16<BF16>(a.resid, m * a.ldr + n) : 0.0f;
+                for (int p = 0; p < split; p++) {
+                    float x;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x)
+                                 : "r"(mapa_u32(part + c * TILE_N + quad * 32 + lane, p)) : "memory");
+                    v += x;
+                }
+                v = act16(v + bias, a.act);
+                if (a.resid) v += res;
+                store16<BF16>(a.y, m * a.ldy + n, v);
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();   // the partial tiles live until every CTA has read them
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, COLS);
+    }
+}
+
+// ------------------------------------------------------------------ many tiles
+// A pair of CTAs owns 256 n x 256 m: each loads its half of both operands (64 KB of a stage's
+// 64 KB arrive once per pair), the even CTA issues M256 x N256 MMAs that read both halves, and each
+// CTA keeps its 128 n x 256 m accumulator in its own TMEM, twice, so that the epilogue of one tile
+// runs under the MMAs of the next.  Persistent over tiles.
+namespace lp {
+constexpr int ST = 6, THREADS = 384;   // warp 0 copies, warp 1 issues MMAs, warps 4-11 read results
+constexpr int TN = 256, TM = 256;
+constexpr uint32_t SB = 2 * A_BYTES, RING = ST * SB, SMEM = 1024 + RING + 256;
+constexpr int GROUP = 8;   // tiles walk 8 m-tiles before the next n-tile: both operands stay in L2
+}  // namespace lp
+
+template <bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lp::THREADS, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const LinArgs a) {
+    using namespace lp;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = align1024_smem(smem_raw);
+    uint64_t* full = (uint64_t*)(sm + RING);   // [ST] even CTA: both CTAs' copies of the stage landed
+    uint64_t* empty = full + ST;               // [ST] the MMAs that read the stage are done
+    uint64_t* acc_full = empty + ST;           // [2]
+    uint64_t* acc_empty = acc_full + 2;        // [2] even CTA: 16 epilogue warps have read it
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int ks = (a.K + BK - 1) / BK;
+    const int ntn = (a.N + TN - 1) / TN, ntm = (a.M + TM - 1) / TM;
+    const int tiles = ntn * ntm;
+    auto tile_at = [&](int t, int& n0, int& m0) {
+        const int per = GROUP * ntn, g = t / per, first = g * GROUP, size = min(GROUP, ntm - first), r = t - g * per;
+        m0 = (first + r % size) * TM;
+        n0 = r / size * TN;
+    };
+
+    if (tid == 0) {
+        for (int i = 0; i < ST; i++) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 16); }
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_map(&mw);
+        tma_prefetch_map(&mx);
+    }
+    if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+    griddep_wait();
+    griddep_launch();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();   // both CTAs' barriers are initialised
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += npairs) {
+            int n0, m0;
+            tile_at(t, n0, m0);
+            for (int k = 0; k < ks; k++, it++) {
+                const int s = it % ST;
+                if (it >= ST && !(ok = mbar_wait(empty + s, (it / ST - 1) & 1, abort_flag, 45))) break;
+                if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * SB);
+                const uint32_t bar = mapa_u32(full + s, 0);
+                tma_load_2d_pair(sm + s * SB, &mw, k * BK, n0 + (int)rank * 128, bar);
+                tma_load_2d_pair(sm + s * SB + A_BYTES, &mx, k * BK, m0 + (int)rank * 128, bar);
+            }
+        }
+        if (!ok && rank == 0) {
+            volatile int never = 0;
+            for (int t = max(0, it - ST); t < it; t++) mbar_wait(full + t % ST, (t / ST) & 1, &never, 42);
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        constexpr uint32_t idesc = idesc_make(1, BF16, BF16, TN, TM);
+        int it = 0, n = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += npairs, n++) {
+            const int b = n & 1;
+            if (n >= 2 && !(ok = mbar_wait(acc_empty + b, (n / 2 - 1) & 1, abort_flag, 46))) break;
+            tc_fence_after();
+            for (int k = 0; k < ks; k++, it++) {
+                const int s = it % ST;
+                if (!(ok = mbar_wait(full + s, (it / ST) & 1, abort_flag, 47))) break;
+                tc_fence_after();
+                const uint64_t da = sdesc_sw128(smem_u32(sm + s * SB)), db = sdesc_sw128(smem_u32(sm + s * SB + A_BYTES));
+#pragma unroll
+                for (int kk = 0; kk < BK / 16; kk++)
+                    mma_f16_pair(tmem + b * TM, da + 2 * kk, db + 2 * kk, idesc, (k | kk) != 0);
+                mma_commit_pair(empty + s);
+            }
+            if (ok) mma_commit_pair(acc_full + b);
+        }
+    } else if (warp >= 4) {
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        int n = 0;
+        for (int t = pair; t < tiles; t += npairs, n++) {
+            const int b = n & 1;
+            int n0, m0;
+            tile_at(t, n0, m0);
+            const int col = n0 + (int)rank * 128 + quad * 32 + lane;
+            const float bias = a.bias && col < a.N ? __ldg(a.bias + col) : 0.0f;
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_full + b, (n / 2) & 1, abort_flag, 48))) break;
+            tc_fence_after();
+            const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16) + b * TM + half * 128;
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+                const int m = m0 + half * 128 + c;
+                if (m >= a.M) break;
+                uint32_t acc[32];
+                tmem_ld32(t_row + c, acc);
+                tmem_ld_wait();
+                if (col < a.N) finish_cols<BF16>(acc, a, m, col, bias);
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_u32(acc_empty + b, 0));
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();   // no CTA leaves while its pair may still signal or read it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------ host
+template <class K, class... Args>
+void launch_cluster(K kernel, unsigned grid, unsigned block, uint32_t smem, unsigned cluster, cudaStream_t st, Args... args) {
+    ++g_launch_count;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster ? 1 : 0;   // 0: the kernel fixes its own
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+    }
+}
+
+CUtensorMap operand_map(const void* p, bool bf16, int rows, int K, long long ld, int box_rows) {
+    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows}, strides[1] = {(uint64_t)ld};
+    const uint32_t box[2] = {BK, (uint32_t)box_rows};
+    return make_map16(p, bf16, 2, dims, strides, box);
+}
+
+template <bool BF16, int BN>
+void run_split(const void* w, long long ldw, const void* x, long long ldx, const LinArgs& a, int split, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto kernel = linear_split_kernel<BF16, BN>;
+    allow_smem(kernel, ls::smem<BN>(), done);
+    const CUtensorMap mw = operand_map(w, BF16, a.N, a.K, ldw, TILE_N), mx = operand_map(x, BF16, a.M, a.K, ldx, BN);
+    const long long tiles = (long long)((a.N + TILE_N - 1) / TILE_N) * ((a.M + BN - 1) / BN);
+    if (tiles * split > 0x7fffffffLL) throw std::runtime_error("M * N is too large for one launch");
+    launch_cluster(kernel, (unsigned)(tiles * split), ls::THREADS, ls::smem<BN>(), split, st, mw, mx, a, split);
+}
+
+template <bool BF16>
+void run_linear(const void* w, long long ldw, const void* x, long long ldx, const LinArgs& a, cudaStream_t st) {
+    const int sms = current_sms();
+    const long long big = (long long)((a.N + lp::TN - 1) / lp::TN) * ((a.M + lp::TM - 1) / lp::TM);
+    if (a.M > 128 && big >= sms / 4) {
+        static std::atomic<uint64_t> done{0};
+        auto kernel = linear_pair_kernel<BF16>;
+        allow_smem(kernel, lp::SMEM, done);
+        const CUtensorMap mw = operand_map(w, BF16, a.N, a.K, ldw, 128), mx = operand_map(x, BF16, a.M, a.K, ldx, 128);
+        if (big > 0x7fffffffLL) throw std::runtime_error("M * N is too large for one launch");
+        const unsigned pairs = (unsigned)std::min<long long>(big, sms / 2);
+        launch_cluster(kernel, 2 * pairs, lp::THREADS, lp::SMEM, 0, st, mw, mx, a);
+        return;
+    }
+    const int bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+    const long long tiles = (long long)((a.N + TILE_N - 1) / TILE_N) * ((a.M + bn - 1) / bn);
+    const int ks = (a.K + BK - 1) / BK;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && ks / (split * 2) >= 2) split *= 2;
+    if (bn == 16) run_split<BF16, 16>(w, ldw, x, ldx, a, split, st);
+    else if (bn == 32) run_split<BF16, 32>(w, ldw, x, ldx, a, split, st);
+    else if (bn == 64) run_split<BF16, 64>(w, ldw, x, ldx, a, split, st);
+    else run_split<BF16, 128>(w, ldw, x, ldx, a, split, st);
+}
+
+}  // namespace
+}  // namespace mgc
+
+using namespace mgc;
+
+extern "C" int mgc_linear(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int M, int N, int K,
+                          const float* bias, int act, const void* resid, int64_t ldr, void* y, int64_t ldy, void* stream) {
+    return guarded("mgc_linear", [&] {
+        auto need = [](bool ok, const char* m) { if (!ok) throw std::invalid_argument(m); };
+        need(dtype == MGC_F16 || dtype == MGC_BF16, "dtype must be F16 or BF16");
+        need(M >= 0 && N >= 0, "negative size");
+        need(K > 0 && K % 8 == 0, "K must be a positive multiple of 8");
+        need(act >= 0 && act <= 2, "act must be 0 (none), 1 (GELU) or 2 (SiLU)");
+        if (M == 0 || N == 0) return;
+        need(x && w && y, "x, w and y must not be NULL");
+        need(((uintptr_t)x | (uintptr_t)w) % 16 == 0, "x and w must be 16-byte aligned");
+        need(((uintptr_t)y | (uintptr_t)resid) % 2 == 0 && (uintptr_t)bias % 4 == 0, "y, resid and bias must be aligned to their type");
+        need((M == 1 || (ldx >= K && ldx % 8 == 0)) && (N == 1 || (ldw >= K && ldw % 8 == 0)),
+             "ldx and ldw must be multiples of 8 and at least K");
+        need(M == 1 || (ldy >= N && (!resid || ldr >= N)), "ldy and ldr must be at least N");
+        LinArgs a{M, N, K, bias, resid, ldr, y, ldy, act};
+        if (dtype == MGC_BF16) run_linear<true>(w, ldw, x, ldx, a, (cudaStream_t)stream);
+        else run_linear<false>(w, ldw, x, ldx, a, (cudaStream_t)stream);
+    });
+}

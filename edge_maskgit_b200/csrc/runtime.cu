@@ -933,11 +933,79 @@ int mgc_transformer_forward_dump(mgc_runtime* rt, const int32_t* tokens, int B, 
     });
 }
 
+}  // extern "C"
+
+namespace {
+// Device copies of mgc_generate_with's controls, for the length of one call.
+struct ControlBuffers {
+    float* pen = nullptr;        // [3]
+    float* bias = nullptr;       // [CB]
+    uint32_t* allowed = nullptr; // [1 or S][words]
+    int words = 0;
+    bool per_position = false;
+
+    ControlBuffers(const mgc_logit_controls* c, int CB, int S) {
+        if (!c) return;
+        try {
+            words = (CB + 31) / 32;
+            if (c->repetition != 1.0f || c->frequency != 0.0f || c->presence != 0.0f) {
+                if (!(c->repetition > 0.0f) || !std::isfinite(c->repetition) || !std::isfinite(c->frequency) ||
+                    !std::isfinite(c->presence))
+                    throw Err("mgc_generate_with: repetition must be positive and all penalties finite");
+                const float p[3] = {c->repetition, c->frequency, c->presence};
+                pen = dupload(p, 3);
+            }
+            if (c->bias) {
+                for (int v = 0; v < CB; v++)
+                    if (!std::isfinite(c->bias[v])) throw Err("mgc_generate_with: bias must be finite (forbid codes with allowed)");
+                bias = dupload(c->bias, CB);
+            }
+            if (c->allowed) {
+                if (c->allowed_rows != 1 && c->allowed_rows != S - 1)
+                    throw Err("mgc_generate_with: allowed_rows must be 1 or n_tokens");
+                per_position = c->allowed_rows != 1;
+                // row 0 of the sequence is the class token, whose logits are never drawn from
+                std::vector<uint32_t> m((size_t)(per_position ? S : 1) * words, ~0u);
+                for (int r = 0; r < c->allowed_rows; r++) {
+                    uint32_t any = 0;
+                    for (int w = 0; w < words; w++) {
+                        const uint32_t last = w == words - 1 && CB % 32 ? (1u << (CB % 32)) - 1 : ~0u;
+                        const uint32_t bits = c->allowed[(size_t)r * words + w];
+                        any |= bits & last;
+                        m[(size_t)(r + (per_position ? 1 : 0)) * words + w] = bits;
+                    }
+                    if (!any) throw Err("mgc_generate_with: a row of allowed allows no code");
+                }
+                allowed = dupload(m.data(), m.size());
+            }
+        } catch (...) { release(); throw; }
+    }
+    ~ControlBuffers() { release(); }
+    ControlBuffers(const ControlBuffers&) = delete;
+    ControlBuffers& operator=(const ControlBuffers&) = delete;
+    void release() { cudaFree(pen); cudaFree(bias); cudaFree(allowed); }
+
+    // rt->logits, in place, on the runtime's stream; the history of an image's rows is its own
+    // tokens as the forward saw them (the mask and class ids are not codes, so they count for none).
+    void adjust(mgc_runtime* rt, int B, int S, int CB) const {
+        if (!pen && !bias && !allowed) return;
+        for (int i = 0; i < B; i++) {
+            float* z = rt->logits + (size_t)i * S * rt->V;
+            if (mgc_logits_adjust(MGC_F32, z, rt->V, S, CB, pen ? rt->tokens + (size_t)i * S : nullptr, 0, S, nullptr, pen, 0,
+                                  bias, 0, allowed, per_position ? words : 0, z, rt->V, rt->st) != 0)
+                throw Err(g_err);
+        }
+    }
+};
+}  // namespace
+
+extern "C" {
+
 // generate() sampling (mg-generate.cpp:24-35 helpers, :53-123 loop) for B independent
 // images; the same libstdc++ mt19937_64 / uniform_real_distribution<double> streams.
-int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_t* seeds, int steps,
-                 float temperature, int32_t* tokens_out) {
-    return guard([&] {
+// controls (may be null): adjust the logits of the codes before every draw.
+static void generate_impl(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_t* seeds, int steps,
+                          float temperature, const mgc_logit_controls* controls, int32_t* tokens_out) {
         if (!rt || B <= 0 || !class_ids || !seeds || !tokens_out || steps <= 0) throw Err("mgc_generate: bad arguments");
         const int CB = rt->codebook, MASK = rt->mask_id, S = rt->n_tokens + 1;
         const size_t vocab = (size_t)rt->V;
@@ -952,6 +1020,7 @@ int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_
         const size_t R = (size_t)B * S;
         CK(cudaSetDevice(rt->device));
         ensure_attn_scratch(rt, B, S);
+        ControlBuffers ctl(controls, CB, S);
         for (int step = 0; step < steps; step++) {
             // forward on the device; the logits stay there (no read-back)
             std::memcpy(rt->h_tokens, tokens.data(), sizeof(int32_t) * R);
@@ -964,7 +1033,9 @@ int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_
                 for (int s = 0; s < S; s++) rt->h_r[(size_t)i * S + s] = u(rng[i]);
             }
             CK(cudaMemcpyAsync(rt->d_r, rt->h_r, sizeof(double) * R, cudaMemcpyHostToDevice, rt->st));
-            launch_sample_codes(rt->logits, (int)R, (int)vocab, CB, rt->d_r, rt->d_sid, rt->d_psid, rt->st);
+            ctl.adjust(rt, B, S, CB);
+            launch_sample_codes(rt->logits, (int)R, (int)vocab, CB, rt->d_r, rt->d_sid, rt->d_psid, rt->st,
+                                ctl.allowed != nullptr);
             CK(cudaMemcpyAsync(rt->h_sid, rt->d_sid, sizeof(int32_t) * R, cudaMemcpyDeviceToHost, rt->st));
             CK(cudaMemcpyAsync(rt->h_psid, rt->d_psid, sizeof(float) * R, cudaMemcpyDeviceToHost, rt->st));
             CK(cudaMemcpyFromSymbolAsync(rt->h_err, g_dev_error, sizeof(int), 0, cudaMemcpyDeviceToHost, rt->st));
@@ -998,7 +1069,16 @@ int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_
             }
         }
         std::memcpy(tokens_out, result.data(), sizeof(int32_t) * B * S);
-    });
+}
+
+int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_t* seeds, int steps,
+                 float temperature, int32_t* tokens_out) {
+    return guard([&] { generate_impl(rt, B, class_ids, seeds, steps, temperature, nullptr, tokens_out); });
+}
+
+int mgc_generate_with(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_t* seeds, int steps,
+                      float temperature, const mgc_logit_controls* controls, int32_t* tokens_out) {
+    return guard([&] { generate_impl(rt, B, class_ids, seeds, steps, temperature, controls, tokens_out); });
 }
 
 int mgc_runtime_kernel_count(const mgc_runtime* rt) { return rt ? rt->last_launches : -1; }

@@ -14,13 +14,14 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import MgcError, check, lib
+from ._lib import AttentionArgs, MgcError, check, lib
+from ._lib import LogitControls as _LogitControls
 
 __all__ = ["CudaRuntime", "VqganDecoder", "QWeight", "MgcError", "pack_q8_0", "pack_q4_k", "dequant", "tp_unique_id",
            "quantize_act", "gemm_f32", "layernorm_affine", "flash_attn", "embed", "device_error",
-           "F32", "Q8_0", "Q4_K"]
+           "linear", "attention", "logits_adjust", "LogitControls", "F32", "F16", "BF16", "Q8_0", "Q4_K"]
 
-F32, Q8_0, Q4_K = 0, 8, 12
+F32, F16, Q8_0, Q4_K, BF16 = 0, 1, 8, 12, 30
 
 
 def _ptr(a) -> C.c_void_p:
@@ -154,6 +155,194 @@ def embed(tok, pos, tokens, B: int, S: int):
     return y
 
 
+# ----------------------------------------------------------------- 16-bit operators
+def _dtype_code(t, name, f32: bool = False) -> int:
+    import torch
+    code = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32 if f32 else None}.get(t.dtype)
+    if code is None:
+        raise MgcError(f"{name} must be {'float32, ' if f32 else ''}float16 or bfloat16, not {t.dtype}")
+    return code
+
+
+def _operand(t, name, dtype, device, shape=None, contiguous: bool = False):
+    """Checks a tensor that goes to the library by its address; None passes."""
+    import torch
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != device or t.device.type != "cuda":
+        raise MgcError(f"{name} must be a CUDA tensor on {device}")
+    if t.dtype != dtype:
+        raise MgcError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise MgcError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise MgcError(f"{name} must be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise MgcError(f"{name} requires a gradient, which this operator does not give (use torch.no_grad())")
+    return t
+
+
+def _rows(t, name):
+    """The row stride of a 2-D tensor whose last axis is contiguous."""
+    if t is None:
+        return 0
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise MgcError(f"{name} must have two axes, the last one contiguous")
+    return t.stride(0)
+
+
+class _on:
+    """Makes `device` current for a call and gives torch's stream there."""
+
+    def __init__(self, device):
+        import torch
+        self._guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
+        self._device = device
+
+    def __enter__(self):
+        import torch
+        if self._guard is not None:
+            self._guard.__enter__()
+        return C.c_void_p(torch.cuda.current_stream(self._device).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def linear(x, w, bias=None, act: int = 0, resid=None, out=None):
+    """y = act(x W^T + bias) + resid in f16 / bf16 (mgc_linear): x [M][K], w [N][K], resid and y
+    [M][N], bias f32 [N]; act 0 none, 1 erf-GELU, 2 SiLU; summed in f32, rounded once.  Rows may be
+    strided; K and the row strides of x and w are multiples of 8.  `out` may be `resid`."""
+    import torch
+    code = _dtype_code(x, "x")
+    dt, dev = x.dtype, x.device
+    _operand(x, "x", dt, dev)
+    _operand(w, "w", dt, dev)
+    ldx, ldw = _rows(x, "x"), _rows(w, "w")
+    (M, K), N = x.shape, w.shape[0]
+    if w.shape[1] != K:
+        raise MgcError(f"x has {K} columns, w has {w.shape[1]}")
+    _operand(bias, "bias", torch.float32, dev, (N,), contiguous=True)
+    _operand(resid, "resid", dt, dev, (M, N))
+    y = torch.empty((M, N), dtype=dt, device=dev) if out is None else _operand(out, "out", dt, dev, (M, N))
+    with _on(dev) as st:
+        check(lib.mgc_linear(code, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, _ptr(bias), act, _ptr(resid),
+                             _rows(resid, "resid"), y.data_ptr(), _rows(y, "out"), st), "linear")
+    return y
+
+
+def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None, dist_bias=None, causal: bool = False,
+              prefix=None, k_len=None, q_pos=None, doc_q=None, doc_k=None, out=None):
+    """Attention with shaped scores in f16 / bf16 (mgc_attention).
+
+    q [B][Sq][Hq][D], k and v [B][Sk][Hkv][D] (D a multiple of 8 up to 128, the last axis
+    contiguous, the other strides multiples of 8) -> out like q.  With p = q_pos[b] + i (default
+    Sk - Sq + i):
+        s = scale * q.k;  cap > 0: s = cap tanh(s / cap);  s -= slopes[h] |p - j|
+        s += dist_bias[h][clamp(j - p, -R, R) + R]     (dist_bias f32 [Hq][2 R + 1])
+    over the keys j < k_len[b] that are j <= p or j < prefix[b] if causal, with doc_q[b][i] ==
+    doc_k[b][j] >= 0 if given.  A query that sees no key gives zeros.  scale defaults to D ** -0.5;
+    slopes f32 [Hq]; prefix, k_len, q_pos int32 [B]; doc_q, doc_k int32 [B][Sq], [B][Sk]."""
+    import torch
+    code = _dtype_code(q, "q")
+    dt, dev = q.dtype, q.device
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _operand(t, name, dt, dev)
+        if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
+            raise MgcError(f"{name} must have four axes, the last one contiguous")
+    B, Sq, Hq, D = q.shape
+    _, Sk, Hkv, _ = k.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise MgcError(f"k and v must be [{B}][Sk][Hkv][{D}], not {list(k.shape)} and {list(v.shape)}")
+    i32, f32 = torch.int32, torch.float32
+    _operand(slopes, "slopes", f32, dev, (Hq,), contiguous=True)
+    reach = 0
+    if dist_bias is not None:
+        if dist_bias.dim() != 2 or dist_bias.shape[0] != Hq or dist_bias.shape[1] % 2 != 1:
+            raise MgcError(f"dist_bias must be [{Hq}][2 R + 1], not {list(dist_bias.shape)}")
+        _operand(dist_bias, "dist_bias", f32, dev, contiguous=True)
+        reach = dist_bias.shape[1] // 2
+    if prefix is not None and not causal:
+        raise MgcError("prefix is for causal attention")
+    for t, name in ((prefix, "prefix"), (k_len, "k_len"), (q_pos, "q_pos")):
+        _operand(t, name, i32, dev, (B,), contiguous=True)
+    _operand(doc_q, "doc_q", i32, dev, (B, Sq), contiguous=True)
+    _operand(doc_k, "doc_k", i32, dev, (B, Sk), contiguous=True)
+    if out is None:
+        out = torch.empty((B, Sq, Hq, D), dtype=dt, device=dev)
+    else:
+        _operand(out, "out", dt, dev, (B, Sq, Hq, D))
+        if out.shape[3] > 1 and out.stride(3) != 1:
+            raise MgcError("out's last axis must be contiguous")
+    args = AttentionArgs(code, B, Sq, Sk, Hq, Hkv, D, bool(causal), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                         out.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3],
+                         D ** -0.5 if scale is None else scale, cap, _ptr(slopes), _ptr(dist_bias), reach, 0,
+                         _ptr(prefix), _ptr(k_len), _ptr(q_pos), _ptr(doc_q), _ptr(doc_k), None, 0)
+    need = C.c_uint64()
+    with _on(dev) as st:
+        check(lib.mgc_attention_workspace(args, need), "attention")
+        if need.value:   # torch's allocator: this stream's (or this capture's) own memory
+            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
+        check(lib.mgc_attention(args, st), "attention")
+    return out
+
+
+def logits_adjust(logits, history=None, hist_len=None, penalties=None, bias=None, allowed=None, out=None):
+    """Penalties for repeated tokens, a bias and a bit mask on logits [R][V] (mgc_logits_adjust).
+
+    For a token that row r's history (its first hist_len[r] values) holds c > 0 times,
+    z = z > 0 ? z / rep : z * rep and z -= freq * c + pres; then z += bias[v], and -inf where bit
+    v % 32 of allowed[v // 32] is 0.  logits f32, f16 or bf16; history int32 [R][L], hist_len int32
+    [R], penalties f32 [R][3] = (rep, freq, pres), bias f32 [R][V], allowed int32 [R][(V + 31) // 32].
+    One-axis history, penalties, bias or allowed are shared by all rows.  `out` may be `logits`."""
+    import torch
+    code = _dtype_code(logits, "logits", f32=True)
+    dt, dev = logits.dtype, logits.device
+    _operand(logits, "logits", dt, dev)
+    ld = _rows(logits, "logits")
+    R, V = logits.shape
+    i32, f32 = torch.int32, torch.float32
+
+    def table(t, name, dtype, width):   # (pointer, row stride), 0 = one row for all
+        if t is None:
+            return None, 0
+        _operand(t, name, dtype, dev)
+        if t.dim() == 1:
+            t = t[None]
+            if t.shape[1] > 1 and t.stride(1) != 1:
+                raise MgcError(f"{name} must be contiguous")
+            stride = 0
+        else:
+            stride = _rows(t, name)
+            if t.shape[0] != R:
+                raise MgcError(f"{name} must have {R} rows, not {t.shape[0]}")
+            if R > 1 and stride != 0 and stride < t.shape[1]:
+                raise MgcError(f"{name}'s rows overlap")
+        if width is not None and t.shape[1] != width:
+            raise MgcError(f"{name} must have {width} columns, not {t.shape[1]}")
+        return t.data_ptr(), (0 if R == 1 else stride)
+
+    hist_p, ld_h = table(history, "history", i32, None)
+    L = 0 if history is None else history.shape[-1]
+    pen_p, ld_p = table(penalties, "penalties", f32, 3)
+    bias_p, ld_b = table(bias, "bias", f32, V)
+    allowed_p, ld_a = table(allowed, "allowed", i32, (V + 31) // 32)
+    _operand(hist_len, "hist_len", i32, dev, (R,), contiguous=True)
+    if (history is None) != (penalties is None):
+        raise MgcError("history and penalties are given together")
+    if hist_len is not None and history is None:
+        raise MgcError("hist_len is for a history")
+    if L == 0:   # an empty history: nothing is repeated
+        hist_p = pen_p = None
+    y = torch.empty((R, V), dtype=dt, device=dev) if out is None else _operand(out, "out", dt, dev, (R, V))
+    with _on(dev) as st:
+        check(lib.mgc_logits_adjust(code, logits.data_ptr(), ld, R, V, hist_p, ld_h, L, _ptr(hist_len), pen_p, ld_p,
+                                    bias_p, ld_b, allowed_p, ld_a, y.data_ptr(), _rows(y, "out"), st), "logits_adjust")
+    return y
+
+
 # ----------------------------------------------------------------- runtime
 @dataclass
 class HParams:
@@ -174,6 +363,35 @@ class OpProfile:   # include/mg-opencl.hpp:17-21
     op: str
     count: int
     ms: float
+
+
+@dataclass
+class LogitControls:
+    """What generate() does to the logits of the codes before each draw (mgc_logit_controls):
+    penalties against the codes an image already holds, a bias [codebook], and allowed codes as
+    truth values [codebook] or, one row per grid cell, [n_tokens][codebook]."""
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    bias: np.ndarray | None = None
+    allowed: np.ndarray | None = None
+
+    def _struct(self, codebook: int):
+        """The C struct and the arrays that must outlive it."""
+        bias = None
+        if self.bias is not None:
+            bias = np.ascontiguousarray(self.bias, np.float32)
+            if bias.shape != (codebook,):
+                raise MgcError(f"bias must have shape [{codebook}], not {list(bias.shape)}")
+        bits, rows = None, 0
+        if self.allowed is not None:
+            a = np.atleast_2d(np.asarray(self.allowed, bool))
+            if a.ndim != 2 or a.shape[1] != codebook:
+                raise MgcError(f"allowed must have {codebook} columns, not shape {list(a.shape)}")
+            rows = a.shape[0]
+            a = np.pad(a, ((0, 0), (0, -codebook % 32)))
+            bits = np.ascontiguousarray(np.packbits(a, axis=1, bitorder="little")).view("<u4")
+        return _LogitControls(self.repetition, self.frequency, self.presence, _ptr(bias), _ptr(bits), rows), (bias, bits)
 
 
 def tp_unique_id() -> bytes:
@@ -280,13 +498,19 @@ class CudaRuntime:
     def stream_handle(self) -> int:
         return int(lib.mgc_runtime_stream(self._h) or 0)
 
-    def generate(self, class_ids, seeds, steps: int = 8, temperature: float = 4.5) -> np.ndarray:
-        """generate() (src/mg-generate.cpp:53-123) for len(class_ids) images -> tokens [B][S]."""
+    def generate(self, class_ids, seeds, steps: int = 8, temperature: float = 4.5,
+                 controls: LogitControls | None = None) -> np.ndarray:
+        """generate() (src/mg-generate.cpp:53-123) for len(class_ids) images -> tokens [B][S].
+        `controls` adjusts the logits before every draw."""
         cls = np.ascontiguousarray(class_ids, dtype=np.int32)
         sd = np.ascontiguousarray(seeds, dtype=np.uint64)
         B = cls.shape[0]
         out = np.empty((B, self.hparams.n_tokens + 1), np.int32)
-        check(lib.mgc_generate(self._h, B, _ptr(cls), _ptr(sd), steps, temperature, _ptr(out)), "generate")
+        if controls is None:
+            check(lib.mgc_generate(self._h, B, _ptr(cls), _ptr(sd), steps, temperature, _ptr(out)), "generate")
+        else:
+            c, _alive = controls._struct(self.hparams.codebook_size)
+            check(lib.mgc_generate_with(self._h, B, _ptr(cls), _ptr(sd), steps, temperature, C.byref(c), _ptr(out)), "generate")
         return out
 
     def generate_images(self, vq: "VqganDecoder", class_ids, seeds, steps: int = 8,

@@ -8,7 +8,8 @@
  *   - stream is a cudaStream_t passed as void* (NULL = the legacy default stream).
  *   - Layouts follow the reference's row-major activation convention x[m*K + k]
  *     (ggml ne = {K, M}); weight bytes are the GGUF Q8_0 / Q4_K blocks unchanged.
- *   - wtype codes are GGML's: 0 = F32, 8 = Q8_0, 12 = Q4_K.
+ *   - wtype codes are GGML's: 0 = F32, 8 = Q8_0, 12 = Q4_K; dtype codes too: 0 = F32, 1 = F16,
+ *     30 = BF16.
  */
 #ifndef MGC_H
 #define MGC_H
@@ -20,8 +21,10 @@ extern "C" {
 #endif
 
 #define MGC_F32 0
+#define MGC_F16 1
 #define MGC_Q8_0 8
 #define MGC_Q4_K 12
+#define MGC_BF16 30
 
 const char* mgc_last_error(void);
 /* Reads and clears the device-side error word written by bounded waits inside kernels
@@ -104,6 +107,77 @@ int mgc_flash_attn(const float* qkv_dev, int B, int S, int H, int Dh, float scal
 int mgc_embed(const float* tok_embd_dev, int vocab, const float* pos_embd_dev, int E,
               const int32_t* tokens_dev, int B, int S, float* out_dev, void* stream);
 
+/* ------------------------------------------------------------------ 16-bit operators
+ * No counterpart in the reference, whose activations are f32: the linear layer and the attention
+ * of a model kept in f16 or bf16, and the adjustment of its logits before a draw.  All three are
+ * enqueued on `stream` of the current device, which must be the device the pointers belong to;
+ * they neither allocate nor synchronise, so they can be captured into a graph.
+ *
+ * Linear layer: y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + resid[m][n], summed in f32 and
+ * rounded once.  x [M][K], w [N][K], resid and y [M][N] are all `dtype` (MGC_F16 or MGC_BF16),
+ * bias f32; bias / resid may be NULL; act 0 none, 1 erf-GELU, 2 SiLU.  ld* are row strides in
+ * elements.  K, ldx and ldw must be multiples of 8, x and w 16-byte aligned; N, ldr and ldy may
+ * be odd.  y may be the buffer of resid (same stride), not of x or w.  M = 0 or N = 0 is a no-op. */
+int mgc_linear(int dtype, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int M, int N, int K,
+               const float* bias_dev, int act, const void* resid_dev, int64_t ldr, void* y_dev, int64_t ldy,
+               void* stream);
+
+/* Attention over whole sequences, prompts or a cache, with shaped scores.  For batch row b, query
+ * head h (which reads key head h / (Hq / Hkv)), query i at position p = q_pos[b] + i and key j:
+ *   s = scale * q.k;  cap > 0: s = cap * tanh(s / cap);  slopes: s -= slopes[h] * |p - j|;
+ *   dist_bias: s += dist_bias[h][clamp(j - p, -dist_range, dist_range) + dist_range]
+ * Key j is seen by query i where all that are given hold:
+ *   j < k_len[b];  causal: j <= p or j < prefix[b];  documents: doc_q[b][i] == doc_k[b][j] >= 0;
+ *   and its score is not -inf (a -inf in dist_bias hides a distance).
+ * out = softmax(s) . v over the seen keys, and zeros for a query that sees none.  What k and v
+ * hold at unseen keys, NaN included, does not reach the result, and keys from k_len[b] on are not
+ * used at all.  Scores, softmax statistics and sums are f32; probabilities are rounded to dtype
+ * for the product with v, as is the result. */
+typedef struct mgc_attention_args {
+    int32_t dtype;              /* MGC_F16 or MGC_BF16: q, k, v and out */
+    int32_t B, Sq, Sk;          /* batch rows, queries and keys per row (Sq, Sk >= 0) */
+    int32_t Hq, Hkv, D;         /* query heads, key heads (Hq % Hkv == 0), head size: 8..128, % 8 == 0 */
+    int32_t causal;             /* 0 or 1 */
+    const void* q;              /* dev [B][Sq][Hq][D], strides below, 16-byte aligned; so are k, v, out */
+    const void* k;              /* dev [B][Sk][Hkv][D] */
+    const void* v;              /* dev [B][Sk][Hkv][D] */
+    void* out;                  /* dev [B][Sq][Hq][D], no overlap with q, k, v */
+    int64_t q_stride[3];        /* elements from one batch row, position and head to the next: >= 0, */
+    int64_t k_stride[3];        /* multiples of 8 (the D axis is contiguous); 0 repeats (not in out) */
+    int64_t v_stride[3];
+    int64_t out_stride[3];
+    float scale;
+    float cap;                  /* 0 = none */
+    const float* slopes;        /* dev [Hq] or NULL */
+    const float* dist_bias;     /* dev [Hq][2 * dist_range + 1] or NULL */
+    int32_t dist_range;         /* >= 0 */
+    int32_t reserved;           /* 0 */
+    const int32_t* prefix;      /* dev [B] or NULL (0); read only where causal */
+    const int32_t* k_len;       /* dev [B] or NULL (Sk); values are clamped to 0..Sk */
+    const int32_t* q_pos;       /* dev [B] or NULL (Sk - Sq: the queries are the last positions) */
+    const int32_t* doc_q;       /* dev [B][Sq] document numbers, with doc_k, or NULL; < 0 = padding */
+    const int32_t* doc_k;       /* dev [B][Sk] */
+    void* workspace;            /* dev, 16-byte aligned, mgc_attention_workspace bytes; the call's own */
+    uint64_t workspace_bytes;   /*   until it has run: calls that may overlap need one each */
+} mgc_attention_args;
+/* Bytes of workspace the call needs (0 = none); reads the sizes and which pointers are NULL. */
+int mgc_attention_workspace(const mgc_attention_args* args, uint64_t* bytes);
+int mgc_attention(const mgc_attention_args* args, void* stream);
+
+/* Adjusts logits before a draw.  Row r of logits [R][V] (dtype MGC_F32, MGC_F16 or MGC_BF16):
+ *   z = z > 0 ? z / rep : z * rep   and   z -= freq * c + pres   for a token that the row's history
+ *   holds c > 0 times;   z += bias[v];   z = -inf where bit v % 32 of allowed[v / 32] is 0,
+ * in f32, rounded once into out [R][V] (the logits' own buffer, or one that does not overlap it).
+ * history int32 [R][L], of which row r uses its first hist_len[r] (NULL: L; clamped to 0..L);
+ * values outside 0..V-1 are skipped.  penalties f32 [R][3]: rep, freq, pres; history and penalties
+ * are given together or both NULL.  bias f32 [R][V], allowed [R][(V + 31) / 32], each may be NULL.
+ * ld* are row strides in elements; 0 for history, penalties, bias or allowed shares one row among
+ * all (with hist_len still [R]).  R = 0 or V = 0 is a no-op. */
+int mgc_logits_adjust(int dtype, const void* logits_dev, int64_t ld, int R, int V,
+                      const int32_t* history_dev, int64_t ld_history, int L, const int32_t* hist_len_dev,
+                      const float* penalties_dev, int64_t ld_penalties, const float* bias_dev, int64_t ld_bias,
+                      const uint32_t* allowed_dev, int64_t ld_allowed, void* out_dev, int64_t ld_out, void* stream);
+
 /* ------------------------------------------------------------------ runtime
  * The CUDA counterpart of mg::OpenCLRuntime (include/mg-opencl.hpp:23-58) specialised to
  * the MaskGIT transformer graph of src/mg-transformer.cpp:32-111. */
@@ -156,6 +230,17 @@ void* mgc_runtime_stream(mgc_runtime* rt);
  * tokens_out host [B][S] = the final sampled sequence (class token first). */
 int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_t* seeds,
                  int steps, float temperature, int32_t* tokens_out);
+
+/* mgc_generate with its logits adjusted (mgc_logits_adjust) before every draw.  All host pointers. */
+typedef struct mgc_logit_controls {
+    float repetition, frequency, presence;   /* against the codes an image already holds; 1, 0, 0 = none */
+    const float* bias;                       /* [codebook] added to every position's logits, or NULL */
+    const uint32_t* allowed;                 /* [allowed_rows][(codebook + 31) / 32] bit masks, or NULL */
+    int32_t allowed_rows;                    /* 1: one mask for every position; n_tokens: one each (a
+                                                region's own codes).  Each must allow a code. */
+} mgc_logit_controls;
+int mgc_generate_with(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_t* seeds,
+                      int steps, float temperature, const mgc_logit_controls* controls, int32_t* tokens_out);
 
 /* Number of kernels the runtime's last forward enqueued (all are this library's own). */
 int mgc_runtime_kernel_count(const mgc_runtime* rt);
