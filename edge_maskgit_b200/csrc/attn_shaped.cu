@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "attn_shaped.cuh"
+#include "attn_tile.cuh"
 
 namespace mgc {
 namespace {
@@ -10,8 +10,29 @@ namespace {
 struct Plan {
     AttnCall c{};
     bool tile = false;          // the 128-row tcgen05 kernel
-    uint64_t opart_bytes = 0, bytes = 0;
+    at::TileCall t{};
+    uint64_t doc_bytes = 0, opart_bytes = 0, bytes = 0;   // workspace: document ranges, partials, (max, sum)
 };
+
+// Lowest and highest document number of every 128-key tile.
+__global__ void __launch_bounds__(128) doc_range_kernel(const int32_t* __restrict__ doc, int Sk, int nkt, int2* out) {
+    griddep_wait();
+    griddep_launch();
+    __shared__ int2 part[4];
+    const int kt = blockIdx.x % nkt, b = blockIdx.x / nkt, j = kt * 128 + threadIdx.x;
+    const int d = j < Sk ? __ldg(doc + (long long)b * Sk + j) : 0;
+    int mn = j < Sk ? d : INT_MAX, mx = j < Sk ? d : INT_MIN;
+    for (int k = 16; k; k >>= 1) {
+        mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, k));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+    }
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_int2(mn, mx);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 4; w++) { mn = min(mn, part[w].x); mx = max(mx, part[w].y); }
+        out[blockIdx.x] = make_int2(mn, mx);
+    }
+}
 
 void check(const mgc_attention_args& a) {
     auto need = [](bool ok, const char* m) { if (!ok) throw std::invalid_argument(m); };
@@ -60,21 +81,72 @@ Plan plan(const mgc_attention_args& args) {
     p.c.chunk = std::max(16, (a.Sk + 15) / 16 * 16);
     if (a.B == 0 || a.Sq == 0) return p;
     const int rows = a.Sq * p.c.g, sms = current_sms();
-    const long long heads = (long long)a.B * a.Hkv * ((rows + 15) / 16);
-    const long long want = std::max<long long>(1, (4LL * sms + heads - 1) / heads);
-    long long chunk = ((a.Sk + want - 1) / want + 63) / 64 * 64;
-    chunk = std::max<long long>(128, std::min<long long>(1024, chunk));
-    if (heads >= 4LL * sms && a.Sk <= 4096) chunk = (a.Sk + 63) / 64 * 64;
-    if (a.Sk > chunk) {
-        p.c.chunk = (int)chunk;
-        p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);
+    // A position stride of 0 (one key repeated) has no tensor map; the other kernel takes any.
+    const bool maps = a.Sk > 0 && (a.Sq == 1 || a.q_stride[1] > 0) && (a.Sk == 1 || (a.k_stride[1] > 0 && a.v_stride[1] > 0));
+    p.tile = maps && a.Sq >= 32;
+    if (p.tile) {
+        const long long heads = (long long)a.B * a.Hq;
+        const int nkt = (a.Sk + at::KT - 1) / at::KT, nqt = (a.Sq + at::QT - 1) / at::QT;
+        at::TileCall& t = p.t;
+        t.tiles_per_cta = heads * ((nqt + 1) / 2) >= sms ? 2 : 1;
+        t.qblocks = (nqt + t.tiles_per_cta - 1) / t.tiles_per_cta;
+        t.q_outer = a.causal;
+        const long long ctas = heads * t.qblocks;
+        const int split = (int)std::max<long long>(1, std::min<long long>(sms / ctas, nkt / 4));
+        const int per = (nkt + split - 1) / split;
+        p.c.chunk = per * at::KT;
+        p.c.nsplit = (nkt + per - 1) / per;
+        for (int i = 0; i < 3; i += 2) {
+            t.qmul[i] = a.q_stride[i] != 0;
+            t.kmul[i] = a.k_stride[i] != 0;
+            t.vmul[i] = a.v_stride[i] != 0;
+        }
+        if (a.doc_k) p.doc_bytes = ((uint64_t)a.B * nkt * sizeof(int2) + 15) / 16 * 16;
+    } else {
+        const long long heads = (long long)a.B * a.Hkv * ((rows + 15) / 16);
+        const long long want = std::max<long long>(1, (4LL * sms + heads - 1) / heads);
+        long long chunk = ((a.Sk + want - 1) / want + 63) / 64 * 64;
+        chunk = std::max<long long>(128, std::min<long long>(1024, chunk));
+        if (heads >= 4LL * sms && a.Sk <= 4096) chunk = (a.Sk + 63) / 64 * 64;
+        if (a.Sk > chunk) {
+            p.c.chunk = (int)chunk;
+            p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);
+        }
     }
+    p.bytes = p.doc_bytes;
     if (p.c.nsplit > 1) {
         const uint64_t all = (uint64_t)a.B * a.Sq * a.Hq * p.c.nsplit;
         p.opart_bytes = (all * a.D * 4 + 15) / 16 * 16;
-        p.bytes = p.opart_bytes + all * 8;
+        p.bytes += p.opart_bytes + all * 8;
     }
     return p;
+}
+
+CUtensorMap operand_map(const void* p, bool bf16, int D, int S, int H, int B, const int64_t* stride) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)S, (uint64_t)H, (uint64_t)B};
+    const uint64_t strides[3] = {(uint64_t)stride[1], (uint64_t)stride[2], (uint64_t)stride[0]};
+    const uint32_t box[4] = {64, 128, 1, 1};
+    return make_map16(p, bf16, 4, dims, strides, box);
+}
+
+void run_tile(Plan& p, cudaStream_t st) {
+    const mgc_attention_args& a = p.c.a;
+    const bool bf16 = a.dtype == MGC_BF16;
+    if (a.doc_k) {
+        const int nkt = (a.Sk + at::KT - 1) / at::KT;
+        int2* range = reinterpret_cast<int2*>(a.workspace);
+        if ((long long)a.B * nkt > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
+        ++g_launch_count;
+        const cudaError_t e = launch_k(doc_range_kernel, dim3((unsigned)(a.B * nkt)), dim3(128), 0, st, a.doc_k, a.Sk, nkt, range);
+        if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+        p.t.doc_range = range;
+    }
+    p.t.c = p.c;
+    const CUtensorMap mq = operand_map(a.q, bf16, a.D, a.Sq, a.Hq, a.B, a.q_stride);
+    const CUtensorMap mk = operand_map(a.k, bf16, a.D, a.Sk, a.Hkv, a.B, a.k_stride);
+    const CUtensorMap mv = operand_map(a.v, bf16, a.D, a.Sk, a.Hkv, a.B, a.v_stride);
+    (bf16 ? (a.D <= 64 ? at::launch_tile_bf16_64 : at::launch_tile_bf16_128)
+          : (a.D <= 64 ? at::launch_tile_f16_64 : at::launch_tile_f16_128))(mq, mk, mv, p.t, st);
 }
 
 }  // namespace
@@ -100,11 +172,13 @@ int mgc_attention(const mgc_attention_args* args, void* stream) {
         if (p.bytes) {
             if (!args->workspace || ((uintptr_t)args->workspace & 15) || args->workspace_bytes < p.bytes)
                 throw std::invalid_argument("workspace must be 16-byte aligned and hold mgc_attention_workspace() bytes");
-            p.c.opart = reinterpret_cast<float*>(args->workspace);
-            p.c.mlpart = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(args->workspace) + p.opart_bytes);
+            uint8_t* ws = reinterpret_cast<uint8_t*>(args->workspace);
+            p.c.opart = reinterpret_cast<float*>(ws + p.doc_bytes);
+            p.c.mlpart = reinterpret_cast<float2*>(ws + p.doc_bytes + p.opart_bytes);
         }
         const cudaStream_t st = (cudaStream_t)stream;
-        launch_attn_step(p.c, st);
+        if (p.tile) run_tile(p, st);
+        else launch_attn_step(p.c, st);
         if (p.c.nsplit > 1) launch_attn_combine(p.c, st);
     });
 }

@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const __grid_constant
 #pragma unroll 4
     for (int s = 0; s < c.nsplit; s++) {
         const float2 ml = c.mlpart[s * all + id];
+        if (ml.x == -INFINITY) continue;   // nothing seen in this split
         const float f = ex2_approx(ml.x - base);
         ll += ml.y * f;
         const float* o = c.opart + (s * all + id) * a.D;

@@ -1,0 +1,507 @@
+// attn_tile.cuh -- mgc_attention for many queries, on tcgen05 tensor cores.
+//
+// One CTA owns up to two 128-query tiles of one head and walks the key tiles (128 keys) that any of
+// its rows sees.  Copies, products and softmax run in separate warps:
+//   warp 8   loads Q once, then K and V tiles through two rings (tensor maps, 128-byte swizzle)
+//   warp 9   issues S = Q K^T into TMEM and, once P is there, O += P V with P read from TMEM
+//   warps 0-3, 4-7   the softmax of query tile 0 and 1: one thread owns one row, so the running
+//            maximum and sum need no exchange between threads (warps 10, 11 only complete a
+//            warpgroup, whose registers move together)
+// P (16 bits) overwrites the first half of its S.  While one tile's softmax runs, the tensor cores
+// work on the other's products.  The output is rescaled in TMEM only when a row's maximum has grown
+// by more than 2^8 since its last rescale: until then probabilities are relative to the old
+// maximum, which costs no precision in floating point.
+#pragma once
+#include <climits>
+
+#include "attn_shaped.cuh"
+
+namespace mgc {
+namespace at {
+
+constexpr int QT = 128, KT = 128, THREADS = 384;
+constexpr uint32_t SLAB = 128 * 128;   // 128 rows of 64 16-bit values
+template <int DP> constexpr uint32_t tile_bytes() { return SLAB * (DP / 64); }
+template <int DP> constexpr int kv_stages() { return DP == 64 ? 3 : 2; }
+constexpr uint32_t OFF_TABLE = 0;                        // [2 tiles][2 buffers][256] f32 bias by distance
+constexpr uint32_t OFF_DOC = OFF_TABLE + 4 * 256 * 4;    // [2][2][128] int32 document numbers
+constexpr uint32_t OFF_BAR = OFF_DOC + 4 * 128 * 4, OFF_TILES = OFF_BAR + 512;   // (from a 1024-byte boundary)
+static_assert(OFF_TILES % 512 == 0, "");
+constexpr uint32_t HEAD = (OFF_TILES + 1023) / 1024 * 1024;
+template <int DP> constexpr uint32_t smem() { return 1024 + HEAD + (2 + 2 * kv_stages<DP>()) * tile_bytes<DP>(); }
+constexpr uint32_t TM_O = 256;   // TMEM columns: S0 | S1 | O0 | O1
+
+enum Mode { CAP = 1, SLOPE = 2, TABLE = 4 };
+
+struct TileCall {
+    AttnCall c;
+    int tiles_per_cta;      // 1 or 2 query tiles
+    int qblocks;            // CTAs along the queries
+    int q_outer;            // 1: the last queries of every head first (causal: the long rows first)
+    const int2* doc_range;  // [B][key tiles] lowest and highest document number of a tile, or null
+    int kmul[3], vmul[3], qmul[3];   // 0 where a stride is 0 (batch, -, head): the map has one entry there
+};
+
+template <bool BF16, int DP, int MODE>
+__global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_constant__ CUtensorMap mq,
+                                                               const __grid_constant__ CUtensorMap mk,
+                                                               const __grid_constant__ CUtensorMap mv,
+                                                               const __grid_constant__ TileCall tc) {
+    constexpr int NST = kv_stages<DP>(), NSLAB = DP / 64;
+    constexpr uint32_t TB = tile_bytes<DP>();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = align1024_smem(smem_raw);
+    uint8_t* sQ = sm + HEAD;
+    uint8_t* sK = sQ + 2 * TB;
+    uint8_t* sV = sK + NST * TB;
+    uint64_t* bars = (uint64_t*)(sm + OFF_BAR);
+    uint64_t* q_full = bars;               // [2] a query tile landed
+    uint64_t* k_full = bars + 2;           // [NST]
+    uint64_t* k_empty = k_full + NST;
+    uint64_t* v_full = k_empty + NST;
+    uint64_t* v_empty = v_full + NST;
+    uint64_t* s_full = v_empty + NST;      // [2] S is in TMEM, and the product before it is done
+    uint64_t* p_full = s_full + 2;         // [2] P is in TMEM (4 warps)
+    uint64_t* o_full = p_full + 2;         // [2] the last product is done
+    uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    int* range = (int*)(tmem_slot + 2);    // lo0, lo1, hi0, hi1, then a tile's lowest / highest document
+
+    const AttnCall& c = tc.c;
+    const mgc_attention_args& a = c.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x % c.nsplit;
+    long long rest = blockIdx.x / c.nsplit;
+    int qb, h, b;
+    if (tc.q_outer) {
+        h = (int)(rest % a.Hq); rest /= a.Hq;
+        b = (int)(rest % a.B);
+        qb = tc.qblocks - 1 - (int)(rest / a.B);
+    } else {
+        qb = (int)(rest % tc.qblocks); rest /= tc.qblocks;
+        h = (int)(rest % a.Hq);
+        b = (int)(rest / a.Hq);
+    }
+    const int hk = h / c.g, q0 = qb * tc.tiles_per_cta * QT;
+    const RowBounds rb = row_bounds(a, b);
+    const int nkt = (a.Sk + KT - 1) / KT;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(q_full + i, 1); mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(o_full + i, 1);
+        }
+        for (int i = 0; i < NST; i++) {
+            mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_map(&mq); tma_prefetch_map(&mk); tma_prefetch_map(&mv);
+    }
+    if (tid < 2) {
+        range[tid] = INT_MAX; range[2 + tid] = 0; range[4 + tid] = INT_MAX; range[6 + tid] = -1;
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    griddep_wait();
+    griddep_launch();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    // ---- the key tiles [lo, hi) of each query tile
+    const int kt_first = split * (c.chunk / KT), kt_last = min(nkt, kt_first + c.chunk / KT);
+    int lo[2], hi[2];
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        const int first = q0 + w * QT, last = min(first + QT, a.Sq) - 1;
+        lo[w] = kt_first;
+        hi[w] = w < tc.tiles_per_cta && last >= first
+                    ? max(lo[w], min(kt_last, (key_end(rb, rb.pos0 + last) + KT - 1) / KT)) : lo[w];
+    }
+    if (a.doc_q) {   // only tiles that share a document number with the queries (sorted or not)
+        if (warp < 8) {
+            const int w = warp >> 2, i = q0 + w * QT + (tid & 127);
+            const int d = w < tc.tiles_per_cta && i < a.Sq ? __ldg(a.doc_q + (long long)b * a.Sq + i) : -1;
+            int mn = d >= 0 ? d : INT_MAX, mx = d;
+            for (int k = 16; k; k >>= 1) {
+                mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, k));
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+            }
+            if (lane == 0) { atomicMin(range + 4 + w, mn); atomicMax(range + 6 + w, mx); }
+        }
+        __syncthreads();
+        for (int kt = kt_first + tid; kt < kt_last; kt += THREADS) {
+            const int2 r = __ldg(tc.doc_range + (long long)b * nkt + kt);
+#pragma unroll
+            for (int w = 0; w < 2; w++)
+                if (r.y >= range[4 + w] && r.x <= range[6 + w]) { atomicMin(range + w, kt); atomicMax(range + 2 + w, kt + 1); }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            lo[w] = max(lo[w], range[w]);
+            hi[w] = min(hi[w], range[2 + w]);
+        }
+    }
+    const bool on[2] = {hi[0] > lo[0], hi[1] > lo[1]};
+    const int lo_all = min(on[0] ? lo[0] : INT_MAX, on[1] ? lo[1] : INT_MAX);
+    const int hi_all = max(on[0] ? hi[0] : 0, on[1] ? hi[1] : 0);
+    const int n = hi_all > lo_all ? hi_all - lo_all : 0;
+    auto active = [&](int w, int kt) { return on[w] && kt >= lo[w] && kt < hi[w]; };
+
+    // Registers: 384 threads start with 168 each (64512); the 256 softmax threads take 216, the
+    // other warpgroup keeps 72: 256 * 216 + 128 * 72 = 64512, all of the launch's own.
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+
+    if (warp == 8) {
+        // ---------------------------------------------------------------- copies
+        if (lane == 0 && n > 0) {
+            auto load = [&](uint8_t* dst, const CUtensorMap* map, int pos, int head, int batch, uint64_t* bar) {
+                mbar_arrive_expect_tx(bar, TB);
+#pragma unroll
+                for (int s = 0; s < NSLAB; s++) tma_load_4d(dst + s * SLAB, map, s * 64, pos, head, batch, bar);
+            };
+            auto load_q = [&](int w) {
+                if (on[w]) load(sQ + w * TB, &mq, q0 + w * QT, h * tc.qmul[2], b * tc.qmul[0], q_full + w);
+            };
+            bool ok = true;
+            int i = 0;
+            for (; i < n; i++) {
+                const int s = i % NST, par = (i / NST - 1) & 1;
+                if (i == 0) load_q(0);
+                if (i >= NST && !(ok = mbar_wait(k_empty + s, par, abort_flag, 51))) break;
+                load(sK + s * TB, &mk, (lo_all + i) * KT, hk * tc.kmul[2], b * tc.kmul[0], k_full + s);
+                if (i == 0) load_q(1);
+                if (i >= NST && !(ok = mbar_wait(v_empty + s, par, abort_flag, 52))) break;
+                load(sV + s * TB, &mv, (lo_all + i) * KT, hk * tc.vmul[2], b * tc.vmul[0], v_full + s);
+            }
+            if (!ok) {   // gave up: let the copies in flight land (tile i may have K only)
+                volatile int never = 0;
+                for (int w = 0; w < 2; w++) if (on[w]) mbar_wait(q_full + w, 0, &never, 53);
+                for (int t = max(0, i - NST); t <= i; t++) mbar_wait(k_full + t % NST, (t / NST) & 1, &never, 53);
+                for (int t = max(0, i - NST); t < i; t++) mbar_wait(v_full + t % NST, (t / NST) & 1, &never, 53);
+            }
+        }
+    } else if (warp == 9) {
+        // ---------------------------------------------------------------- products
+        if (lane == 0 && n > 0) {
+            const int dsteps = (a.D + 15) / 16;
+            constexpr uint32_t idesc_s = idesc_make(1, BF16, BF16, QT, KT);
+            const uint32_t idesc_o = idesc_make(1, BF16, BF16, QT, (uint32_t)dsteps * 16) | IDESC_B_MN;
+            auto qk = [&](int w, int i) {
+                const uint64_t dq = sdesc_sw128(smem_u32(sQ + w * TB)), dk = sdesc_sw128(smem_u32(sK + (i % NST) * TB));
+                for (int k = 0; k < dsteps; k++) {
+                    const uint64_t off = (uint64_t)(k >> 2) * (SLAB >> 4) + 2 * (k & 3);
+                    mma_f16(tmem + w * KT, dq + off, dk + off, idesc_s, k > 0);
+                }
+                mma_commit(s_full + w);
+            };
+            auto pv = [&](int w, int i, bool first) {
+                const uint64_t dv = sdesc_mn_sw128(smem_u32(sV + (i % NST) * TB), SLAB);
+#pragma unroll
+                for (int k = 0; k < KT / 16; k++)
+                    mma_f16_ts(tmem + TM_O + w * DP, tmem + w * KT + k * 8, dv + (uint64_t)k * (2048 >> 4), idesc_o, !(first && k == 0));
+            };
+            bool ok = true;
+            int np[2] = {0, 0};   // P tiles consumed
+            for (int i = -1; ok && i < n; i++) {
+                const int kt = lo_all + i;
+                if (i + 1 < n && !(ok = mbar_wait(k_full + (i + 1) % NST, ((i + 1) / NST) & 1, abort_flag, 54))) break;
+                bool have_v = false;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    if (i >= 0 && active(w, kt)) {
+                        if (!(ok = mbar_wait(p_full + w, np[w] & 1, abort_flag, 55))) break;
+                        if (!have_v && !(ok = mbar_wait(v_full + i % NST, (i / NST) & 1, abort_flag, 56))) break;
+                        have_v = true;
+                        tc_fence_after();
+                        pv(w, i, np[w] == 0);
+                        np[w]++;
+                        if (kt + 1 == hi[w]) mma_commit(o_full + w);
+                    }
+                    if (active(w, kt + 1) && i + 1 < n) {
+                        if ((w == 0 ? lo[0] : lo[1]) == kt + 1 && !(ok = mbar_wait(q_full + w, 0, abort_flag, 57))) break;
+                        tc_fence_after();
+                        qk(w, i + 1);
+                    }
+                }
+                if (!ok) break;
+                // a tile between the two ranges is used by neither, but its copy has to land
+                if (i >= 0 && !have_v && !(ok = mbar_wait(v_full + i % NST, (i / NST) & 1, abort_flag, 56))) break;
+                if (i >= 0) mma_commit(v_empty + i % NST);
+                if (i + 1 < n) mma_commit(k_empty + (i + 1) % NST);
+            }
+        }
+    } else if (warp < 8) {
+        // ---------------------------------------------------------------- softmax: thread = row
+        const int w = warp >> 2, r = tid & 127;
+        const int i = q0 + w * QT + r, qi = min(i, a.Sq - 1);
+        const int p = rb.pos0 + qi;
+        const ScoreShape sh = score_shape(a, h);
+        const bool live = w < tc.tiles_per_cta && i < a.Sq;
+        // (rows past the last query compute on as copies of it, so that they force no masking)
+        const int doc = a.doc_q ? __ldg(a.doc_q + (long long)b * a.Sq + qi) : 0;
+        const int end = doc >= 0 ? key_end(rb, p) : 0;
+        const bool idle = q0 + w * QT + (warp & 3) * 32 >= a.Sq;   // a warp of such rows only
+        const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t tS = t_row + w * KT, tO = t_row + TM_O + w * DP;
+        float* win = reinterpret_cast<float*>(sm + OFF_TABLE) + w * 512;
+        int* sdoc = reinterpret_cast<int*>(sm + OFF_DOC) + w * 256;
+        const int bar_id = 1 + w;
+        // a scale of 0 must not meet the -inf of a masked score
+        const float c1 = (MODE & CAP) ? sh.c1 : fmaxf(fabsf(sh.c1), 1.17549435e-38f);
+        const uint32_t flip = !(MODE & CAP) && sh.c1 < 0.0f ? 0x80000000u : 0u;   // a negative scale
+        // probabilities are 2^(t - base), base = row maximum - SHIFT: f16 keeps its small ones normal
+        constexpr float SHIFT = BF16 ? 0.0f : 6.0f, SLACK = 8.0f;
+
+        // bias window and documents of key tile kt: fetched a tile ahead
+        float pre_b[2] = {0.0f, 0.0f};
+        int pre_d = 0;
+        auto fetch = [&](int kt) {
+            if (MODE & TABLE) {
+                const int d0 = kt * KT - (rb.pos0 + q0 + w * QT) - 127;   // distance of window entry 0
+#pragma unroll
+                for (int u = 0; u < 2; u++) pre_b[u] = __ldg(sh.table + max(-sh.range, min(sh.range, d0 + r + 128 * u)));
+            }
+            if (a.doc_k) pre_d = kt * KT + r < a.Sk ? __ldg(a.doc_k + (long long)b * a.Sk + kt * KT + r) : -1;
+        };
+        float m = -INFINITY, base = 0.0f, l = 0.0f;   // base: what probabilities are relative to
+        bool ok = true;
+        const int lo_w = lo[w], n_w = on[w] ? hi[w] - lo[w] : 0;
+        if (n_w > 0) fetch(lo_w);
+        for (int x = 0; x < n_w; x++) {
+            const int kt = lo_w + x, buf = x & 1;
+            if ((MODE & TABLE) || a.doc_k) {
+                if (MODE & TABLE) {
+                    win[buf * 256 + r] = bias2(pre_b[0]);
+                    win[buf * 256 + 128 + r] = bias2(pre_b[1]);
+                }
+                if (a.doc_k) sdoc[buf * 128 + r] = pre_d;
+                named_bar_sync(bar_id, 128);
+                if (x + 1 < n_w) fetch(kt + 1);
+            }
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, x & 1, abort_flag, 58));
+            if (!ok) break;
+            tc_fence_after();
+            if (!idle) {
+            uint32_t s[4][32];
+#pragma unroll
+            for (int q = 0; q < 4; q++) tmem_ld32(tS + q * 32, s[q]);
+            tmem_ld_wait();
+            auto S = [&](int j) -> float { return __uint_as_float(s[j >> 5][j & 31]); };
+            auto put = [&](int j, float v) { s[j >> 5][j & 31] = __float_as_uint(v); };
+
+            // ---- shape: S becomes t in base 2 (no cap, no bias: scaled later, in one fma with the max)
+            if (MODE & CAP) {
+#pragma unroll
+                for (int j = 0; j < 128; j++) put(j, capped(S(j), c1, sh.cap2));
+            } else if (flip) {
+#pragma unroll
+                for (int j = 0; j < 128; j++) s[j >> 5][j & 31] ^= flip;
+            }
+            if (MODE & (SLOPE | TABLE)) {
+                const float d0 = (float)(kt * KT - p);
+                const float* wp = win + buf * 256 + 127 - r;
+#pragma unroll
+                for (int j = 0; j < 128; j++) {
+                    float bias = 0.0f;
+                    if (MODE & TABLE) bias = wp[j];
+                    if (MODE & SLOPE) bias = fmaf(-sh.slope2, fabsf(d0 + (float)j), bias);
+                    put(j, (MODE & CAP) ? S(j) + bias : fmaf(S(j), c1, bias));
+                }
+            }
+            // ---- mask
+            const int lim = end - kt * KT;   // keys of the tile below the row's end
+            if (!__all_sync(0xffffffffu, lim >= KT)) {
+#pragma unroll
+                for (int j = 0; j < 128; j++) put(j, j < lim ? S(j) : -INFINITY);
+            }
+            if (a.doc_k) {
+                const int2 dr = __ldg(tc.doc_range + (long long)b * nkt + kt);
+                if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) {
+                    const int4* dk = reinterpret_cast<const int4*>(sdoc + buf * 128);
+#pragma unroll
+                    for (int j = 0; j < 128; j += 4) {
+                        const int4 d = dk[j / 4];
+                        put(j, d.x == doc ? S(j) : -INFINITY);
+                        put(j + 1, d.y == doc ? S(j + 1) : -INFINITY);
+                        put(j + 2, d.z == doc ? S(j + 2) : -INFINITY);
+                        put(j + 3, d.w == doc ? S(j + 3) : -INFINITY);
+                    }
+                }
+            }
+            // ---- maximum (NaN scores are passed over here and reach the sum through 2^x)
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 128; j += 2) {
+                float& y = mx[(j >> 1) & 3];
+                asm("max.f32 %0, %0, %1, %2;" : "+f"(y) : "f"(S(j)), "f"(S(j + 1)));
+            }
+            float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (MODE == 0) tile_max = tile_max == -INFINITY ? tile_max : tile_max * c1;
+            m = fmaxf(m, tile_max);
+            const bool grow = m - SHIFT > base + SLACK || (x == 0 && m != -INFINITY) || (l == 0.0f && m != -INFINITY);
+            if (__any_sync(0xffffffffu, grow)) {
+                float alpha = 1.0f;
+                if (grow) {
+                    const float nb = m - SHIFT;
+                    alpha = l == 0.0f ? 1.0f : ex2_approx(base - nb);
+                    l *= alpha;
+                    base = nb;
+                }
+                if (x > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {   // S arrived after the last product: O is at rest
+#pragma unroll
+                    for (int d = 0; d < DP; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + d, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(tO + d, o);
+                    }
+                }
+            }
+            // ---- probabilities
+            const uint64_t c2 = pack2(MODE == 0 ? c1 : 1.0f, MODE == 0 ? c1 : 1.0f), nb2 = pack2(-base, -base);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    const int j = q * 64 + 2 * e;
+                    const uint64_t t2 = pack2(S(j), S(j + 1));
+                    float t0, t1;
+                    unpack2(MODE == 0 ? fma2(t2, c2, nb2) : add2(t2, nb2), t0, t1);
+                    const float p0 = ex2_approx(t0), p1 = ex2_approx(t1);
+                    sum[e & 1] = add2(sum[e & 1], pack2(p0, p1));
+                    pk[e] = pack16<BF16>(p0, p1);   // rounded to the type of v: what tensor cores multiply
+                }
+                tmem_st32(tS + q * 32, pk);
+            }
+            float s0, s1, s2, s3;
+            unpack2(sum[0], s0, s1);
+            unpack2(sum[1], s2, s3);
+            l += (s0 + s1) + (s2 + s3);
+            }
+            // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
+            if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && active(0, kt))) {
+                const int st = (kt - lo_all) % NST;
+                ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, ((kt - lo_all) / NST) & 1, abort_flag, 59));
+                if (!ok) break;
+                if (r >= rb.len - kt * KT) {
+#pragma unroll
+                    for (int sl = 0; sl < NSLAB; sl++)
+#pragma unroll
+                        for (int ch = 0; ch < 8; ch++)
+                            *reinterpret_cast<uint4*>(sV + st * TB + sl * SLAB + r * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + w);
+        }
+        // ---------------------------------------------------------------- output
+        if (ok && n_w > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, 0, abort_flag, 60));
+        tc_fence_after();
+        if (ok && w < tc.tiles_per_cta && q0 + w * QT + (warp & 3) * 32 < a.Sq) {
+            const bool any = n_w > 0 && l != 0.0f;   // (a NaN sum is not 0)
+            const float inv = any ? 1.0f / l : 0.0f;
+            const long long row = ((long long)b * a.Sq + i) * a.Hq + h, id = (long long)split * a.B * a.Sq * a.Hq + row;
+            if (c.nsplit > 1 && live) c.mlpart[id] = make_float2(any ? base : -INFINITY, l);
+            uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b * a.out_stride[0] + qi * a.out_stride[1] + h * a.out_stride[2];
+            bool bad = false;
+#pragma unroll
+            for (int d = 0; d < DP; d += 32) {
+                if (d >= a.D) break;
+                uint32_t o[32];
+                if (n_w > 0) {
+                    tmem_ld32(tO + d, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    const float v = any ? __uint_as_float(o[e]) : 0.0f;
+                    bad |= d + e < a.D && isnan(v);
+                    o[e] = __float_as_uint(c.nsplit > 1 ? v : v * inv);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (d + e >= a.D || !live) break;
+                    if (c.nsplit > 1) {
+                        float4* op = reinterpret_cast<float4*>(c.opart + id * a.D + d + e);
+                        op[0] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                        op[1] = make_float4(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]), __uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
+                    } else {
+                        uint4 v;
+                        v.x = pack16<BF16>(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+                        v.y = pack16<BF16>(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                        v.z = pack16<BF16>(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]));
+                        v.w = pack16<BF16>(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7]));
+                        *reinterpret_cast<uint4*>(dst + d + e) = v;
+                    }
+                }
+                __syncwarp();
+            }
+            bad = (bad || isnan(l)) && live && c.nsplit == 1;   // (split: the join looks for NaN)
+            unsigned todo = __ballot_sync(0xffffffffu, bad);
+            while (todo) {
+                const int k = __ffs(todo) - 1;
+                todo &= todo - 1;
+                const int row_i = q0 + w * QT + (warp & 3) * 32 + k;
+                float o[4];
+                exact_row<BF16>(a, c.g, b, h, row_i, o);
+                const long long at = b * a.out_stride[0] + row_i * a.out_stride[1] + h * a.out_stride[2];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (lane + 32 * u < a.D) store16<BF16>(a.out, at + lane + 32 * u, o[u]);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <bool BF16, int DP, int MODE>
+void launch_tile(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TileCall& t, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto kernel = attn_tile_kernel<BF16, DP, MODE>;
+    allow_smem(kernel, smem<DP>(), done);
+    const long long grid = (long long)t.qblocks * t.c.a.B * t.c.a.Hq * t.c.nsplit;
+    if (grid > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
+    ++g_launch_count;
+    const cudaError_t e = launch_k(kernel, dim3((unsigned)grid), dim3(THREADS), smem<DP>(), st, mq, mk, mv, t);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+}
+
+template <bool BF16, int DP>
+void dispatch_mode(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TileCall& t, cudaStream_t st) {
+    const mgc_attention_args& a = t.c.a;
+    switch ((a.cap > 0.0f ? CAP : 0) | (a.slopes ? SLOPE : 0) | (a.dist_bias ? TABLE : 0)) {
+        case 0: launch_tile<BF16, DP, 0>(mq, mk, mv, t, st); break;
+        case 1: launch_tile<BF16, DP, 1>(mq, mk, mv, t, st); break;
+        case 2: launch_tile<BF16, DP, 2>(mq, mk, mv, t, st); break;
+        case 3: launch_tile<BF16, DP, 3>(mq, mk, mv, t, st); break;
+        case 4: launch_tile<BF16, DP, 4>(mq, mk, mv, t, st); break;
+        case 5: launch_tile<BF16, DP, 5>(mq, mk, mv, t, st); break;
+        case 6: launch_tile<BF16, DP, 6>(mq, mk, mv, t, st); break;
+        default: launch_tile<BF16, DP, 7>(mq, mk, mv, t, st); break;
+    }
+}
+
+// One translation unit per type (and head size): they compile side by side.
+void launch_tile_f16_64(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);
+void launch_tile_f16_128(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);
+void launch_tile_bf16_64(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);
+void launch_tile_bf16_128(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);
+
+}  // namespace at
+}  // namespace mgc
