@@ -14,23 +14,23 @@ struct Plan {
     uint64_t doc_bytes = 0, opart_bytes = 0, bytes = 0;   // workspace: document ranges, partials, (max, sum)
 };
 
-// Lowest and highest document number of every 128-key tile.
+// Lowest and highest document number of every 128-key tile (TileCall::doc_range).
 __global__ void __launch_bounds__(128) doc_range_kernel(const int32_t* __restrict__ doc, int Sk, int nkt, int2* out) {
     griddep_wait();
     griddep_launch();
     __shared__ int2 part[4];
     const int kt = blockIdx.x % nkt, b = blockIdx.x / nkt, j = kt * 128 + threadIdx.x;
-    const int d = j < Sk ? __ldg(doc + (long long)b * Sk + j) : 0;
-    int mn = j < Sk ? d : INT_MAX, mx = j < Sk ? d : INT_MIN;
+    const int d = j < Sk ? __ldg(doc + (long long)b * Sk + j) : INT_MAX;
+    int mn = d < 0 ? INT_MAX : d, mx = j < Sk ? d : -1;
     for (int k = 16; k; k >>= 1) {
         mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, k));
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, k));
     }
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_int2(mn, mx);
-    __syncthreads();
+    const bool padding = __syncthreads_or(d < 0);
     if (threadIdx.x == 0) {
         for (int w = 1; w < 4; w++) { mn = min(mn, part[w].x); mx = max(mx, part[w].y); }
-        out[blockIdx.x] = make_int2(mn, mx);
+        out[blockIdx.x] = make_int2(padding ? mn | INT_MIN : mn, mx);
     }
 }
 

@@ -38,7 +38,9 @@ struct TileCall {
     int tiles_per_cta;      // 1 or 2 query tiles
     int qblocks;            // CTAs along the queries
     int q_outer;            // 1: the last queries of every head first (causal: the long rows first)
-    const int2* doc_range;  // [B][key tiles] lowest and highest document number of a tile, or null
+    // [B][key tiles] or null: x = lowest number >= 0 of the tile (INT_MAX: none), with the sign bit
+    // set if some are negative; y = the highest
+    const int2* doc_range;
     int kmul[3], vmul[3], qmul[3];   // 0 where a stride is 0 (batch, -, head): the map has one entry there
 };
 
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             const int2 r = __ldg(tc.doc_range + (long long)b * nkt + kt);
 #pragma unroll
             for (int w = 0; w < 2; w++)
-                if (r.y >= range[4 + w] && r.x <= range[6 + w]) { atomicMin(range + w, kt); atomicMax(range + 2 + w, kt + 1); }
+                if (r.y >= range[4 + w] && (r.x & INT_MAX) <= range[6 + w]) { atomicMin(range + w, kt); atomicMax(range + 2 + w, kt + 1); }
         }
         __syncthreads();
 #pragma unroll

@@ -10,6 +10,7 @@ torch is only used for device memory and streams.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -156,58 +157,77 @@ def embed(tok, pos, tokens, B: int, S: int):
 
 
 # ----------------------------------------------------------------- 16-bit operators
-def _dtype_code(t, name, f32: bool = False) -> int:
+# The checks below look at each tensor's type, device and gradient flag in one condition and
+# explain only what failed: a small call is as long as its host side.
+def _codes():
     import torch
-    code = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32 if f32 else None}.get(t.dtype)
-    if code is None:
-        raise MgcError(f"{name} must be {'float32, ' if f32 else ''}float16 or bfloat16, not {t.dtype}")
+    return {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
+
+
+_CODE: dict = {}
+# mgc_attention_args; mgc_attention takes its address
+_ATTN_PACK = struct.Struct("8i4Q12q2f2Q2i5Q2Q")
+assert _ATTN_PACK.size == C.sizeof(AttentionArgs)
+
+
+def _code_of(t, name, f32: bool = False) -> int:
+    if not _CODE:
+        _CODE.update(_codes())
+    code = _CODE.get(getattr(t, "dtype", None))
+    if code is None or (code == F32 and not f32):
+        raise MgcError(f"{name} must be {'float32, ' if f32 else ''}float16 or bfloat16, not {getattr(t, 'dtype', type(t))}")
     return code
 
 
-def _operand(t, name, dtype, device, shape=None, contiguous: bool = False):
-    """Checks a tensor that goes to the library by its address; None passes."""
+def _refuse(t, name, dtype, index):
     import torch
-    if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or t.device != device or t.device.type != "cuda":
-        raise MgcError(f"{name} must be a CUDA tensor on {device}")
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index:
+        raise MgcError(f"{name} must be a CUDA tensor" + (f" on device {index}" if index >= 0 else ""))
     if t.dtype != dtype:
         raise MgcError(f"{name} must be {dtype}, not {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise MgcError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
-    if contiguous and not t.is_contiguous():
-        raise MgcError(f"{name} must be contiguous")
     if t.requires_grad and torch.is_grad_enabled():
         raise MgcError(f"{name} requires a gradient, which this operator does not give (use torch.no_grad())")
+
+
+def _operand(t, name, dtype, index):
+    """Checks a tensor that goes to the library by its address."""
+    if t.__class__.__name__ != "Tensor" or t.dtype is not dtype or index < 0 or t.get_device() != index or t.requires_grad:
+        _refuse(t, name, dtype, index)
     return t
 
 
-def _rows(t, name):
-    """The row stride of a 2-D tensor whose last axis is contiguous."""
+def _vector(t, name, dtype, index, shape):
+    """Address of an optional contiguous tensor of exactly this shape (0 for None)."""
     if t is None:
-        return 0
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise MgcError(f"{name} must have two axes, the last one contiguous")
-    return t.stride(0)
+        return None
+    _operand(t, name, dtype, index)
+    if t.shape != shape or not t.is_contiguous():
+        raise MgcError(f"{name} must be contiguous with shape {list(shape)}, not {list(t.shape)}")
+    return t.data_ptr()
 
 
-class _on:
-    """Makes `device` current for a call and gives torch's stream there."""
+def _matrix(t, name, dtype, index):
+    """Row stride of a 2-D tensor whose last axis is contiguous."""
+    _operand(t, name, dtype, index)
+    if t.dim() != 2:
+        raise MgcError(f"{name} must have two axes, not {t.dim()}")
+    ld, one = t.stride()
+    if one != 1 and t.shape[1] > 1:
+        raise MgcError(f"{name}'s last axis must be contiguous")
+    return ld
 
-    def __init__(self, device):
-        import torch
-        self._guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
-        self._device = device
 
-    def __enter__(self):
-        import torch
-        if self._guard is not None:
-            self._guard.__enter__()
-        return C.c_void_p(torch.cuda.current_stream(self._device).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _call(index, what, fn, *args):
+    """Calls the library on torch's current stream of device `index`, made current for the call."""
+    import torch
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc != 0:
+        check(rc, what)
 
 
 def linear(x, w, bias=None, act: int = 0, resid=None, out=None):
@@ -215,21 +235,38 @@ def linear(x, w, bias=None, act: int = 0, resid=None, out=None):
     [M][N], bias f32 [N]; act 0 none, 1 erf-GELU, 2 SiLU; summed in f32, rounded once.  Rows may be
     strided; K and the row strides of x and w are multiples of 8.  `out` may be `resid`."""
     import torch
-    code = _dtype_code(x, "x")
-    dt, dev = x.dtype, x.device
-    _operand(x, "x", dt, dev)
-    _operand(w, "w", dt, dev)
-    ldx, ldw = _rows(x, "x"), _rows(w, "w")
-    (M, K), N = x.shape, w.shape[0]
-    if w.shape[1] != K:
-        raise MgcError(f"x has {K} columns, w has {w.shape[1]}")
-    _operand(bias, "bias", torch.float32, dev, (N,), contiguous=True)
-    _operand(resid, "resid", dt, dev, (M, N))
-    y = torch.empty((M, N), dtype=dt, device=dev) if out is None else _operand(out, "out", dt, dev, (M, N))
-    with _on(dev) as st:
-        check(lib.mgc_linear(code, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, _ptr(bias), act, _ptr(resid),
-                             _rows(resid, "resid"), y.data_ptr(), _rows(y, "out"), st), "linear")
-    return y
+    code = _code_of(x, "x")
+    dt, index = x.dtype, x.get_device()
+    ldx, ldw = _matrix(x, "x", dt, index), _matrix(w, "w", dt, index)
+    (M, K), (N, Kw) = x.shape, w.shape
+    if Kw != K:
+        raise MgcError(f"x has {K} columns, w has {Kw}")
+    bias_p = _vector(bias, "bias", torch.float32, index, (N,)) if bias is not None else None
+    resid_p, ldr = None, 0
+    if resid is not None:
+        resid_p, ldr = resid.data_ptr(), _matrix(resid, "resid", dt, index)
+        if resid.shape != (M, N):
+            raise MgcError(f"resid must have shape {[M, N]}, not {list(resid.shape)}")
+    if out is None:
+        out, ldy = x.new_empty((M, N)), N
+    else:
+        ldy = _matrix(out, "out", dt, index)
+        if out.shape != (M, N):
+            raise MgcError(f"out must have shape {[M, N]}, not {list(out.shape)}")
+    _call(index, "linear", lib.mgc_linear, code, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, bias_p, act, resid_p, ldr,
+          out.data_ptr(), ldy)
+    return out
+
+
+def _heads(t, name, dtype, index):
+    """Strides of a [batch][position][head][D] tensor."""
+    _operand(t, name, dtype, index)
+    if t.dim() != 4:
+        raise MgcError(f"{name} must have four axes, not {t.dim()}")
+    st = t.stride()
+    if st[3] != 1 and t.shape[3] > 1:
+        raise MgcError(f"{name}'s last axis must be contiguous")
+    return st
 
 
 def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None, dist_bias=None, causal: bool = False,
@@ -245,47 +282,55 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
     doc_k[b][j] >= 0 if given.  A query that sees no key gives zeros.  scale defaults to D ** -0.5;
     slopes f32 [Hq]; prefix, k_len, q_pos int32 [B]; doc_q, doc_k int32 [B][Sq], [B][Sk]."""
     import torch
-    code = _dtype_code(q, "q")
-    dt, dev = q.dtype, q.device
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _operand(t, name, dt, dev)
-        if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
-            raise MgcError(f"{name} must have four axes, the last one contiguous")
+    code = _code_of(q, "q")
+    dt, index = q.dtype, q.get_device()
+    qs, ks, vs = _heads(q, "q", dt, index), _heads(k, "k", dt, index), _heads(v, "v", dt, index)
     B, Sq, Hq, D = q.shape
-    _, Sk, Hkv, _ = k.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+    Bk, Sk, Hkv, Dk = k.shape
+    if k.shape != v.shape or Bk != B or Dk != D:
         raise MgcError(f"k and v must be [{B}][Sk][Hkv][{D}], not {list(k.shape)} and {list(v.shape)}")
-    i32, f32 = torch.int32, torch.float32
-    _operand(slopes, "slopes", f32, dev, (Hq,), contiguous=True)
-    reach = 0
+    i32, reach = torch.int32, 0
+    slopes_p = table_p = prefix_p = k_len_p = q_pos_p = doc_q_p = doc_k_p = None
+    if slopes is not None:
+        slopes_p = _vector(slopes, "slopes", torch.float32, index, (Hq,))
     if dist_bias is not None:
-        if dist_bias.dim() != 2 or dist_bias.shape[0] != Hq or dist_bias.shape[1] % 2 != 1:
-            raise MgcError(f"dist_bias must be [{Hq}][2 R + 1], not {list(dist_bias.shape)}")
-        _operand(dist_bias, "dist_bias", f32, dev, contiguous=True)
-        reach = dist_bias.shape[1] // 2
-    if prefix is not None and not causal:
-        raise MgcError("prefix is for causal attention")
-    for t, name in ((prefix, "prefix"), (k_len, "k_len"), (q_pos, "q_pos")):
-        _operand(t, name, i32, dev, (B,), contiguous=True)
-    _operand(doc_q, "doc_q", i32, dev, (B, Sq), contiguous=True)
-    _operand(doc_k, "doc_k", i32, dev, (B, Sk), contiguous=True)
+        reach = dist_bias.shape[-1] // 2
+        table_p = _vector(dist_bias, "dist_bias", torch.float32, index, (Hq, 2 * reach + 1))
+    if prefix is not None:
+        if not causal:
+            raise MgcError("prefix is for causal attention")
+        prefix_p = _vector(prefix, "prefix", i32, index, (B,))
+    if k_len is not None:
+        k_len_p = _vector(k_len, "k_len", i32, index, (B,))
+    if q_pos is not None:
+        q_pos_p = _vector(q_pos, "q_pos", i32, index, (B,))
+    if doc_q is not None:
+        doc_q_p = _vector(doc_q, "doc_q", i32, index, (B, Sq))
+    if doc_k is not None:
+        doc_k_p = _vector(doc_k, "doc_k", i32, index, (B, Sk))
     if out is None:
-        out = torch.empty((B, Sq, Hq, D), dtype=dt, device=dev)
+        out, os = q.new_empty((B, Sq, Hq, D)), (Sq * Hq * D, Hq * D, D)
     else:
-        _operand(out, "out", dt, dev, (B, Sq, Hq, D))
-        if out.shape[3] > 1 and out.stride(3) != 1:
-            raise MgcError("out's last axis must be contiguous")
-    args = AttentionArgs(code, B, Sq, Sk, Hq, Hkv, D, bool(causal), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                         out.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3],
-                         D ** -0.5 if scale is None else scale, cap, _ptr(slopes), _ptr(dist_bias), reach, 0,
-                         _ptr(prefix), _ptr(k_len), _ptr(q_pos), _ptr(doc_q), _ptr(doc_k), None, 0)
+        os = _heads(out, "out", dt, index)
+        if out.shape != q.shape:
+            raise MgcError(f"out must have shape {list(q.shape)}, not {list(out.shape)}")
+    head = (code, B, Sq, Sk, Hq, Hkv, D, 1 if causal else 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os[0], os[1], os[2],
+            D ** -0.5 if scale is None else scale, cap, slopes_p or 0, table_p or 0, reach, 0, prefix_p or 0, k_len_p or 0,
+            q_pos_p or 0, doc_q_p or 0, doc_k_p or 0)
+    args = _ATTN_PACK.pack(*head, 0, 0)
     need = C.c_uint64()
-    with _on(dev) as st:
-        check(lib.mgc_attention_workspace(args, need), "attention")
-        if need.value:   # torch's allocator: this stream's (or this capture's) own memory
-            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-            args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
-        check(lib.mgc_attention(args, st), "attention")
+    if torch._C._cuda_getDevice() == index:   # (the split follows the device's size)
+        rc = lib.mgc_attention_workspace(args, C.byref(need))
+    else:
+        with torch.cuda.device(index):
+            rc = lib.mgc_attention_workspace(args, C.byref(need))
+    if rc != 0:
+        check(rc, "attention")
+    if need.value:   # from torch's allocator: this stream's (or this capture's) own memory
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        args = _ATTN_PACK.pack(*head, ws.data_ptr(), need.value)
+    _call(index, "attention", lib.mgc_attention, args)
     return out
 
 
@@ -298,49 +343,56 @@ def logits_adjust(logits, history=None, hist_len=None, penalties=None, bias=None
     [R], penalties f32 [R][3] = (rep, freq, pres), bias f32 [R][V], allowed int32 [R][(V + 31) // 32].
     One-axis history, penalties, bias or allowed are shared by all rows.  `out` may be `logits`."""
     import torch
-    code = _dtype_code(logits, "logits", f32=True)
-    dt, dev = logits.dtype, logits.device
-    _operand(logits, "logits", dt, dev)
-    ld = _rows(logits, "logits")
+    code = _code_of(logits, "logits", f32=True)
+    dt, index = logits.dtype, logits.get_device()
+    ld = _matrix(logits, "logits", dt, index)
     R, V = logits.shape
     i32, f32 = torch.int32, torch.float32
 
     def table(t, name, dtype, width):   # (pointer, row stride), 0 = one row for all
-        if t is None:
-            return None, 0
-        _operand(t, name, dtype, dev)
         if t.dim() == 1:
-            t = t[None]
-            if t.shape[1] > 1 and t.stride(1) != 1:
+            _operand(t, name, dtype, index)
+            if t.shape[0] > 1 and t.stride(0) != 1:
                 raise MgcError(f"{name} must be contiguous")
-            stride = 0
+            cols, stride = t.shape[0], 0
         else:
-            stride = _rows(t, name)
-            if t.shape[0] != R:
-                raise MgcError(f"{name} must have {R} rows, not {t.shape[0]}")
-            if R > 1 and stride != 0 and stride < t.shape[1]:
-                raise MgcError(f"{name}'s rows overlap")
-        if width is not None and t.shape[1] != width:
-            raise MgcError(f"{name} must have {width} columns, not {t.shape[1]}")
-        return t.data_ptr(), (0 if R == 1 else stride)
+            stride = _matrix(t, name, dtype, index)
+            rows, cols = t.shape
+            if rows != R:
+                raise MgcError(f"{name} must have {R} rows, not {rows}")
+            if R == 1:
+                stride = 0
+        if cols != width:
+            raise MgcError(f"{name} must have {width} columns, not {cols}")
+        return t.data_ptr(), stride
 
-    hist_p, ld_h = table(history, "history", i32, None)
-    L = 0 if history is None else history.shape[-1]
-    pen_p, ld_p = table(penalties, "penalties", f32, 3)
-    bias_p, ld_b = table(bias, "bias", f32, V)
-    allowed_p, ld_a = table(allowed, "allowed", i32, (V + 31) // 32)
-    _operand(hist_len, "hist_len", i32, dev, (R,), contiguous=True)
+    hist_p = len_p = pen_p = bias_p = allowed_p = None
+    L = ld_h = ld_p = ld_b = ld_a = 0
     if (history is None) != (penalties is None):
         raise MgcError("history and penalties are given together")
-    if hist_len is not None and history is None:
+    if history is not None:
+        L = history.shape[-1]
+        hist_p, ld_h = table(history, "history", i32, L)
+        pen_p, ld_p = table(penalties, "penalties", f32, 3)
+        if hist_len is not None:
+            len_p = _vector(hist_len, "hist_len", i32, index, (R,))
+        if L == 0:   # an empty history: nothing is repeated
+            hist_p = pen_p = None
+    elif hist_len is not None:
         raise MgcError("hist_len is for a history")
-    if L == 0:   # an empty history: nothing is repeated
-        hist_p = pen_p = None
-    y = torch.empty((R, V), dtype=dt, device=dev) if out is None else _operand(out, "out", dt, dev, (R, V))
-    with _on(dev) as st:
-        check(lib.mgc_logits_adjust(code, logits.data_ptr(), ld, R, V, hist_p, ld_h, L, _ptr(hist_len), pen_p, ld_p,
-                                    bias_p, ld_b, allowed_p, ld_a, y.data_ptr(), _rows(y, "out"), st), "logits_adjust")
-    return y
+    if bias is not None:
+        bias_p, ld_b = table(bias, "bias", f32, V)
+    if allowed is not None:
+        allowed_p, ld_a = table(allowed, "allowed", i32, (V + 31) // 32)
+    if out is None:
+        out, ld_o = logits.new_empty((R, V)), V
+    else:
+        ld_o = _matrix(out, "out", dt, index)
+        if out.shape != logits.shape:
+            raise MgcError(f"out must have shape {list(logits.shape)}, not {list(out.shape)}")
+    _call(index, "logits_adjust", lib.mgc_logits_adjust, code, logits.data_ptr(), ld, R, V, hist_p, ld_h, L, len_p, pen_p,
+          ld_p, bias_p, ld_b, allowed_p, ld_a, out.data_ptr(), ld_o)
+    return out
 
 
 # ----------------------------------------------------------------- runtime

@@ -37,8 +37,8 @@ def test_empty_calls_are_no_ops():
     for change in (dict(B=0), dict(Sq=0)):
         args = _attn(**change)
         need = C.c_uint64(7)
-        assert lib.mgc_attention_workspace(args, need) == 0 and need.value == 0
-        assert lib.mgc_attention(args, None) == 0
+        assert lib.mgc_attention_workspace(C.byref(args), C.byref(need)) == 0 and need.value == 0
+        assert lib.mgc_attention(C.byref(args), None) == 0
     assert isinstance(args, AttentionArgs)
 
 
@@ -82,14 +82,14 @@ def _attn(**kw):
 def test_attention_refuses_sizes(bad, word):
     from edge_maskgit_b200._lib import lib
     need = C.c_uint64()
-    for rc in (lib.mgc_attention_workspace(_attn(**bad), need), lib.mgc_attention(_attn(**bad), None)):
+    for rc in (lib.mgc_attention_workspace(C.byref(_attn(**bad)), C.byref(need)), lib.mgc_attention(C.byref(_attn(**bad)), None)):
         assert rc == -1 and word in _err(lib)
 
 
 def test_null_structs_are_refused():
     from edge_maskgit_b200._lib import lib
     assert lib.mgc_attention(None, None) == -1 and "NULL" in _err(lib)
-    assert lib.mgc_attention_workspace(None, C.c_uint64()) == -1
+    assert lib.mgc_attention_workspace(None, C.byref(C.c_uint64())) == -1
 
 
 def test_python_forms_refuse():
