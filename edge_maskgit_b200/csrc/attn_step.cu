@@ -14,7 +14,7 @@
 namespace mgc {
 namespace {
 
-constexpr int WARPS = 4, KT = 16, STAGES = 4;
+constexpr int WARPS = 4, KT = 16, STAGES = 3;
 template <int DP> constexpr int row_bytes() { return DP * 2 + 16; }   // odd in 16-byte units: ldmatrix without conflicts
 template <int DP> constexpr int stage_bytes() { return 2 * KT * row_bytes<DP>(); }
 template <int DP> constexpr int ring_bytes() { return WARPS * STAGES * stage_bytes<DP>(); }
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
     }
 }
 
-// Joins the splits of one row per warp, in split order.
+// Joins the splits of one row per warp, in split order; lane = four dims.
 template <bool BF16>
 __global__ void __launch_bounds__(128) attn_combine_kernel(const __grid_constant__ AttnCall c) {
     griddep_wait();
@@ -252,24 +252,45 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const __grid_constant
     for (int s = lane; s < c.nsplit; s += 32) mm = fmaxf(mm, c.mlpart[s * all + id].x);
     for (int k = 16; k; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
     const float base = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = 0; s < c.nsplit; s++) {
-        const float2 ml = c.mlpart[s * all + id];
-        if (ml.x == -INFINITY) continue;   // nothing seen in this split
-        const float f = ex2_approx(ml.x - base);
-        ll += ml.y * f;
-        const float* o = c.opart + (s * all + id) * a.D;
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (lane + 32 * u < a.D) acc[u] = fmaf(o[lane + 32 * u], f, acc[u]);
+    const bool dims = lane * 4 < a.D;
+    const float4* op = reinterpret_cast<const float4*>(c.opart + id * a.D) + lane;
+    const long long step = all * a.D / 4;
+    float ll = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < c.nsplit; s0 += 32) {
+        const int n = min(32, c.nsplit - s0);
+        float f = 0.0f, lf = 0.0f;   // lane = split: its weight, its sum
+        if (lane < n) {
+            const float2 ml = c.mlpart[(s0 + lane) * all + id];
+            f = ex2_approx(ml.x - base);   // 0 where the split saw nothing (its partial is 0)
+            lf = ml.y * f;
+        }
+        for (int k = 16; k; k >>= 1) lf += __shfl_xor_sync(0xffffffffu, lf, k);
+        ll += lf;
+#pragma unroll 8
+        for (int s = 0; s < n; s++) {   // independent loads: eight splits in flight
+            const float w = __shfl_sync(0xffffffffu, f, s);
+            if (dims) {
+                const float4 o = __ldcs(op + (s0 + s) * step);
+                acc.x = fmaf(o.x, w, acc.x); acc.y = fmaf(o.y, w, acc.y);
+                acc.z = fmaf(o.z, w, acc.z); acc.w = fmaf(o.w, w, acc.w);
+            }
+        }
     }
-    const float inv = 1.0f / ll;
-#pragma unroll
-    for (int u = 0; u < 4; u++) acc[u] = ll == 0.0f ? 0.0f : acc[u] * inv;
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
     const int h = (int)(id % a.Hq);
     const long long bi = id / a.Hq;
-    write_row<BF16>(c, (int)(bi / a.Sq), h, (int)(bi % a.Sq), acc);
+    const int b = (int)(bi / a.Sq), i = (int)(bi % a.Sq);
+    const bool bad = dims && (isnan(acc.x) || isnan(acc.y) || isnan(acc.z) || isnan(acc.w) || isnan(ll));
+    if (__any_sync(0xffffffffu, bad)) {
+        float o[4] = {NAN, NAN, NAN, NAN};   // write_row repairs
+        write_row<BF16>(c, b, h, i, o);
+        return;
+    }
+    if (dims) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b * a.out_stride[0] + i * a.out_stride[1] + h * a.out_stride[2];
+        reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
+    }
 }
 
 template <bool BF16, int DP>

@@ -30,26 +30,115 @@ struct LinArgs {
     int act;
 };
 
-__device__ __forceinline__ float act16(float v, int a) {
-    if (a == 1) return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    if (a == 2) return v / (1.0f + __expf(-v));
-    return v;
+// x Phi(x) = max(x, 0) - |x| h(|x|), h(a) = 0.5 erfc(a / sqrt 2) = e^(-a^2 / 2) t P(t), t = 1 / (1 + 0.26 a):
+// the form of Abramowitz and Stegun 7.1.26, with seven coefficients fitted here to a relative error
+// of 8.4e-7 on 0 <= a <= 13 (beyond, h is below 2^-120), so small results keep their precision.
+// 11 FP32 operations and two MUFU against erff's ~25 and a branch: the epilogue of a 256 x 256 tile
+// has to fit under its MMAs.
+__device__ __forceinline__ float gelu16(float x) {
+    const float a = fminf(fabsf(x), 30.0f);
+    float t;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.26f, a, 1.0f)));
+    float p = fmaf(-0.0729497778f, t, 0.229241262f);
+    p = fmaf(p, t, -0.107327773f);
+    p = fmaf(p, t, 0.167471854f);
+    p = fmaf(p, t, 0.0727312424f);
+    p = fmaf(p, t, 0.107331982f);
+    p = fmaf(p, t, 0.103501627f);
+    const float h = ex2_approx(a * a * -0.7213475204f) * (p * t);
+    return fmaf(0.5f, x + fabsf(x), -(a * h));   // (x + |x|: a NaN stays one)
+}
+__device__ __forceinline__ float silu16(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_approx(x * -1.4426950409f)));
+    return x * r;
+}
+__device__ __forceinline__ float act16(float v, int a) { return a == 1 ? gelu16(v) : a == 2 ? silu16(v) : v; }
+template <int N>
+__device__ __forceinline__ void act16_all(float (&v)[N], int a) {
+    if (a == 1) {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = gelu16(v[j]);
+    } else if (a == 2) {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = silu16(v[j]);
+    }
 }
 
-// Columns [c0, c0 + 32) of the accumulator at TMEM address t (this warp's lanes): x rows m0 + c0 +
-// j, output n of this lane.
+// 32 accumulators of one output n, for x rows m .. m + 31: a warp moves 32 consecutive n of a row
+// at a time, 2 bytes a lane.
 template <bool BF16>
 __device__ __forceinline__ void finish_cols(const uint32_t (&acc)[32], const LinArgs& a, int m, int n, float bias) {
-    float res[32];
-    if (a.resid) {
+    const int rows = min(32, a.M - m);
+    uint16_t* y = reinterpret_cast<uint16_t*>(a.y) + m * a.ldy + n;
+    const uint16_t* r = a.resid ? reinterpret_cast<const uint16_t*>(a.resid) + m * a.ldr + n : nullptr;
+    float v[32], res[32];
+    if (r) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) res[j] = m + j < a.M ? load16<BF16>(a.resid, (m + j) * a.ldr + n) : 0.0f;
+        for (int j = 0; j < 32; j++) {
+            res[j] = j < rows ? load16<BF16>(r, 0) : 0.0f;
+            r += a.ldr;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = __uint_as_float(acc[j]) + bias;
+    act16_all(v, a.act);
+    if (r) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] += res[j];
     }
 #pragma unroll
     for (int j = 0; j < 32; j++) {
-        float v = act16(__uint_as_float(acc[j]) + bias, a.act);
-        if (a.resid) v += res[j];
-        if (m + j < a.M) store16<BF16>(a.y, (m + j) * a.ldy + n, v);
+        if (j < rows) store16<BF16>(y, 0, v[j]);
+        y += a.ldy;
+    }
+}
+
+// 32 accumulators of one x row m, for outputs n .. n + 31 (N a multiple of 8, y and resid rows
+// 16-byte aligned): 16 bytes a move.
+template <bool BF16>
+__device__ __forceinline__ void finish_row(const uint32_t (&acc)[32], const LinArgs& a, int m, int n) {
+    const int groups = min(4, (a.N - n) / 8);
+    uint4 res[4];
+    if (a.resid) {
+        const uint4* r = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.resid) + m * a.ldr + n);
+#pragma unroll
+        for (int g = 0; g < 4; g++) res[g] = g < groups ? __ldcs(r + g) : make_uint4(0, 0, 0, 0);
+    }
+    float v[32];
+    if (a.bias) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            float4 b0 = make_float4(0, 0, 0, 0), b1 = b0;
+            if (g < groups) {   // (bias is only 4-byte aligned)
+                const float* b = a.bias + n + 8 * g;
+                b0 = make_float4(__ldg(b), __ldg(b + 1), __ldg(b + 2), __ldg(b + 3));
+                b1 = make_float4(__ldg(b + 4), __ldg(b + 5), __ldg(b + 6), __ldg(b + 7));
+            }
+            const float b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[8 * g + j] = __uint_as_float(acc[8 * g + j]) + b[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = __uint_as_float(acc[j]);
+    }
+    act16_all(v, a.act);
+    uint4* y = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.y) + m * a.ldy + n);
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float2 f = make_float2(v[8 * g + 2 * j], v[8 * g + 2 * j + 1]);
+            if (a.resid) {
+                const float2 x = unpack16<BF16>((&res[g].x)[j]);
+                f.x += x.x;
+                f.y += x.y;
+            }
+            o[j] = pack16<BF16>(f.x, f.y);
+        }
+        if (g < groups) y[g] = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
@@ -71,7 +160,7 @@ __global__ void __launch_bounds__(ls::THREADS) linear_split_kernel(const __grid_
                                                                    const LinArgs a, int split) {
     constexpr int ST = ls::stages<BN>();
     constexpr uint32_t SB = ls::stage_bytes<BN>(), COLS = BN < 32 ? 32 : BN;
-    static_assert((uint32_t)BN * TILE_N * 4 <= ls::ring<BN>(), "the partial tile reuses the ring");
+    static_assert((uint32_t)(BN + 8) * TILE_N * 4 <= ls::ring<BN>(), "the partial tile reuses the ring");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = align1024_smem(smem_raw);
     uint64_t* full = (uint64_t*)(sm + ls::ring<BN>());
@@ -166,20 +255,33 @@ __global__ void __launch_bounds__(ls::THREADS) linear_split_kernel(const __grid_
         __syncwarp();
         cluster_sync_all();
         if (warp >= 2 && ok && n < a.N) {
+constexpr int G = BN == 16 ? 2 : 8;   // columns in flight: remote reads take a microsecond
+            const int c0 = cols * rank / split, c1 = cols * (rank + 1) / split;   // this CTA's columns
 #pragma unroll 1
-            for (int c = rank; c < cols; c += split) {   // this CTA finishes every split-th column
-                float v = 0.0f;
-                const int m = m0 + c;
-                float res = a.resid ? load16<BF16>(a.resid, m * a.ldr + n) : 0.0f;
-                for (int p = 0; p < split; p++) {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x)
-                                 : "r"(mapa_u32(part + c * TILE_N + quad * 32 + lane, p)) : "memory");
-                    v += x;
+            for (int c = c0; c < c1; c += G) {
+                float v[G], res[G];
+#pragma unroll
+                for (int j = 0; j < G; j++) {
+                    v[j] = 0.0f;
+                    res[j] = a.resid && c + j < c1 ? load16<BF16>(a.resid, (m0 + c + j) * a.ldr + n) : 0.0f;
                 }
-                v = act16(v + bias, a.act);
-                if (a.resid) v += res;
-                store16<BF16>(a.y, m * a.ldy + n, v);
+#pragma unroll 4
+                for (int p = 0; p < split; p++) {
+                    const uint32_t at = mapa_u32(part + c * TILE_N + quad * 32 + lane, p);
+#pragma unroll
+                    for (int j = 0; j < G; j++) {   // (columns past c1 lie inside the ring: read, not used)
+                        float x;
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at + j * TILE_N * 4) : "memory");
+                        v[j] += x;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < G; j++) {
+                    if (c + j >= c1) break;
+                    v[j] = act16(v[j] + bias, a.act);
+                    if (a.resid) v[j] += res[j];
+                    store16<BF16>(a.y, (m0 + c + j) * a.ldy + n, v[j]);
+                }
             }
         }
         __syncwarp();
@@ -205,7 +307,9 @@ constexpr uint32_t SB = 2 * A_BYTES, RING = ST * SB, SMEM = 1024 + RING + 256;
 constexpr int GROUP = 8;   // tiles walk 8 m-tiles before the next n-tile: both operands stay in L2
 }  // namespace lp
 
-template <bool BF16>
+// ROWS: x's rows are the lanes (a thread holds consecutive n of one row and moves 16 bytes at a
+// time, 1/8 of the instructions), where y's and resid's rows allow it; else W's rows are, as above.
+template <bool BF16, bool ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lp::THREADS, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, const LinArgs a) {
     using namespace lp;
@@ -258,8 +362,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lp::THREADS, 1)
                 if (it >= ST && !(ok = mbar_wait(empty + s, (it / ST - 1) & 1, abort_flag, 45))) break;
                 if (rank == 0) mbar_arrive_expect_tx(full + s, 2 * SB);
                 const uint32_t bar = mapa_u32(full + s, 0);
-                tma_load_2d_pair(sm + s * SB, &mw, k * BK, n0 + (int)rank * 128, bar);
-                tma_load_2d_pair(sm + s * SB + A_BYTES, &mx, k * BK, m0 + (int)rank * 128, bar);
+                tma_load_2d_pair(sm + s * SB + (ROWS ? A_BYTES : 0), &mw, k * BK, n0 + (int)rank * 128, bar);
+                tma_load_2d_pair(sm + s * SB + (ROWS ? 0 : A_BYTES), &mx, k * BK, m0 + (int)rank * 128, bar);
             }
         }
         if (!ok && rank == 0) {
@@ -293,19 +397,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lp::THREADS, 1)
             const int b = n & 1;
             int n0, m0;
             tile_at(t, n0, m0);
-            const int col = n0 + (int)rank * 128 + quad * 32 + lane;
-            const float bias = a.bias && col < a.N ? __ldg(a.bias + col) : 0.0f;
+            const int own = (ROWS ? m0 : n0) + (int)rank * 128 + quad * 32 + lane;   // this lane's row or output
+            const float bias = !ROWS && a.bias && own < a.N ? __ldg(a.bias + own) : 0.0f;
             if (!__all_sync(0xffffffffu, mbar_wait(acc_full + b, (n / 2) & 1, abort_flag, 48))) break;
             tc_fence_after();
             const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16) + b * TM + half * 128;
 #pragma unroll 1
             for (int c = 0; c < 128; c += 32) {
-                const int m = m0 + half * 128 + c;
-                if (m >= a.M) break;
+                const int other = (ROWS ? n0 : m0) + half * 128 + c;
+                if (other >= (ROWS ? a.N : a.M)) break;
                 uint32_t acc[32];
                 tmem_ld32(t_row + c, acc);
                 tmem_ld_wait();
-                if (col < a.N) finish_cols<BF16>(acc, a, m, col, bias);
+                if (own < (ROWS ? a.M : a.N)) {
+                    if (ROWS) finish_row<BF16>(acc, a, own, other);
+                    else finish_cols<BF16>(acc, a, other, own, bias);
+                }
                 __syncwarp();
             }
             tc_fence_before();
@@ -367,12 +474,14 @@ void run_linear(const void* w, long long ldw, const void* x, long long ldx, cons
     const int sms = current_sms();
     const long long big = (long long)((a.N + lp::TN - 1) / lp::TN) * ((a.M + lp::TM - 1) / lp::TM);
     if (a.M > 128 && big >= sms / 4) {
-        static std::atomic<uint64_t> done{0};
-        auto kernel = linear_pair_kernel<BF16>;
-        allow_smem(kernel, lp::SMEM, done);
-        const CUtensorMap mw = operand_map(w, BF16, a.N, a.K, ldw, 128), mx = operand_map(x, BF16, a.M, a.K, ldx, 128);
+        const bool rows = a.N % 8 == 0 && a.ldy % 8 == 0 && (uintptr_t)a.y % 16 == 0 &&
+                          (!a.resid || (a.ldr % 8 == 0 && (uintptr_t)a.resid % 16 == 0));
         if (big > 0x7fffffffLL) throw std::runtime_error("M * N is too large for one launch");
+        const CUtensorMap mw = operand_map(w, BF16, a.N, a.K, ldw, 128), mx = operand_map(x, BF16, a.M, a.K, ldx, 128);
         const unsigned pairs = (unsigned)std::min<long long>(big, sms / 2);
+        static std::atomic<uint64_t> done[2];
+        auto kernel = rows ? linear_pair_kernel<BF16, true> : linear_pair_kernel<BF16, false>;
+        allow_smem(kernel, lp::SMEM, done[rows]);
         launch_cluster(kernel, 2 * pairs, lp::THREADS, lp::SMEM, 0, st, mw, mx, a);
         return;
     }
