@@ -8,9 +8,9 @@
 //            maximum and sum need no exchange between threads (warps 10, 11 only complete a
 //            warpgroup, whose registers move together)
 // P (16 bits) overwrites the first half of its S.  While one tile's softmax runs, the tensor cores
-// work on the other's products.  The output is rescaled in TMEM only when a row's maximum has grown
-// by more than 2^8 since its last rescale: until then probabilities are relative to the old
-// maximum, which costs no precision in floating point.
+// work on the other's products.  Probabilities are relative to a base that follows the row's maximum
+// in large steps only, so the output in TMEM is hardly ever rescaled and no pass over a tile has to
+// find its maximum first; in floating point this costs no precision.
 #pragma once
 #include <climits>
 
@@ -23,10 +23,10 @@ constexpr int QT = 128, KT = 128, THREADS = 384;
 constexpr uint32_t SLAB = 128 * 128;   // 128 rows of 64 16-bit values
 template <int DP> constexpr uint32_t tile_bytes() { return SLAB * (DP / 64); }
 template <int DP> constexpr int kv_stages() { return DP == 64 ? 3 : 2; }
-constexpr uint32_t OFF_TABLE = 0;                        // [2 tiles][2 buffers][256] f32 bias by distance
-constexpr uint32_t OFF_DOC = OFF_TABLE + 4 * 256 * 4;    // [2][2][128] int32 document numbers
+constexpr int WIN = 264;   // entries of one copy of a tile's bias window (256 used)
+constexpr uint32_t OFF_TABLE = 0;                        // [2 tiles][2 buffers][4 copies][WIN] f32 bias by distance
+constexpr uint32_t OFF_DOC = OFF_TABLE + 16 * WIN * 4;    // [2][2][128] int32 document numbers
 constexpr uint32_t OFF_BAR = OFF_DOC + 4 * 128 * 4, OFF_TILES = OFF_BAR + 512;   // (from a 1024-byte boundary)
-static_assert(OFF_TILES % 512 == 0, "");
 constexpr uint32_t HEAD = (OFF_TILES + 1023) / 1024 * 1024;
 template <int DP> constexpr uint32_t smem() { return 1024 + HEAD + (2 + 2 * kv_stages<DP>()) * tile_bytes<DP>(); }
 constexpr uint32_t TM_O = 256;   // TMEM columns: S0 | S1 | O0 | O1
@@ -43,6 +43,133 @@ struct TileCall {
     const int2* doc_range;
     int kmul[3], vmul[3], qmul[3];   // 0 where a stride is 0 (batch, -, head): the map has one entry there
 };
+
+// What the softmax of one row needs of one key tile.
+struct RowTile {
+    uint32_t tS;           // TMEM address of S (this warp's lanes)
+    float c1;              // no cap: scale in base 2 (sign in `flip`); cap: scale / cap
+    uint32_t flip;
+    float cap2, slope2;
+    float d0;              // distance of the tile's key 0
+    const float* win;      // bias of key j at win[j], 16-byte aligned
+    int lim;               // keys below the row's end
+    const int4* docs;      // documents of the tile's keys, or null
+    int doc;
+};
+
+// cap tanh(u) in base 2 for |u| <= 1: u (c0 + c1 u^2 + ...), fitted here to a relative error of 5.2e-7
+// (times the cap: an error of that size in the exponent).  A score within the cap, the usual case,
+// then takes no MUFU operation; tanh from its definition would take two beside the one of 2^x.
+__device__ __forceinline__ uint64_t capped_poly(uint64_t u, uint64_t cap2) {
+    const uint64_t w = mul2(u, u);
+    uint64_t p = fma2(w, pack2(-0.00310273808f, -0.00310273808f), pack2(0.0168325986f, 0.0168325986f));
+    p = fma2(p, w, pack2(-0.0516843035f, -0.0516843035f));
+    p = fma2(p, w, pack2(0.132842583f, 0.132842583f));
+    p = fma2(p, w, pack2(-0.333293984f, -0.333293984f));
+    p = fma2(p, w, pack2(0.999999486f, 0.999999486f));
+    return mul2(mul2(u, cap2), p);
+}
+
+// Scores of 32 keys (S, from key `first` of the tile) become t, shaped scores in base 2, -inf where
+// unseen; with nothing to shape (MODE 0) they stay raw, to be scaled in one fma with the base.
+// Returns their maximum, of t in either case.
+template <int MODE>
+__device__ __forceinline__ float shape32(uint32_t (&s)[32], const RowTile& x, bool masked, int first) {
+    const uint64_t c2 = pack2(x.c1, x.c1);
+    auto S = [&](int j) -> float { return __uint_as_float(s[j]); };
+    if (!(MODE & CAP) && x.flip) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) s[j] ^= x.flip;
+    }
+    if (MODE & CAP) {
+        float hi[2] = {-INFINITY, -INFINITY}, lo[2] = {INFINITY, INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            hi[(j >> 1) & 1] = max3(hi[(j >> 1) & 1], S(j), S(j + 1));
+            lo[(j >> 1) & 1] = min3(lo[(j >> 1) & 1], S(j), S(j + 1));
+        }
+        const float top = fmaxf(fmaxf(hi[0], hi[1]), -fminf(lo[0], lo[1])) * fabsf(x.c1);
+        if (__all_sync(0xffffffffu, top <= 1.0f)) {   // (a NaN score escapes the comparison and stays NaN)
+            const uint64_t cp2 = pack2(x.cap2, x.cap2);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                float a, b;
+                unpack2(capped_poly(mul2(pack2(S(j), S(j + 1)), c2), cp2), a, b);
+                s[j] = __float_as_uint(a);
+                s[j + 1] = __float_as_uint(b);
+            }
+        } else {
+            const float k = x.c1 * (2.0f * ATTN_LOG2E);
+#pragma unroll
+            for (int j = 0; j < 32; j++) s[j] = __float_as_uint(capped(S(j), k, x.cap2));
+        }
+    }
+    if (MODE & (SLOPE | TABLE)) {
+        const float d0 = x.d0 + (float)first;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (MODE & TABLE) {
+                const float4 f = *reinterpret_cast<const float4*>(x.win + first + j);
+                b[0] = f.x; b[1] = f.y; b[2] = f.z; b[3] = f.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (MODE & SLOPE) b[e] = fmaf(-x.slope2, fabsf(d0 + (float)(j + e)), b[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const uint64_t t2 = pack2(S(j + e), S(j + e + 1)), b2 = pack2(b[e], b[e + 1]);
+                float u, v;
+                unpack2((MODE & CAP) ? add2(t2, b2) : fma2(t2, c2, b2), u, v);
+                s[j + e] = __float_as_uint(u);
+                s[j + e + 1] = __float_as_uint(v);
+            }
+        }
+    }
+    if (masked) {
+        const int lim = x.lim - first;
+#pragma unroll
+        for (int j = 0; j < 32; j++) s[j] = j < lim ? s[j] : 0xFF800000u;
+        if (x.docs) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const int4 d = x.docs[(first + j) / 4];
+                s[j] = d.x == x.doc ? s[j] : 0xFF800000u;
+                s[j + 1] = d.y == x.doc ? s[j + 1] : 0xFF800000u;
+                s[j + 2] = d.z == x.doc ? s[j + 2] : 0xFF800000u;
+                s[j + 3] = d.w == x.doc ? s[j + 3] : 0xFF800000u;
+            }
+        }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};   // (NaN is passed over here and reaches the sum through 2^t)
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) mx[(j >> 1) & 1] = max3(mx[(j >> 1) & 1], S(j), S(j + 1));
+    const float m = fmaxf(mx[0], mx[1]);
+    return MODE == 0 && m != -INFINITY ? m * x.c1 : m;
+}
+
+// A row held as columns of packed 16-bit (P) or f32 (O) TMEM words, times a power of two: exact.
+template <bool BF16>
+__device__ __forceinline__ void scale_p(uint32_t taddr, float f) {
+    uint32_t v[16];
+    tmem_ld16(taddr, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const float2 x = unpack16<BF16>(v[e]);
+        v[e] = pack16<BF16>(x.x * f, x.y * f);
+    }
+    tmem_st16(taddr, v);
+}
+__device__ __forceinline__ void scale_o(uint32_t taddr, float f) {
+    uint32_t v[32];
+    tmem_ld32(taddr, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+    tmem_st32(taddr, v);
+}
 
 template <bool BF16, int DP, int MODE>
 __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_constant__ CUtensorMap mq,
@@ -248,14 +375,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         const bool idle = q0 + w * QT + (warp & 3) * 32 >= a.Sq;   // a warp of such rows only
         const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t tS = t_row + w * KT, tO = t_row + TM_O + w * DP;
-        float* win = reinterpret_cast<float*>(sm + OFF_TABLE) + w * 512;
+        float* win = reinterpret_cast<float*>(sm + OFF_TABLE) + w * 8 * WIN;
         int* sdoc = reinterpret_cast<int*>(sm + OFF_DOC) + w * 256;
         const int bar_id = 1 + w;
-        // a scale of 0 must not meet the -inf of a masked score
-        const float c1 = (MODE & CAP) ? sh.c1 : fmaxf(fabsf(sh.c1), 1.17549435e-38f);
-        const uint32_t flip = !(MODE & CAP) && sh.c1 < 0.0f ? 0x80000000u : 0u;   // a negative scale
-        // probabilities are 2^(t - base), base = row maximum - SHIFT: f16 keeps its small ones normal
-        constexpr float SHIFT = BF16 ? 0.0f : 6.0f, SLACK = 8.0f;
+        RowTile x;
+        x.tS = tS;
+        // (a scale of 0 must not meet the -inf of a masked score)
+        x.c1 = (MODE & CAP) ? a.scale / a.cap : fmaxf(fabsf(sh.c1), 1.17549435e-38f);
+        x.flip = sh.c1 < 0.0f ? 0x80000000u : 0u;   // a negative scale
+        x.cap2 = sh.cap2;
+        x.slope2 = sh.slope2;
+        x.doc = doc;
+        // Probabilities are 2^(t - base).  base is a whole number, set at the first scores to SHIFT below
+        // their maximum, and again only when a score passes it by SLACK: what was computed before is
+        // then scaled by a power of two, exactly.  So no pass over the tile has to find its maximum
+        // first.  Probabilities go up to 2^15, which f16 holds; its smallest normal number is 2^-17
+        // of the row's maximum.
+        constexpr float SHIFT = 3.0f, SLACK = 15.0f;
 
         // bias window and documents of key tile kt: fetched a tile ahead
         float pre_b[2] = {0.0f, 0.0f};
@@ -268,124 +404,82 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             }
             if (a.doc_k) pre_d = kt * KT + r < a.Sk ? __ldg(a.doc_k + (long long)b * a.Sk + kt * KT + r) : -1;
         };
-        float m = -INFINITY, base = 0.0f, l = 0.0f;   // base: what probabilities are relative to
-        bool ok = true;
+        float base = 0.0f, l = 0.0f;
+        bool fresh = true, ok = true;   // fresh: the row has seen nothing yet, base is not set
         const int lo_w = lo[w], n_w = on[w] ? hi[w] - lo[w] : 0;
         if (n_w > 0) fetch(lo_w);
-        for (int x = 0; x < n_w; x++) {
-            const int kt = lo_w + x, buf = x & 1;
+        for (int it = 0; it < n_w; it++) {
+            const int kt = lo_w + it, buf = it & 1;
             if ((MODE & TABLE) || a.doc_k) {
-                if (MODE & TABLE) {
-                    win[buf * 256 + r] = bias2(pre_b[0]);
-                    win[buf * 256 + 128 + r] = bias2(pre_b[1]);
+                if (MODE & TABLE) {   // four copies, each shifted by one entry: every row reads aligned vectors
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const float v = bias2(pre_b[u]);
+                        const int e = r + 128 * u;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (e >= k) win[(buf * 4 + k) * WIN + e - k] = v;
+                    }
                 }
                 if (a.doc_k) sdoc[buf * 128 + r] = pre_d;
                 named_bar_sync(bar_id, 128);
-                if (x + 1 < n_w) fetch(kt + 1);
+                if (it + 1 < n_w) fetch(kt + 1);
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, x & 1, abort_flag, 58));
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, it & 1, abort_flag, 58));
             if (!ok) break;
             tc_fence_after();
             if (!idle) {
-            uint32_t s[4][32];
-#pragma unroll
-            for (int q = 0; q < 4; q++) tmem_ld32(tS + q * 32, s[q]);
-            tmem_ld_wait();
-            auto S = [&](int j) -> float { return __uint_as_float(s[j >> 5][j & 31]); };
-            auto put = [&](int j, float v) { s[j >> 5][j & 31] = __float_as_uint(v); };
-
-            // ---- shape: S becomes t in base 2 (no cap, no bias: scaled later, in one fma with the max)
-            if (MODE & CAP) {
-#pragma unroll
-                for (int j = 0; j < 128; j++) put(j, capped(S(j), c1, sh.cap2));
-            } else if (flip) {
-#pragma unroll
-                for (int j = 0; j < 128; j++) s[j >> 5][j & 31] ^= flip;
-            }
-            if (MODE & (SLOPE | TABLE)) {
-                const float d0 = (float)(kt * KT - p);
-                const float* wp = win + buf * 256 + 127 - r;
-#pragma unroll
-                for (int j = 0; j < 128; j++) {
-                    float bias = 0.0f;
-                    if (MODE & TABLE) bias = wp[j];
-                    if (MODE & SLOPE) bias = fmaf(-sh.slope2, fabsf(d0 + (float)j), bias);
-                    put(j, (MODE & CAP) ? S(j) + bias : fmaf(S(j), c1, bias));
+                x.d0 = (float)(kt * KT - p);
+                x.win = win + (buf * 4 + ((127 - r) & 3)) * WIN + ((127 - r) & ~3);
+                x.lim = end - kt * KT;
+                x.docs = nullptr;
+                if (a.doc_k) {
+                    const int2 dr = __ldg(tc.doc_range + (long long)b * nkt + kt);
+                    if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) x.docs = reinterpret_cast<const int4*>(sdoc + buf * 128);
                 }
-            }
-            // ---- mask
-            const int lim = end - kt * KT;   // keys of the tile below the row's end
-            if (!__all_sync(0xffffffffu, lim >= KT)) {
-#pragma unroll
-                for (int j = 0; j < 128; j++) put(j, j < lim ? S(j) : -INFINITY);
-            }
-            if (a.doc_k) {
-                const int2 dr = __ldg(tc.doc_range + (long long)b * nkt + kt);
-                if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) {
-                    const int4* dk = reinterpret_cast<const int4*>(sdoc + buf * 128);
-#pragma unroll
-                    for (int j = 0; j < 128; j += 4) {
-                        const int4 d = dk[j / 4];
-                        put(j, d.x == doc ? S(j) : -INFINITY);
-                        put(j + 1, d.y == doc ? S(j + 1) : -INFINITY);
-                        put(j + 2, d.z == doc ? S(j + 2) : -INFINITY);
-                        put(j + 3, d.w == doc ? S(j + 3) : -INFINITY);
+                const bool masked = x.docs || !__all_sync(0xffffffffu, x.lim >= KT);
+                // (rolled: a CTA may run few tiles, and would spend them fetching an unrolled loop's code)
+#pragma unroll 1
+                for (int q = 0; q < 4; q++) {
+                    uint32_t s[32];
+                    tmem_ld32(tS + q * 32, s);
+                    tmem_ld_wait();
+                    const float mx = shape32<MODE>(s, x, masked, q * 32);
+                    const bool set = fresh ? mx != -INFINITY : mx > base + SLACK;
+                    if (__any_sync(0xffffffffu, set)) {
+                        float alpha = 1.0f;
+                        if (set) {
+                            const float nb = ceilf(mx) - SHIFT;
+                            if (!fresh) alpha = ex2_approx(base - nb);
+                            l *= alpha;
+                            base = nb;
+                            fresh = false;
+                        }
+                        if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+                            for (int k = 0; k < q; k++) scale_p<BF16>(tS + k * 16, alpha);   // this tile's P so far
+                            if (it > 0)   // (the product before S is done: O is at rest)
+                                for (int d = 0; d < DP; d += 32) scale_o(tO + d, alpha);
+                        }
                     }
-                }
-            }
-            // ---- maximum (NaN scores are passed over here and reach the sum through 2^x)
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    const uint64_t c2 = pack2(x.c1, x.c1), nb2 = pack2(-base, -base);
+                    uint64_t sum2[2] = {0, 0};
+                    uint32_t pk[16];
 #pragma unroll
-            for (int j = 0; j < 128; j += 2) {
-                float& y = mx[(j >> 1) & 3];
-                asm("max.f32 %0, %0, %1, %2;" : "+f"(y) : "f"(S(j)), "f"(S(j + 1)));
-            }
-            float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            if (MODE == 0) tile_max = tile_max == -INFINITY ? tile_max : tile_max * c1;
-            m = fmaxf(m, tile_max);
-            const bool grow = m - SHIFT > base + SLACK || (x == 0 && m != -INFINITY) || (l == 0.0f && m != -INFINITY);
-            if (__any_sync(0xffffffffu, grow)) {
-                float alpha = 1.0f;
-                if (grow) {
-                    const float nb = m - SHIFT;
-                    alpha = l == 0.0f ? 1.0f : ex2_approx(base - nb);
-                    l *= alpha;
-                    base = nb;
-                }
-                if (x > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {   // S arrived after the last product: O is at rest
-#pragma unroll
-                    for (int d = 0; d < DP; d += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(tO + d, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(tO + d, o);
+                    for (int j = 0; j < 32; j += 2) {
+                        const uint64_t t2 = pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                        float u, v;
+                        unpack2(MODE == 0 ? fma2(t2, c2, nb2) : add2(t2, nb2), u, v);
+                        u = ex2_approx(u);
+                        v = ex2_approx(v);
+                        sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pack2(u, v));
+                        pk[j / 2] = pack16<BF16>(u, v);   // rounded to the type of v: what tensor cores multiply
                     }
+                    tmem_st16(tS + q * 16, pk);   // over scores that were read
+                    float e0, e1, e2, e3;
+                    unpack2(sum2[0], e0, e1);
+                    unpack2(sum2[1], e2, e3);
+                    l += (e0 + e1) + (e2 + e3);
                 }
-            }
-            // ---- probabilities
-            const uint64_t c2 = pack2(MODE == 0 ? c1 : 1.0f, MODE == 0 ? c1 : 1.0f), nb2 = pack2(-base, -base);
-            uint64_t sum[2] = {0, 0};
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                uint32_t pk[32];
-#pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    const int j = q * 64 + 2 * e;
-                    const uint64_t t2 = pack2(S(j), S(j + 1));
-                    float t0, t1;
-                    unpack2(MODE == 0 ? fma2(t2, c2, nb2) : add2(t2, nb2), t0, t1);
-                    const float p0 = ex2_approx(t0), p1 = ex2_approx(t1);
-                    sum[e & 1] = add2(sum[e & 1], pack2(p0, p1));
-                    pk[e] = pack16<BF16>(p0, p1);   // rounded to the type of v: what tensor cores multiply
-                }
-                tmem_st32(tS + q * 32, pk);
-            }
-            float s0, s1, s2, s3;
-            unpack2(sum[0], s0, s1);
-            unpack2(sum[1], s2, s3);
-            l += (s0 + s1) + (s2 + s3);
             }
             // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
             if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && active(0, kt))) {
@@ -410,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         if (ok && n_w > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, 0, abort_flag, 60));
         tc_fence_after();
         if (ok && w < tc.tiles_per_cta && q0 + w * QT + (warp & 3) * 32 < a.Sq) {
-            const bool any = n_w > 0 && l != 0.0f;   // (a NaN sum is not 0)
+            const bool any = n_w > 0 && !fresh;
             const float inv = any ? 1.0f / l : 0.0f;
             const long long row = ((long long)b * a.Sq + i) * a.Hq + h, id = (long long)split * a.B * a.Sq * a.Hq + row;
             if (c.nsplit > 1 && live) c.mlpart[id] = make_float2(any ? base : -INFINITY, l);

@@ -81,6 +81,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d; asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d;
+}
 // Shared-memory matrix descriptor, MN-major, 128-byte swizzle: each 128-byte row holds 64
 // consecutive 16-bit values of the M/N axis for one k; 8 k make a 1024-byte atom (stride byte
 // offset), the next 64 M/N values lie `slab` bytes further (leading byte offset).
