@@ -24,6 +24,14 @@ NVFLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-rdc=true", "-Xcompiler", "
     os.environ.get("MGC_EXTRA_NVFLAGS", "").split()
 
 
+def _flags(src: Path) -> list[str]:
+    """attn_tile_*: whole programs.  Relocatable device code would make the assembler ignore the
+    register split between their warps (setmaxnreg)."""
+    if src.name.startswith("attn_tile_"):
+        return [f for f in NVFLAGS if f != "-rdc=true"] + ["-DMGC_WHOLE_PROGRAM"]
+    return NVFLAGS
+
+
 def _headers() -> list[Path]:
     return list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + [ROOT / "include" / "mgc.h"]
 
@@ -47,7 +55,7 @@ def build(verbose: bool = False) -> Path:
         obj = BUILD / (src.name + ".o")
         objs.append(obj)
         if _stale(src, obj, hdr):
-            jobs.append([NVCC, *NVFLAGS, "-c", str(src), "-o", str(obj)])
+            jobs.append([NVCC, *_flags(src), "-c", str(src), "-o", str(obj)])
     if jobs:
         with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
             list(ex.map(_run, jobs))

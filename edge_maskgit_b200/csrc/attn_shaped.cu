@@ -142,6 +142,7 @@ void run_tile(Plan& p, cudaStream_t st) {
         p.t.doc_range = range;
     }
     p.t.c = p.c;
+    p.t.dev_error = dev_error_address();
     const CUtensorMap mq = operand_map(a.q, bf16, a.D, a.Sq, a.Hq, a.B, a.q_stride);
     const CUtensorMap mk = operand_map(a.k, bf16, a.D, a.Sk, a.Hkv, a.B, a.k_stride);
     const CUtensorMap mv = operand_map(a.v, bf16, a.D, a.Sk, a.Hkv, a.B, a.v_stride);

@@ -41,6 +41,7 @@ struct TileCall {
     // [B][key tiles] or null: x = lowest number >= 0 of the tile (INT_MAX: none), with the sign bit
     // set if some are negative; y = the highest
     const int2* doc_range;
+    int* dev_error;         // the library's device error word
     int kmul[3], vmul[3], qmul[3];   // 0 where a stride is 0 (batch, -, head): the map has one entry there
 };
 
@@ -280,9 +281,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
 
     // Registers: 384 threads start with 168 each (64512); the 256 softmax threads take 216, the
     // other warpgroup keeps 72: 256 * 216 + 128 * 72 = 64512, all of the launch's own.
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-
+    // (Inside the branches: where they meet again the compiler has to assume the smaller number.)
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
         // ---------------------------------------------------------------- copies
         if (lane == 0 && n > 0) {
@@ -299,71 +300,89 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             for (; i < n; i++) {
                 const int s = i % NST, par = (i / NST - 1) & 1;
                 if (i == 0) load_q(0);
-                if (i >= NST && !(ok = mbar_wait(k_empty + s, par, abort_flag, 51))) break;
+                if (i >= NST && !(ok = mbar_wait(k_empty + s, par, abort_flag, 51, tc.dev_error))) break;
                 load(sK + s * TB, &mk, (lo_all + i) * KT, hk * tc.kmul[2], b * tc.kmul[0], k_full + s);
                 if (i == 0) load_q(1);
-                if (i >= NST && !(ok = mbar_wait(v_empty + s, par, abort_flag, 52))) break;
+                if (i >= NST && !(ok = mbar_wait(v_empty + s, par, abort_flag, 52, tc.dev_error))) break;
                 load(sV + s * TB, &mv, (lo_all + i) * KT, hk * tc.vmul[2], b * tc.vmul[0], v_full + s);
             }
             if (!ok) {   // gave up: let the copies in flight land (tile i may have K only)
                 volatile int never = 0;
-                for (int w = 0; w < 2; w++) if (on[w]) mbar_wait(q_full + w, 0, &never, 53);
-                for (int t = max(0, i - NST); t <= i; t++) mbar_wait(k_full + t % NST, (t / NST) & 1, &never, 53);
-                for (int t = max(0, i - NST); t < i; t++) mbar_wait(v_full + t % NST, (t / NST) & 1, &never, 53);
+                for (int w = 0; w < 2; w++) if (on[w]) mbar_wait(q_full + w, 0, &never, 53, tc.dev_error);
+                for (int t = max(0, i - NST); t <= i; t++) mbar_wait(k_full + t % NST, (t / NST) & 1, &never, 53, tc.dev_error);
+                for (int t = max(0, i - NST); t < i; t++) mbar_wait(v_full + t % NST, (t / NST) & 1, &never, 53, tc.dev_error);
             }
         }
     } else if (warp == 9) {
         // ---------------------------------------------------------------- products
-        if (lane == 0 && n > 0) {
+        // The whole warp walks the loop, so that descriptors stay in uniform registers; one elected
+        // lane issues.
+        if (n > 0) {
             const int dsteps = (a.D + 15) / 16;
             constexpr uint32_t idesc_s = idesc_make(1, BF16, BF16, QT, KT);
             const uint32_t idesc_o = idesc_make(1, BF16, BF16, QT, (uint32_t)dsteps * 16) | IDESC_B_MN;
-            auto qk = [&](int w, int i) {
-                const uint64_t dq = sdesc_sw128(smem_u32(sQ + w * TB)), dk = sdesc_sw128(smem_u32(sK + (i % NST) * TB));
-                for (int k = 0; k < dsteps; k++) {
-                    const uint64_t off = (uint64_t)(k >> 2) * (SLAB >> 4) + 2 * (k & 3);
-                    mma_f16(tmem + w * KT, dq + off, dk + off, idesc_s, k > 0);
-                }
-                mma_commit(s_full + w);
-            };
-            auto pv = [&](int w, int i, bool first) {
-                const uint64_t dv = sdesc_mn_sw128(smem_u32(sV + (i % NST) * TB), SLAB);
+            const uint64_t dq0 = sdesc_sw128(smem_u32(sQ)), dk0 = sdesc_sw128(smem_u32(sK));
+            const uint64_t dv0 = sdesc_mn_sw128(smem_u32(sV), SLAB);
+            const bool lead = elect_one();
+            auto qk = [&](int w, int st) {
+                const uint64_t dq = dq0 + w * (TB >> 4), dk = dk0 + (uint32_t)st * (TB >> 4);
+                if (lead) {
 #pragma unroll
-                for (int k = 0; k < KT / 16; k++)
-                    mma_f16_ts(tmem + TM_O + w * DP, tmem + w * KT + k * 8, dv + (uint64_t)k * (2048 >> 4), idesc_o, !(first && k == 0));
+                    for (int k = 0; k < DP / 16; k++) {
+                        if (k < dsteps) {
+                            const uint32_t off = (k >> 2) * (SLAB >> 4) + 2 * (k & 3);
+                            mma_f16(tmem + w * KT, dq + off, dk + off, idesc_s, k > 0);
+                        }
+                    }
+                    mma_commit(s_full + w);
+                }
+            };
+            auto pv = [&](int w, int st, bool first, bool last) {
+                const uint64_t dv = dv0 + (uint32_t)st * (TB >> 4);
+                if (lead) {
+#pragma unroll
+                    for (int k = 0; k < KT / 16; k++)
+                        mma_f16_ts(tmem + TM_O + w * DP, tmem + w * KT + k * 8, dv + k * (2048 >> 4), idesc_o, k > 0 || !first);
+                    if (last) mma_commit(o_full + w);
+                }
             };
             bool ok = true;
-            int np[2] = {0, 0};   // P tiles consumed
+            int np[2] = {0, 0};      // P tiles consumed
+            int st = 0, par = 0;     // ring stage and parity of key tile i
             for (int i = -1; ok && i < n; i++) {
                 const int kt = lo_all + i;
-                if (i + 1 < n && !(ok = mbar_wait(k_full + (i + 1) % NST, ((i + 1) / NST) & 1, abort_flag, 54))) break;
-                bool have_v = false;
+                const int st1 = i < 0 ? 0 : st + 1 == NST ? 0 : st + 1, par1 = i < 0 ? 0 : st1 == 0 ? par ^ 1 : par;
+                if (i + 1 < n && !(ok = mbar_wait(k_full + st1, par1, abort_flag, 54, tc.dev_error))) break;
+                // (the copy of a tile between the two ranges is used by neither, but has to land)
+                if (i >= 0 && !(ok = mbar_wait(v_full + st, par, abort_flag, 56, tc.dev_error))) break;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
                     if (i >= 0 && active(w, kt)) {
-                        if (!(ok = mbar_wait(p_full + w, np[w] & 1, abort_flag, 55))) break;
-                        if (!have_v && !(ok = mbar_wait(v_full + i % NST, (i / NST) & 1, abort_flag, 56))) break;
-                        have_v = true;
+                        if (!(ok = mbar_wait(p_full + w, np[w] & 1, abort_flag, 55, tc.dev_error))) break;
                         tc_fence_after();
-                        pv(w, i, np[w] == 0);
+                        pv(w, st, np[w] == 0, kt + 1 == hi[w]);
                         np[w]++;
-                        if (kt + 1 == hi[w]) mma_commit(o_full + w);
                     }
-                    if (active(w, kt + 1) && i + 1 < n) {
-                        if ((w == 0 ? lo[0] : lo[1]) == kt + 1 && !(ok = mbar_wait(q_full + w, 0, abort_flag, 57))) break;
+                    if (i + 1 < n && active(w, kt + 1)) {
+                        if (lo[w] == kt + 1 && !(ok = mbar_wait(q_full + w, 0, abort_flag, 57, tc.dev_error))) break;
                         tc_fence_after();
-                        qk(w, i + 1);
+                        qk(w, st1);
                     }
                 }
                 if (!ok) break;
-                // a tile between the two ranges is used by neither, but its copy has to land
-                if (i >= 0 && !have_v && !(ok = mbar_wait(v_full + i % NST, (i / NST) & 1, abort_flag, 56))) break;
-                if (i >= 0) mma_commit(v_empty + i % NST);
-                if (i + 1 < n) mma_commit(k_empty + (i + 1) % NST);
+                if (lead) {
+                    if (i >= 0) mma_commit(v_empty + st);
+                    if (i + 1 < n) mma_commit(k_empty + st1);
+                }
+                st = st1;
+                par = par1;
             }
+            __syncwarp();
         }
-    } else if (warp < 8) {
+    }
+    } else {
         // ---------------------------------------------------------------- softmax: thread = row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int w = warp >> 2, r = tid & 127;
         const int i = q0 + w * QT + r, qi = min(i, a.Sq - 1);
         const int p = rb.pos0 + qi;
@@ -425,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 named_bar_sync(bar_id, 128);
                 if (it + 1 < n_w) fetch(kt + 1);
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, it & 1, abort_flag, 58));
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, it & 1, abort_flag, 58, tc.dev_error));
             if (!ok) break;
             tc_fence_after();
             if (!idle) {
@@ -438,12 +457,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) x.docs = reinterpret_cast<const int4*>(sdoc + buf * 128);
                 }
                 const bool masked = x.docs || !__all_sync(0xffffffffu, x.lim >= KT);
-                // (rolled: a CTA may run few tiles, and would spend them fetching an unrolled loop's code)
-#pragma unroll 1
-                for (int q = 0; q < 4; q++) {
-                    uint32_t s[32];
-                    tmem_ld32(tS + q * 32, s);
-                    tmem_ld_wait();
+                // 32 keys at a time, the next 32 on their way (rolled: a CTA may run few tiles, and would
+                // spend them fetching an unrolled loop's code)
+                uint32_t sa[32], sb[32];
+                auto probs = [&](uint32_t(&s)[32], int q) {
+                    tmem_ld_done(s);
+                    if (q < 3) tmem_ld32(tS + (q + 1) * 32, &s == &sa ? sb : sa);
                     const float mx = shape32<MODE>(s, x, masked, q * 32);
                     const bool set = fresh ? mx != -INFINITY : mx > base + SLACK;
                     if (__any_sync(0xffffffffu, set)) {
@@ -479,12 +498,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     unpack2(sum2[0], e0, e1);
                     unpack2(sum2[1], e2, e3);
                     l += (e0 + e1) + (e2 + e3);
+                };
+                tmem_ld32(tS, sa);
+#pragma unroll 1
+                for (int q = 0; q < 4; q += 2) {
+                    probs(sa, q);
+                    probs(sb, q + 1);
                 }
             }
             // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
             if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && active(0, kt))) {
                 const int st = (kt - lo_all) % NST;
-                ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, ((kt - lo_all) / NST) & 1, abort_flag, 59));
+                ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, ((kt - lo_all) / NST) & 1, abort_flag, 59, tc.dev_error));
                 if (!ok) break;
                 if (r >= rb.len - kt * KT) {
 #pragma unroll
@@ -501,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             if (lane == 0) mbar_arrive(p_full + w);
         }
         // ---------------------------------------------------------------- output
-        if (ok && n_w > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, 0, abort_flag, 60));
+        if (ok && n_w > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, 0, abort_flag, 60, tc.dev_error));
         tc_fence_after();
         if (ok && w < tc.tiles_per_cta && q0 + w * QT + (warp & 3) * 32 < a.Sq) {
             const bool any = n_w > 0 && !fresh;

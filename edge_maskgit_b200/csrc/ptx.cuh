@@ -6,8 +6,12 @@
 
 namespace mgc {
 
-// device-side error word: bounded waits that time out record a code here and return.
+// device-side error word: bounded waits that time out record a code here and return.  A kernel
+// whose file is compiled as a whole program (MGC_WHOLE_PROGRAM, build.py) cannot name a variable
+// of another file: it gets the word's address as an argument.
+#ifndef MGC_WHOLE_PROGRAM
 extern __device__ int g_dev_error;
+#endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
@@ -75,7 +79,7 @@ __device__ __forceinline__ bool mbar_try_wait_sleep(uint64_t* bar, uint32_t pari
 // once another thread of the CTA has set *abort.
 constexpr long long kWaitCycles = 4000000000LL;   // ~2 s at 1.9 GHz
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                          int code) {
+                                          int code, int* dev_error) {
     if (mbar_try_wait(bar, parity)) return true;
     long long t0 = clock64();
     for (uint32_t it = 1;; ++it) {
@@ -84,12 +88,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
             if (*abort_flag) return false;
             if (clock64() - t0 > kWaitCycles) {
                 *abort_flag = code;
-                atomicExch(&g_dev_error, code);
+                atomicExch(dev_error, code);
                 return false;
             }
         }
     }
 }
+#ifndef MGC_WHOLE_PROGRAM
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                          int code) {
+    return mbar_wait(bar, parity, abort_flag, code, &g_dev_error);
+}
+#endif
 
 // Named barrier `id` (1..15) over `nthreads` threads (a multiple of 32) of the CTA.
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {

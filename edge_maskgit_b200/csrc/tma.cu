@@ -60,6 +60,21 @@ int current_sms() {
     return n;
 }
 
+int* dev_error_address() {
+    constexpr int kMax = 64;
+    static std::atomic<int*> known[kMax];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMax) throw std::runtime_error("no usable current device");
+    int* p = known[dev].load();
+    if (!p) {
+        void* v = nullptr;
+        const cudaError_t e = cudaGetSymbolAddress(&v, g_dev_error);
+        if (e != cudaSuccess) throw std::runtime_error(std::string("cudaGetSymbolAddress: ") + cudaGetErrorString(e));
+        known[dev].store(p = (int*)v);
+    }
+    return p;
+}
+
 void set_error_for(const char* what, const char* msg) { set_last_error((std::string(what) + ": " + msg).c_str()); }
 
 }  // namespace mgc

@@ -21,7 +21,8 @@ namespace mgc {
 // outside.  Throws where the driver refuses the map.
 CUtensorMap make_map16(const void* base, bool bf16, int rank, const uint64_t* dims, const uint64_t* strides,
                        const uint32_t* box);
-int current_sms();   // of the current device
+int current_sms();          // of the current device
+int* dev_error_address();   // the device error word of the current device
 
 // Raises a kernel's dynamic shared-memory limit, once per device.
 template <class K>
@@ -80,6 +81,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+// Waits for this thread's TMEM loads; r's uses stay below it.
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                          "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d;
