@@ -29,7 +29,9 @@ constexpr uint32_t OFF_DOC = OFF_TABLE + 16 * WIN * 4;    // [2][2][128] int32 d
 constexpr uint32_t OFF_BAR = OFF_DOC + 4 * 128 * 4, OFF_TILES = OFF_BAR + 512;   // (from a 1024-byte boundary)
 constexpr uint32_t HEAD = (OFF_TILES + 1023) / 1024 * 1024;
 template <int DP> constexpr uint32_t smem() { return 1024 + HEAD + (2 + 2 * kv_stages<DP>()) * tile_bytes<DP>(); }
-constexpr uint32_t TM_O = 256;   // TMEM columns: S0 | S1 | O0 | O1
+// TMEM columns: S0 | S1 | O0 | O1, and with heads of up to 64 there is room for P0 | P1: then S is
+// free as soon as it is read, and the next one is ready before P is done.
+constexpr uint32_t TM_O = 256, TM_P = 384;
 
 enum Mode { CAP = 1, SLOPE = 2, TABLE = 4 };
 
@@ -47,7 +49,6 @@ struct TileCall {
 
 // What the softmax of one row needs of one key tile.
 struct RowTile {
-    uint32_t tS;           // TMEM address of S (this warp's lanes)
     float c1;              // no cap: scale in base 2 (sign in `flip`); cap: scale / cap
     uint32_t flip;
     float cap2, slope2;
@@ -71,29 +72,32 @@ __device__ __forceinline__ uint64_t capped_poly(uint64_t u, uint64_t cap2) {
     return mul2(mul2(u, cap2), p);
 }
 
-// Scores of 32 keys (S, from key `first` of the tile) become t, shaped scores in base 2, -inf where
-// unseen; with nothing to shape (MODE 0) they stay raw, to be scaled in one fma with the base.
-// Returns their maximum, of t in either case.
+// The scores of a row's 128 keys become t, shaped scores in base 2, -inf where unseen; with nothing
+// to shape (MODE 0) they stay raw, to be scaled in one fma with the base.  Returns their maximum, of
+// t in either case.
 template <int MODE>
-__device__ __forceinline__ float shape32(uint32_t (&s)[32], const RowTile& x, bool masked, int first) {
+__device__ __forceinline__ float shape_row(uint32_t (&s)[128], const RowTile& x, bool masked) {
     const uint64_t c2 = pack2(x.c1, x.c1);
     auto S = [&](int j) -> float { return __uint_as_float(s[j]); };
     if (!(MODE & CAP) && x.flip) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) s[j] ^= x.flip;
+        for (int j = 0; j < 128; j++) s[j] ^= x.flip;
     }
     if (MODE & CAP) {
-        float hi[2] = {-INFINITY, -INFINITY}, lo[2] = {INFINITY, INFINITY};
+        float hi[4], lo[4];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-            hi[(j >> 1) & 1] = max3(hi[(j >> 1) & 1], S(j), S(j + 1));
-            lo[(j >> 1) & 1] = min3(lo[(j >> 1) & 1], S(j), S(j + 1));
+        for (int k = 0; k < 4; k++) { hi[k] = -INFINITY; lo[k] = INFINITY; }
+#pragma unroll
+        for (int j = 0; j < 128; j += 2) {
+            hi[(j >> 1) & 3] = max3(hi[(j >> 1) & 3], S(j), S(j + 1));
+            lo[(j >> 1) & 3] = min3(lo[(j >> 1) & 3], S(j), S(j + 1));
         }
-        const float top = fmaxf(fmaxf(hi[0], hi[1]), -fminf(lo[0], lo[1])) * fabsf(x.c1);
+        const float top = fmaxf(fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])),
+                                -fminf(fminf(lo[0], lo[1]), fminf(lo[2], lo[3]))) * fabsf(x.c1);
         if (__all_sync(0xffffffffu, top <= 1.0f)) {   // (a NaN score escapes the comparison and stays NaN)
             const uint64_t cp2 = pack2(x.cap2, x.cap2);
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
+            for (int j = 0; j < 128; j += 2) {
                 float a, b;
                 unpack2(capped_poly(mul2(pack2(S(j), S(j + 1)), c2), cp2), a, b);
                 s[j] = __float_as_uint(a);
@@ -102,21 +106,20 @@ __device__ __forceinline__ float shape32(uint32_t (&s)[32], const RowTile& x, bo
         } else {
             const float k = x.c1 * (2.0f * ATTN_LOG2E);
 #pragma unroll
-            for (int j = 0; j < 32; j++) s[j] = __float_as_uint(capped(S(j), k, x.cap2));
+            for (int j = 0; j < 128; j++) s[j] = __float_as_uint(capped(S(j), k, x.cap2));
         }
     }
     if (MODE & (SLOPE | TABLE)) {
-        const float d0 = x.d0 + (float)first;
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
+        for (int j = 0; j < 128; j += 4) {
             float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (MODE & TABLE) {
-                const float4 f = *reinterpret_cast<const float4*>(x.win + first + j);
+                const float4 f = *reinterpret_cast<const float4*>(x.win + j);
                 b[0] = f.x; b[1] = f.y; b[2] = f.z; b[3] = f.w;
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (MODE & SLOPE) b[e] = fmaf(-x.slope2, fabsf(d0 + (float)(j + e)), b[e]);
+                if (MODE & SLOPE) b[e] = fmaf(-x.slope2, fabsf(x.d0 + (float)(j + e)), b[e]);
             }
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
@@ -129,13 +132,12 @@ __device__ __forceinline__ float shape32(uint32_t (&s)[32], const RowTile& x, bo
         }
     }
     if (masked) {
-        const int lim = x.lim - first;
 #pragma unroll
-        for (int j = 0; j < 32; j++) s[j] = j < lim ? s[j] : 0xFF800000u;
+        for (int j = 0; j < 128; j++) s[j] = j < x.lim ? s[j] : 0xFF800000u;
         if (x.docs) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                const int4 d = x.docs[(first + j) / 4];
+            for (int j = 0; j < 128; j += 4) {
+                const int4 d = x.docs[j / 4];
                 s[j] = d.x == x.doc ? s[j] : 0xFF800000u;
                 s[j + 1] = d.y == x.doc ? s[j + 1] : 0xFF800000u;
                 s[j + 2] = d.z == x.doc ? s[j + 2] : 0xFF800000u;
@@ -143,26 +145,16 @@ __device__ __forceinline__ float shape32(uint32_t (&s)[32], const RowTile& x, bo
             }
         }
     }
-    float mx[2] = {-INFINITY, -INFINITY};   // (NaN is passed over here and reaches the sum through 2^t)
+    float mx[4];   // (NaN is passed over here and reaches the sum through 2^t)
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) mx[(j >> 1) & 1] = max3(mx[(j >> 1) & 1], S(j), S(j + 1));
-    const float m = fmaxf(mx[0], mx[1]);
+    for (int k = 0; k < 4; k++) mx[k] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 128; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], S(j), S(j + 1));
+    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
     return MODE == 0 && m != -INFINITY ? m * x.c1 : m;
 }
 
-// A row held as columns of packed 16-bit (P) or f32 (O) TMEM words, times a power of two: exact.
-template <bool BF16>
-__device__ __forceinline__ void scale_p(uint32_t taddr, float f) {
-    uint32_t v[16];
-    tmem_ld16(taddr, v);
-    tmem_ld_wait();
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const float2 x = unpack16<BF16>(v[e]);
-        v[e] = pack16<BF16>(x.x * f, x.y * f);
-    }
-    tmem_st16(taddr, v);
-}
+// 32 columns of a row's output in TMEM, times a power of two.
 __device__ __forceinline__ void scale_o(uint32_t taddr, float f) {
     uint32_t v[32];
     tmem_ld32(taddr, v);
@@ -178,6 +170,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                                                                const __grid_constant__ CUtensorMap mv,
                                                                const __grid_constant__ TileCall tc) {
     constexpr int NST = kv_stages<DP>(), NSLAB = DP / 64;
+    constexpr bool SEP = DP == 64;
     constexpr uint32_t TB = tile_bytes<DP>();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = align1024_smem(smem_raw);
@@ -192,8 +185,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     uint64_t* v_empty = v_full + NST;
     uint64_t* s_full = v_empty + NST;      // [2] S is in TMEM, and the product before it is done
     uint64_t* p_full = s_full + 2;         // [2] P is in TMEM (4 warps)
-    uint64_t* o_full = p_full + 2;         // [2] the last product is done
-    uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
+    uint64_t* o_full = p_full + 2;         // [2] a product with P is done
+    uint64_t* s_free = o_full + 2;         // [2] S was read (4 warps; SEP)
+    uint32_t* tmem_slot = (uint32_t*)(s_free + 2);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     int* range = (int*)(tmem_slot + 2);    // lo0, lo1, hi0, hi1, then a tile's lowest / highest document
 
@@ -219,6 +213,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(q_full + i, 1); mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(o_full + i, 1);
+            mbar_init(s_free + i, 4);
         }
         for (int i = 0; i < NST; i++) {
             mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
@@ -337,17 +332,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     mma_commit(s_full + w);
                 }
             };
-            auto pv = [&](int w, int st, bool first, bool last) {
+            auto pv = [&](int w, int st, bool first) {
                 const uint64_t dv = dv0 + (uint32_t)st * (TB >> 4);
                 if (lead) {
 #pragma unroll
                     for (int k = 0; k < KT / 16; k++)
-                        mma_f16_ts(tmem + TM_O + w * DP, tmem + w * KT + k * 8, dv + k * (2048 >> 4), idesc_o, k > 0 || !first);
-                    if (last) mma_commit(o_full + w);
+                        mma_f16_ts(tmem + TM_O + w * DP, tmem + (SEP ? TM_P + w * (KT / 2) : w * KT) + k * 8,
+                                   dv + k * (2048 >> 4), idesc_o, k > 0 || !first);
+                    mma_commit(o_full + w);
                 }
             };
             bool ok = true;
-            int np[2] = {0, 0};      // P tiles consumed
             int st = 0, par = 0;     // ring stage and parity of key tile i
             for (int i = -1; ok && i < n; i++) {
                 const int kt = lo_all + i;
@@ -355,19 +350,27 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 if (i + 1 < n && !(ok = mbar_wait(k_full + st1, par1, abort_flag, 54, tc.dev_error))) break;
                 // (the copy of a tile between the two ranges is used by neither, but has to land)
                 if (i >= 0 && !(ok = mbar_wait(v_full + st, par, abort_flag, 56, tc.dev_error))) break;
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    if (i >= 0 && active(w, kt)) {
-                        if (!(ok = mbar_wait(p_full + w, np[w] & 1, abort_flag, 55, tc.dev_error))) break;
-                        tc_fence_after();
-                        pv(w, st, np[w] == 0, kt + 1 == hi[w]);
-                        np[w]++;
-                    }
-                    if (i + 1 < n && active(w, kt + 1)) {
-                        if (lo[w] == kt + 1 && !(ok = mbar_wait(q_full + w, 0, abort_flag, 57, tc.dev_error))) break;
-                        tc_fence_after();
-                        qk(w, st1);
-                    }
+                auto score = [&](int w) {   // S(i + 1)
+                    if (i + 1 >= n || !active(w, kt + 1)) return;
+                    if (lo[w] == kt + 1) ok = ok && mbar_wait(q_full + w, 0, abort_flag, 57, tc.dev_error);
+                    else if (SEP) ok = ok && mbar_wait(s_free + w, (kt - lo[w]) & 1, abort_flag, 62, tc.dev_error);
+                    if (!ok) return;
+                    tc_fence_after();
+                    qk(w, st1);
+                };
+                auto product = [&](int w) {   // O += P(i) V(i)
+                    if (i < 0 || !active(w, kt)) return;
+                    ok = ok && mbar_wait(p_full + w, (kt - lo[w]) & 1, abort_flag, 55, tc.dev_error);
+                    if (!ok) return;
+                    tc_fence_after();
+                    pv(w, st, kt == lo[w]);
+                };
+                if (SEP) {
+                    score(0); score(1);
+                    product(0); product(1);
+                } else {   // S(i + 1) takes the place of P(i)
+                    product(0); score(0);
+                    product(1); score(1);
                 }
                 if (!ok) break;
                 if (lead) {
@@ -393,12 +396,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         const int end = doc >= 0 ? key_end(rb, p) : 0;
         const bool idle = q0 + w * QT + (warp & 3) * 32 >= a.Sq;   // a warp of such rows only
         const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t tS = t_row + w * KT, tO = t_row + TM_O + w * DP;
+        const uint32_t tS = t_row + w * KT, tO = t_row + TM_O + w * DP, tP = SEP ? t_row + TM_P + w * (KT / 2) : tS;
         float* win = reinterpret_cast<float*>(sm + OFF_TABLE) + w * 8 * WIN;
         int* sdoc = reinterpret_cast<int*>(sm + OFF_DOC) + w * 256;
         const int bar_id = 1 + w;
         RowTile x;
-        x.tS = tS;
         // (a scale of 0 must not meet the -inf of a masked score)
         x.c1 = (MODE & CAP) ? a.scale / a.cap : fmaxf(fabsf(sh.c1), 1.17549435e-38f);
         x.flip = sh.c1 < 0.0f ? 0x80000000u : 0u;   // a negative scale
@@ -447,6 +449,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, it & 1, abort_flag, 58, tc.dev_error));
             if (!ok) break;
             tc_fence_after();
+            uint32_t s[128];
+            if (!idle) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) tmem_ld32(tS + q * 32, reinterpret_cast<uint32_t(&)[32]>(s[q * 32]));
+#pragma unroll
+                for (int q = 0; q < 4; q++) tmem_ld_done(reinterpret_cast<uint32_t(&)[32]>(s[q * 32]));
+            }
+            if (SEP) {   // the next S may come; P and O wait for the product before
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free + w);
+                if (it > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, (it - 1) & 1, abort_flag, 61, tc.dev_error)))) break;
+                tc_fence_after();
+            }
             if (!idle) {
                 x.d0 = (float)(kt * KT - p);
                 x.win = win + (buf * 4 + ((127 - r) & 3)) * WIN + ((127 - r) & ~3);
@@ -457,54 +473,44 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) x.docs = reinterpret_cast<const int4*>(sdoc + buf * 128);
                 }
                 const bool masked = x.docs || !__all_sync(0xffffffffu, x.lim >= KT);
-                // 32 keys at a time, the next 32 on their way (rolled: a CTA may run few tiles, and would
-                // spend them fetching an unrolled loop's code)
-                uint32_t sa[32], sb[32];
-                auto probs = [&](uint32_t(&s)[32], int q) {
-                    tmem_ld_done(s);
-                    if (q < 3) tmem_ld32(tS + (q + 1) * 32, &s == &sa ? sb : sa);
-                    const float mx = shape32<MODE>(s, x, masked, q * 32);
-                    const bool set = fresh ? mx != -INFINITY : mx > base + SLACK;
-                    if (__any_sync(0xffffffffu, set)) {
-                        float alpha = 1.0f;
-                        if (set) {
-                            const float nb = ceilf(mx) - SHIFT;
-                            if (!fresh) alpha = ex2_approx(base - nb);
-                            l *= alpha;
-                            base = nb;
-                            fresh = false;
-                        }
-                        if (__any_sync(0xffffffffu, alpha != 1.0f)) {
-                            for (int k = 0; k < q; k++) scale_p<BF16>(tS + k * 16, alpha);   // this tile's P so far
-                            if (it > 0)   // (the product before S is done: O is at rest)
-                                for (int d = 0; d < DP; d += 32) scale_o(tO + d, alpha);
-                        }
+                const float mx = shape_row<MODE>(s, x, masked);
+                const bool set = fresh ? mx != -INFINITY : mx > base + SLACK;
+                if (__any_sync(0xffffffffu, set)) {
+                    float alpha = 1.0f;
+                    if (set) {
+                        const float nb = ceilf(mx) - SHIFT;
+                        if (!fresh) alpha = ex2_approx(base - nb);
+                        l *= alpha;
+                        base = nb;
+                        fresh = false;
                     }
-                    const uint64_t c2 = pack2(x.c1, x.c1), nb2 = pack2(-base, -base);
-                    uint64_t sum2[2] = {0, 0};
+                    if (it > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll 1
+                        for (int d = 0; d < DP; d += 32) scale_o(tO + d, alpha);
+                    }
+                }
+                const uint64_t c2 = pack2(x.c1, x.c1), nb2 = pack2(-base, -base);
+                uint64_t sum2[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
                     uint32_t pk[16];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
+                    for (int e = 0; e < 16; e++) {
+                        const int j = q * 32 + 2 * e;
                         const uint64_t t2 = pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
                         float u, v;
                         unpack2(MODE == 0 ? fma2(t2, c2, nb2) : add2(t2, nb2), u, v);
                         u = ex2_approx(u);
                         v = ex2_approx(v);
-                        sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pack2(u, v));
-                        pk[j / 2] = pack16<BF16>(u, v);   // rounded to the type of v: what tensor cores multiply
+                        sum2[e & 3] = add2(sum2[e & 3], pack2(u, v));
+                        pk[e] = pack16<BF16>(u, v);   // rounded to the type of v: what tensor cores multiply
                     }
-                    tmem_st16(tS + q * 16, pk);   // over scores that were read
-                    float e0, e1, e2, e3;
-                    unpack2(sum2[0], e0, e1);
-                    unpack2(sum2[1], e2, e3);
-                    l += (e0 + e1) + (e2 + e3);
-                };
-                tmem_ld32(tS, sa);
-#pragma unroll 1
-                for (int q = 0; q < 4; q += 2) {
-                    probs(sa, q);
-                    probs(sb, q + 1);
+                    tmem_st16(tP + q * 16, pk);
                 }
+                float e0, e1, e2, e3;
+                unpack2(add2(sum2[0], sum2[1]), e0, e1);
+                unpack2(add2(sum2[2], sum2[3]), e2, e3);
+                l += (e0 + e1) + (e2 + e3);
             }
             // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
             if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && active(0, kt))) {
@@ -526,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             if (lane == 0) mbar_arrive(p_full + w);
         }
         // ---------------------------------------------------------------- output
-        if (ok && n_w > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, 0, abort_flag, 60, tc.dev_error));
+        if (ok && n_w > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, (n_w - 1) & 1, abort_flag, 60, tc.dev_error));
         tc_fence_after();
         if (ok && w < tc.tiles_per_cta && q0 + w * QT + (warp & 3) * 32 < a.Sq) {
             const bool any = n_w > 0 && !fresh;
