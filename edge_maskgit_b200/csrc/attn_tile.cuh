@@ -53,11 +53,16 @@ struct RowTile {
     uint32_t flip;
     float cap2, slope2;
     float d0;              // distance of the tile's key 0
+    float lin_a, lin_b;    // the bias of key j where it is linear: lin_a + lin_b * j
     const float* win;      // bias of key j at win[j], 16-byte aligned
     int lim;               // keys below the row's end
     const int4* docs;      // documents of the tile's keys, or null
     int doc;
+    float k0, k1, k2;      // cap: t = s (k0 + k1 s^2 + k2 s^4) while |s c1| <= CAP_RAW
 };
+// cap tanh(u) in base 2 for |u| <= 1/3, u (c0 + c1 u^2 + c2 u^4), fitted here to a relative error of
+// 2.2e-6: scores well below their cap, the usual case, take four FP32 operations a pair.
+constexpr float CAP_RAW = 1.0f / 3.0f;
 
 // cap tanh(u) in base 2 for |u| <= 1: u (c0 + c1 u^2 + ...), fitted here to a relative error of 5.2e-7
 // (times the cap: an error of that size in the exponent).  A score within the cap, the usual case,
@@ -72,32 +77,31 @@ __device__ __forceinline__ uint64_t capped_poly(uint64_t u, uint64_t cap2) {
     return mul2(mul2(u, cap2), p);
 }
 
-// The scores of a row's 128 keys become t, shaped scores in base 2, -inf where unseen; with nothing
-// to shape (MODE 0) they stay raw, to be scaled in one fma with the base.  Returns their maximum, of
-// t in either case.
+__device__ __forceinline__ void flip32(uint32_t* s, const RowTile& x) {   // a negative scale
+    if (x.flip) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) s[j] ^= x.flip;
+    }
+}
+// Scores of 32 keys, from key `first` of the tile, become t, shaped scores in base 2 (MODE 0: they
+// stay raw, to be scaled in one fma with the base).
 template <int MODE>
-__device__ __forceinline__ float shape_row(uint32_t (&s)[128], const RowTile& x, bool masked) {
+__device__ __forceinline__ void shape32(uint32_t* s, const RowTile& x, int first) {
     const uint64_t c2 = pack2(x.c1, x.c1);
     auto S = [&](int j) -> float { return __uint_as_float(s[j]); };
-    if (!(MODE & CAP) && x.flip) {
-#pragma unroll
-        for (int j = 0; j < 128; j++) s[j] ^= x.flip;
-    }
+    if (!(MODE & CAP)) flip32(s, x);
     if (MODE & CAP) {
-        float hi[4], lo[4];
+        float hi[2] = {-INFINITY, -INFINITY}, lo[2] = {INFINITY, INFINITY};
 #pragma unroll
-        for (int k = 0; k < 4; k++) { hi[k] = -INFINITY; lo[k] = INFINITY; }
-#pragma unroll
-        for (int j = 0; j < 128; j += 2) {
-            hi[(j >> 1) & 3] = max3(hi[(j >> 1) & 3], S(j), S(j + 1));
-            lo[(j >> 1) & 3] = min3(lo[(j >> 1) & 3], S(j), S(j + 1));
+        for (int j = 0; j < 32; j += 2) {
+            hi[(j >> 1) & 1] = max3(hi[(j >> 1) & 1], S(j), S(j + 1));
+            lo[(j >> 1) & 1] = min3(lo[(j >> 1) & 1], S(j), S(j + 1));
         }
-        const float top = fmaxf(fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])),
-                                -fminf(fminf(lo[0], lo[1]), fminf(lo[2], lo[3]))) * fabsf(x.c1);
+        const float top = fmaxf(fmaxf(hi[0], hi[1]), -fminf(lo[0], lo[1])) * fabsf(x.c1);
         if (__all_sync(0xffffffffu, top <= 1.0f)) {   // (a NaN score escapes the comparison and stays NaN)
             const uint64_t cp2 = pack2(x.cap2, x.cap2);
 #pragma unroll
-            for (int j = 0; j < 128; j += 2) {
+            for (int j = 0; j < 32; j += 2) {
                 float a, b;
                 unpack2(capped_poly(mul2(pack2(S(j), S(j + 1)), c2), cp2), a, b);
                 s[j] = __float_as_uint(a);
@@ -106,20 +110,21 @@ __device__ __forceinline__ float shape_row(uint32_t (&s)[128], const RowTile& x,
         } else {
             const float k = x.c1 * (2.0f * ATTN_LOG2E);
 #pragma unroll
-            for (int j = 0; j < 128; j++) s[j] = __float_as_uint(capped(S(j), k, x.cap2));
+            for (int j = 0; j < 32; j++) s[j] = __float_as_uint(capped(S(j), k, x.cap2));
         }
     }
     if (MODE & (SLOPE | TABLE)) {
+        const float d0 = x.d0 + (float)first;
 #pragma unroll
-        for (int j = 0; j < 128; j += 4) {
+        for (int j = 0; j < 32; j += 4) {
             float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (MODE & TABLE) {
-                const float4 f = *reinterpret_cast<const float4*>(x.win + j);
+                const float4 f = *reinterpret_cast<const float4*>(x.win + first + j);
                 b[0] = f.x; b[1] = f.y; b[2] = f.z; b[3] = f.w;
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (MODE & SLOPE) b[e] = fmaf(-x.slope2, fabsf(x.d0 + (float)(j + e)), b[e]);
+                if (MODE & SLOPE) b[e] = fmaf(-x.slope2, fabsf(d0 + (float)(j + e)), b[e]);
             }
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
@@ -131,27 +136,28 @@ __device__ __forceinline__ float shape_row(uint32_t (&s)[128], const RowTile& x,
             }
         }
     }
-    if (masked) {
+}
+// Unseen keys' scores become -inf.
+__device__ __forceinline__ void mask32(uint32_t* s, const RowTile& x, int first) {
+    const int lim = x.lim - first;
 #pragma unroll
-        for (int j = 0; j < 128; j++) s[j] = j < x.lim ? s[j] : 0xFF800000u;
-        if (x.docs) {
+    for (int j = 0; j < 32; j++) s[j] = j < lim ? s[j] : 0xFF800000u;
+    if (x.docs) {
 #pragma unroll
-            for (int j = 0; j < 128; j += 4) {
-                const int4 d = x.docs[j / 4];
-                s[j] = d.x == x.doc ? s[j] : 0xFF800000u;
-                s[j + 1] = d.y == x.doc ? s[j + 1] : 0xFF800000u;
-                s[j + 2] = d.z == x.doc ? s[j + 2] : 0xFF800000u;
-                s[j + 3] = d.w == x.doc ? s[j + 3] : 0xFF800000u;
-            }
+        for (int j = 0; j < 32; j += 4) {
+            const int4 d = x.docs[(first + j) / 4];
+            s[j] = d.x == x.doc ? s[j] : 0xFF800000u;
+            s[j + 1] = d.y == x.doc ? s[j + 1] : 0xFF800000u;
+            s[j + 2] = d.z == x.doc ? s[j + 2] : 0xFF800000u;
+            s[j + 3] = d.w == x.doc ? s[j + 3] : 0xFF800000u;
         }
     }
-    float mx[4];   // (NaN is passed over here and reaches the sum through 2^t)
+}
+// hi[] = max(hi[], s[]), NaN where a score is
+__device__ __forceinline__ void max32(float (&hi)[4], const uint32_t* s) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) mx[k] = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 128; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], S(j), S(j + 1));
-    const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-    return MODE == 0 && m != -INFINITY ? m * x.c1 : m;
+    for (int j = 0; j < 32; j += 2)
+        hi[(j >> 1) & 3] = max3_nan(hi[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
 }
 
 // 32 columns of a row's output in TMEM, times a power of two.
@@ -187,7 +193,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     uint64_t* p_full = s_full + 2;         // [2] P is in TMEM (4 warps)
     uint64_t* o_full = p_full + 2;         // [2] a product with P is done
     uint64_t* s_free = o_full + 2;         // [2] S was read (4 warps; SEP)
-    uint32_t* tmem_slot = (uint32_t*)(s_free + 2);
+    uint64_t* turn = s_free + 2;           // [2] the other tile's exponentials are done (4 warps)
+    uint64_t* p_half = turn + 2;           // [2] the first half of P is in TMEM (4 warps)
+    uint32_t* tmem_slot = (uint32_t*)(p_half + 2);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     int* range = (int*)(tmem_slot + 2);    // lo0, lo1, hi0, hi1, then a tile's lowest / highest document
 
@@ -213,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(q_full + i, 1); mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(o_full + i, 1);
-            mbar_init(s_free + i, 4);
+            mbar_init(s_free + i, 4); mbar_init(turn + i, 4); mbar_init(p_half + i, 4);
         }
         for (int i = 0; i < NST; i++) {
             mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
@@ -272,7 +280,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     const int lo_all = min(on[0] ? lo[0] : INT_MAX, on[1] ? lo[1] : INT_MAX);
     const int hi_all = max(on[0] ? hi[0] : 0, on[1] ? hi[1] : 0);
     const int n = hi_all > lo_all ? hi_all - lo_all : 0;
-    auto active = [&](int w, int kt) { return on[w] && kt >= lo[w] && kt < hi[w]; };
+    // Step i works on key tile order(i): from the diagonal (the last query's position) down to the first,
+    // then up from there.  A bias that falls with the distance has its largest values first, so bases
+    // are not moved from tile to tile, and causally the tile with the mask comes first.
+    const int centre = max(lo_all, min(hi_all - 1, (rb.pos0 + min(q0 + tc.tiles_per_cta * QT, a.Sq) - 1) >> 7));
+    auto order = [&](int i) { return i <= centre - lo_all ? centre - i : lo_all + i; };
+    auto active = [&](int w, int i) {
+        const int kt = order(i);
+        return on[w] && i >= 0 && i < n && kt >= lo[w] && kt < hi[w];
+    };
 
     // Registers: 384 threads start with 168 each (64512); the 256 softmax threads take 216, the
     // other warpgroup keeps 72: 256 * 216 + 128 * 72 = 64512, all of the launch's own.
@@ -296,10 +312,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 const int s = i % NST, par = (i / NST - 1) & 1;
                 if (i == 0) load_q(0);
                 if (i >= NST && !(ok = mbar_wait(k_empty + s, par, abort_flag, 51, tc.dev_error))) break;
-                load(sK + s * TB, &mk, (lo_all + i) * KT, hk * tc.kmul[2], b * tc.kmul[0], k_full + s);
+                load(sK + s * TB, &mk, order(i) * KT, hk * tc.kmul[2], b * tc.kmul[0], k_full + s);
                 if (i == 0) load_q(1);
                 if (i >= NST && !(ok = mbar_wait(v_empty + s, par, abort_flag, 52, tc.dev_error))) break;
-                load(sV + s * TB, &mv, (lo_all + i) * KT, hk * tc.vmul[2], b * tc.vmul[0], v_full + s);
+                load(sV + s * TB, &mv, order(i) * KT, hk * tc.vmul[2], b * tc.vmul[0], v_full + s);
             }
             if (!ok) {   // gave up: let the copies in flight land (tile i may have K only)
                 volatile int never = 0;
@@ -332,38 +348,46 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     mma_commit(s_full + w);
                 }
             };
-            auto pv = [&](int w, int st, bool first) {
+            auto pv = [&](int w, int st, bool first, int k0, int k1) {
                 const uint64_t dv = dv0 + (uint32_t)st * (TB >> 4);
                 if (lead) {
 #pragma unroll
-                    for (int k = 0; k < KT / 16; k++)
+                    for (int k = k0; k < k1; k++)
                         mma_f16_ts(tmem + TM_O + w * DP, tmem + (SEP ? TM_P + w * (KT / 2) : w * KT) + k * 8,
                                    dv + k * (2048 >> 4), idesc_o, k > 0 || !first);
-                    mma_commit(o_full + w);
+                    if (k1 == KT / 16) mma_commit(o_full + w);
                 }
             };
             bool ok = true;
-            int st = 0, par = 0;     // ring stage and parity of key tile i
+            int ns[2] = {0, 0}, np[2] = {0, 0};   // scores and products issued
+            int st = 0, par = 0;                  // ring stage and parity of step i
             for (int i = -1; ok && i < n; i++) {
-                const int kt = lo_all + i;
                 const int st1 = i < 0 ? 0 : st + 1 == NST ? 0 : st + 1, par1 = i < 0 ? 0 : st1 == 0 ? par ^ 1 : par;
                 if (i + 1 < n && !(ok = mbar_wait(k_full + st1, par1, abort_flag, 54, tc.dev_error))) break;
                 // (the copy of a tile between the two ranges is used by neither, but has to land)
                 if (i >= 0 && !(ok = mbar_wait(v_full + st, par, abort_flag, 56, tc.dev_error))) break;
-                auto score = [&](int w) {   // S(i + 1)
-                    if (i + 1 >= n || !active(w, kt + 1)) return;
-                    if (lo[w] == kt + 1) ok = ok && mbar_wait(q_full + w, 0, abort_flag, 57, tc.dev_error);
-                    else if (SEP) ok = ok && mbar_wait(s_free + w, (kt - lo[w]) & 1, abort_flag, 62, tc.dev_error);
+                auto score = [&](int w) {   // S of step i + 1
+                    if (!active(w, i + 1)) return;
+                    if (ns[w] == 0) ok = ok && mbar_wait(q_full + w, 0, abort_flag, 57, tc.dev_error);
+                    else if (SEP) ok = ok && mbar_wait(s_free + w, (ns[w] - 1) & 1, abort_flag, 62, tc.dev_error);
                     if (!ok) return;
                     tc_fence_after();
                     qk(w, st1);
+                    ns[w]++;
                 };
-                auto product = [&](int w) {   // O += P(i) V(i)
-                    if (i < 0 || !active(w, kt)) return;
-                    ok = ok && mbar_wait(p_full + w, (kt - lo[w]) & 1, abort_flag, 55, tc.dev_error);
+                auto product = [&](int w) {   // O += P V of step i
+                    if (!active(w, i)) return;
+                    if (!SEP) {
+                        ok = ok && mbar_wait(p_half + w, np[w] & 1, abort_flag, 64, tc.dev_error);
+                        if (!ok) return;
+                        tc_fence_after();
+                        pv(w, st, np[w] == 0, 0, KT / 32);
+                    }
+                    ok = ok && mbar_wait(p_full + w, np[w] & 1, abort_flag, 55, tc.dev_error);
                     if (!ok) return;
                     tc_fence_after();
-                    pv(w, st, kt == lo[w]);
+                    pv(w, st, np[w] == 0, SEP ? 0 : KT / 32, KT / 16);
+                    np[w]++;
                 };
                 if (SEP) {
                     score(0); score(1);
@@ -387,10 +411,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         // ---------------------------------------------------------------- softmax: thread = row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int w = warp >> 2, r = tid & 127;
-        const int i = q0 + w * QT + r, qi = min(i, a.Sq - 1);
+        const int row_i = q0 + w * QT + r, qi = min(row_i, a.Sq - 1);
         const int p = rb.pos0 + qi;
         const ScoreShape sh = score_shape(a, h);
-        const bool live = w < tc.tiles_per_cta && i < a.Sq;
+        const bool live = w < tc.tiles_per_cta && row_i < a.Sq;
         // (rows past the last query compute on as copies of it, so that they force no masking)
         const int doc = a.doc_q ? __ldg(a.doc_q + (long long)b * a.Sq + qi) : 0;
         const int end = doc >= 0 ? key_end(rb, p) : 0;
@@ -407,12 +431,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         x.cap2 = sh.cap2;
         x.slope2 = sh.slope2;
         x.doc = doc;
+        x.k0 = 0.999997882f * x.cap2 * x.c1;
+        x.k1 = -0.332985124f * x.cap2 * x.c1 * x.c1 * x.c1;
+        x.k2 = 0.124804431f * x.cap2 * x.c1 * x.c1 * x.c1 * x.c1 * x.c1;
         // Probabilities are 2^(t - base).  base is a whole number, set at the first scores to SHIFT below
         // their maximum, and again only when a score passes it by SLACK: what was computed before is
         // then scaled by a power of two, exactly.  So no pass over the tile has to find its maximum
-        // first.  Probabilities go up to 2^15, which f16 holds; its smallest normal number is 2^-17
-        // of the row's maximum.
-        constexpr float SHIFT = 3.0f, SLACK = 15.0f;
+        // first.  In f16 probabilities go up to 2^15, which it holds, and its smallest normal number
+        // is 2^-17 of the row's maximum; bf16 has room for more.
+        constexpr float SHIFT = 3.0f, SLACK = BF16 ? 40.0f : 15.0f;
 
         // bias window and documents of key tile kt: fetched a tile ahead
         float pre_b[2] = {0.0f, 0.0f};
@@ -427,12 +454,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         };
         float base = 0.0f, l = 0.0f;
         bool fresh = true, ok = true;   // fresh: the row has seen nothing yet, base is not set
-        const int lo_w = lo[w], n_w = on[w] ? hi[w] - lo[w] : 0;
-        if (n_w > 0) fetch(lo_w);
-        for (int it = 0; it < n_w; it++) {
-            const int kt = lo_w + it, buf = it & 1;
-            if ((MODE & TABLE) || a.doc_k) {
-                if (MODE & TABLE) {   // four copies, each shifted by one entry: every row reads aligned vectors
+        const int n_w = on[w] ? hi[w] - lo[w] : 0;
+        int i = 0, it = 0, turns = 0;   // step, this tile's steps so far, turns waited for
+        while (i < n && !active(w, i)) i++;
+        if (n_w > 0) fetch(order(i));
+        for (int next; it < n_w; i = next, it++) {
+            const int kt = order(i), buf = it & 1;
+            for (next = i + 1; next < n && !active(w, next);) next++;
+            // all of the tile's distances beyond the table's range on one side: one bias for all
+            const int dist_lo = kt * KT - (rb.pos0 + q0 + w * QT) - 127, dist_hi = dist_lo + 254;
+            const bool flat = (MODE & TABLE) && (dist_lo >= sh.range || dist_hi <= -sh.range);
+            if (((MODE & TABLE) && !flat) || a.doc_k) {
+                if ((MODE & TABLE) && !flat) {   // four copies, each shifted by one entry: every row reads aligned vectors
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         const float v = bias2(pre_b[u]);
@@ -444,38 +477,131 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 }
                 if (a.doc_k) sdoc[buf * 128 + r] = pre_d;
                 named_bar_sync(bar_id, 128);
-                if (it + 1 < n_w) fetch(kt + 1);
             }
+            x.d0 = (float)(kt * KT - p);
+            x.lin_a = x.lin_b = 0.0f;
+            bool linear = false;
+            if (MODE & (SLOPE | TABLE)) {
+                linear = !(MODE & TABLE) || flat;
+                if (MODE & SLOPE) linear = linear && __all_sync(0xffffffffu, x.d0 >= 0.0f || x.d0 <= -127.0f);
+                x.lin_b = x.d0 >= 0.0f ? -x.slope2 : x.slope2;
+                x.lin_a = ((MODE & SLOPE) ? x.lin_b * x.d0 : 0.0f) + (flat ? bias2(pre_b[0]) : 0.0f);
+            }
+            if (((MODE & TABLE) || a.doc_k) && next < n) fetch(order(next));
+            x.win = win + (buf * 4 + ((127 - r) & 3)) * WIN + ((127 - r) & ~3);
+            x.lim = end - kt * KT;
+            x.docs = nullptr;
+            if (a.doc_k) {
+                const int2 dr = __ldg(tc.doc_range + (long long)b * nkt + kt);
+                if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) x.docs = reinterpret_cast<const int4*>(sdoc + buf * 128);
+            }
+            const bool masked = x.docs || !__all_sync(0xffffffffu, x.lim >= KT);
+
             ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, it & 1, abort_flag, 58, tc.dev_error));
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[128];
-            if (!idle) {
+            // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
+            if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && active(0, i))) {
+                const int st = i % NST;
+                ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, (i / NST) & 1, abort_flag, 59, tc.dev_error));
+                if (!ok) break;
+                if (r >= rb.len - kt * KT) {
+#pragma unroll
+                    for (int sl = 0; sl < NSLAB; sl++)
+#pragma unroll
+                        for (int ch = 0; ch < 8; ch++)
+                            *reinterpret_cast<uint4*>(sV + st * TB + sl * SLAB + r * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+            }
+            // (SEP) the next S may come; P and O are free once the product before is done
+            auto s_is_read = [&] {
+                if (!SEP) return;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free + w);
+            };
+            auto wait_product = [&] {
+                if (!SEP || it == 0) return;
+                ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, (it - 1) & 1, abort_flag, 61, tc.dev_error));
+                tc_fence_after();
+            };
+            auto half_done = [&] {   // P of the first 64 keys is in TMEM
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_half + w);
+            };
+            if (idle) {
+                s_is_read();
+                wait_product();
+                if (!SEP) half_done();
+            } else {
+                uint32_t s[128];
+                bool raw = MODE == 0;   // s holds scores to be shaped with the exponentials, not t
+                float hi[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, lo_s[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
 #pragma unroll
                 for (int q = 0; q < 4; q++) tmem_ld32(tS + q * 32, reinterpret_cast<uint32_t(&)[32]>(s[q * 32]));
 #pragma unroll
                 for (int q = 0; q < 4; q++) tmem_ld_done(reinterpret_cast<uint32_t(&)[32]>(s[q * 32]));
-            }
-            if (SEP) {   // the next S may come; P and O wait for the product before
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_free + w);
-                if (it > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, (it - 1) & 1, abort_flag, 61, tc.dev_error)))) break;
-                tc_fence_after();
-            }
-            if (!idle) {
-                x.d0 = (float)(kt * KT - p);
-                x.win = win + (buf * 4 + ((127 - r) & 3)) * WIN + ((127 - r) & ~3);
-                x.lim = end - kt * KT;
-                x.docs = nullptr;
-                if (a.doc_k) {
-                    const int2 dr = __ldg(tc.doc_range + (long long)b * nkt + kt);
-                    if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) x.docs = reinterpret_cast<const int4*>(sdoc + buf * 128);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    if (MODE == CAP) {
+                        max32(hi, s + q * 32);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2)
+                            lo_s[(j >> 1) & 3] = min3(lo_s[(j >> 1) & 3], __uint_as_float(s[q * 32 + j]), __uint_as_float(s[q * 32 + j + 1]));
+                    }
                 }
-                const bool masked = x.docs || !__all_sync(0xffffffffu, x.lim >= KT);
-                const float mx = shape_row<MODE>(s, x, masked);
+                if (MODE != CAP) {
+                    // (a tile whose bias is linear in the key keeps its raw scores: t is cheap to form twice)
+                    raw = MODE == 0 || ((MODE & CAP) == 0 && linear);
+                    if (!raw || x.flip) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            if (raw) flip32(s + q * 32, x);
+                            else shape32<MODE>(s + q * 32, x, q * 32);
+                        }
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) mask32(s + q * 32, x, q * 32);
+                    }
+                    if ((MODE & SLOPE) && raw) {
+#pragma unroll
+                        for (int j = 0; j < 128; j += 2)
+                            hi[(j >> 1) & 3] = max3_nan(hi[(j >> 1) & 3], fmaf(__uint_as_float(s[j]), x.c1, fmaf((float)j, x.lin_b, x.lin_a)),
+                                                        fmaf(__uint_as_float(s[j + 1]), x.c1, fmaf((float)(j + 1), x.lin_b, x.lin_a)));
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) max32(hi, s + q * 32);
+                    }
+                }
+                float mx = max3_nan(max3_nan(hi[0], hi[1], hi[2]), hi[3], hi[3]);
+                if (raw && !(MODE & SLOPE) && mx != -INFINITY) mx = fmaf(mx, x.c1, x.lin_a);
+                if (MODE == CAP) {
+                    const float low = fminf(fminf(lo_s[0], lo_s[1]), fminf(lo_s[2], lo_s[3]));
+                    raw = !masked && __all_sync(0xffffffffu, fmaxf(mx, -low) * fabsf(x.c1) <= CAP_RAW && mx == mx);
+                    if (raw) {   // capped scores keep their order
+                        mx = x.c1 < 0.0f ? low : mx;
+                        const float w2 = mx * mx;
+                        mx *= fmaf(fmaf(w2, x.k2, x.k1), w2, x.k0);
+                    } else {
+                        hi[0] = hi[1] = hi[2] = hi[3] = -INFINITY;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            shape32<MODE>(s + q * 32, x, q * 32);
+                            if (masked) mask32(s + q * 32, x, q * 32);
+                            max32(hi, s + q * 32);
+                        }
+                        mx = max3_nan(max3_nan(hi[0], hi[1], hi[2]), hi[3], hi[3]);
+                    }
+                }
+                s_is_read();
                 const bool set = fresh ? mx != -INFINITY : mx > base + SLACK;
-                if (__any_sync(0xffffffffu, set)) {
+                const bool move = __any_sync(0xffffffffu, set);
+                wait_product();
+                if (move) {
                     float alpha = 1.0f;
                     if (set) {
                         const float nb = ceilf(mx) - SHIFT;
@@ -489,43 +615,57 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                         for (int d = 0; d < DP; d += 32) scale_o(tO + d, alpha);
                     }
                 }
-                const uint64_t c2 = pack2(x.c1, x.c1), nb2 = pack2(-base, -base);
+                // (SEP) The exponentials of the two tiles take turns (side by side both would wait for MUFU,
+                // then both for their products): tile 1 follows tile 0 in each step that both take, tile 0
+                // follows tile 1's step before.
+                if (SEP && active(w ^ 1, i + w - 1))
+                    ok = __all_sync(0xffffffffu, mbar_wait(turn + w, turns++ & 1, abort_flag, 63, tc.dev_error));
+                const uint64_t nb2 = pack2(-base, -base);
                 uint64_t sum2[4] = {0, 0, 0, 0};
+                auto probs = [&](auto arg) {   // arg: two entries of s -> two exponents
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t pk[16];
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int j = q * 32 + 2 * e;
-                        const uint64_t t2 = pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-                        float u, v;
-                        unpack2(MODE == 0 ? fma2(t2, c2, nb2) : add2(t2, nb2), u, v);
-                        u = ex2_approx(u);
-                        v = ex2_approx(v);
-                        sum2[e & 3] = add2(sum2[e & 3], pack2(u, v));
-                        pk[e] = pack16<BF16>(u, v);   // rounded to the type of v: what tensor cores multiply
+                        for (int e = 0; e < 16; e++) {
+                            const int j = q * 32 + 2 * e;
+                            float u, v;
+                            unpack2(arg(pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), j), u, v);
+                            u = ex2_approx(u);
+                            v = ex2_approx(v);
+                            sum2[e & 3] = add2(sum2[e & 3], pack2(u, v));
+                            pk[e] = pack16<BF16>(u, v);   // rounded to the type of v: what tensor cores multiply
+                        }
+                        tmem_st16(tP + q * 16, pk);
+                        if (!SEP && q == 1) half_done();
                     }
-                    tmem_st16(tP + q * 16, pk);
+                };
+                const uint64_t c2 = pack2(x.c1, x.c1);
+                if (MODE == CAP && raw) {
+                    const uint64_t k0 = pack2(x.k0, x.k0), k1 = pack2(x.k1, x.k1), k2 = pack2(x.k2, x.k2);
+                    probs([&](uint64_t t, int) {
+                        const uint64_t w2 = mul2(t, t);
+                        return fma2(t, fma2(fma2(w2, k2, k1), w2, k0), nb2);
+                    });
+                } else if ((MODE & SLOPE) && raw) {
+                    const float la = x.lin_a - base;
+                    probs([&](uint64_t t, int j) {
+                        return fma2(t, c2, pack2(fmaf((float)j, x.lin_b, la), fmaf((float)(j + 1), x.lin_b, la)));
+                    });
+                } else if (!(MODE & CAP) && raw) {
+                    const uint64_t la2 = pack2(x.lin_a - base, x.lin_a - base);
+                    probs([&](uint64_t t, int) { return fma2(t, c2, la2); });
+                } else {
+                    probs([&](uint64_t t, int) { return add2(t, nb2); });
                 }
                 float e0, e1, e2, e3;
                 unpack2(add2(sum2[0], sum2[1]), e0, e1);
                 unpack2(add2(sum2[2], sum2[3]), e2, e3);
                 l += (e0 + e1) + (e2 + e3);
+                if (mx != mx) l = mx;   // a NaN score: the row is NaN
             }
-            // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
-            if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && active(0, kt))) {
-                const int st = (kt - lo_all) % NST;
-                ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, ((kt - lo_all) / NST) & 1, abort_flag, 59, tc.dev_error));
-                if (!ok) break;
-                if (r >= rb.len - kt * KT) {
-#pragma unroll
-                    for (int sl = 0; sl < NSLAB; sl++)
-#pragma unroll
-                        for (int ch = 0; ch < 8; ch++)
-                            *reinterpret_cast<uint4*>(sV + st * TB + sl * SLAB + r * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_async_smem();
-            }
+            __syncwarp();
+            if (SEP && lane == 0 && active(w ^ 1, i + w)) mbar_arrive(turn + (w ^ 1));
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -537,7 +677,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         if (ok && w < tc.tiles_per_cta && q0 + w * QT + (warp & 3) * 32 < a.Sq) {
             const bool any = n_w > 0 && !fresh;
             const float inv = any ? 1.0f / l : 0.0f;
-            const long long row = ((long long)b * a.Sq + i) * a.Hq + h, id = (long long)split * a.B * a.Sq * a.Hq + row;
+            const long long row = ((long long)b * a.Sq + row_i) * a.Hq + h, id = (long long)split * a.B * a.Sq * a.Hq + row;
             if (c.nsplit > 1 && live) c.mlpart[id] = make_float2(any ? base : -INFINITY, l);
             uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b * a.out_stride[0] + qi * a.out_stride[1] + h * a.out_stride[2];
             bool bad = false;
@@ -578,10 +718,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             while (todo) {
                 const int k = __ffs(todo) - 1;
                 todo &= todo - 1;
-                const int row_i = q0 + w * QT + (warp & 3) * 32 + k;
+                const int bad_i = q0 + w * QT + (warp & 3) * 32 + k;
                 float o[4];
-                exact_row<BF16>(a, c.g, b, h, row_i, o);
-                const long long at = b * a.out_stride[0] + row_i * a.out_stride[1] + h * a.out_stride[2];
+                exact_row<BF16>(a, c.g, b, h, bad_i, o);
+                const long long at = b * a.out_stride[0] + bad_i * a.out_stride[1] + h * a.out_stride[2];
 #pragma unroll
                 for (int u = 0; u < 4; u++)
                     if (lane + 32 * u < a.D) store16<BF16>(a.out, at + lane + 32 * u, o[u]);

@@ -99,6 +99,9 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d;
 }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {   // NaN if any is
+    float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d;
+}
 __device__ __forceinline__ float min3(float a, float b, float c) {
     float d; asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d;
 }
