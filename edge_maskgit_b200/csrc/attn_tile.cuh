@@ -193,8 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     uint64_t* p_full = s_full + 2;         // [2] P is in TMEM (4 warps)
     uint64_t* o_full = p_full + 2;         // [2] a product with P is done
     uint64_t* s_free = o_full + 2;         // [2] S was read (4 warps; SEP)
-    uint64_t* turn = s_free + 2;           // [2] the other tile's exponentials are done (4 warps)
-    uint64_t* p_half = turn + 2;           // [2] the first half of P is in TMEM (4 warps)
+    uint64_t* p_half = s_free + 2;           // [2] the first half of P is in TMEM (4 warps)
     uint32_t* tmem_slot = (uint32_t*)(p_half + 2);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     int* range = (int*)(tmem_slot + 2);    // lo0, lo1, hi0, hi1, then a tile's lowest / highest document
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(q_full + i, 1); mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(o_full + i, 1);
-            mbar_init(s_free + i, 4); mbar_init(turn + i, 4); mbar_init(p_half + i, 4);
+            mbar_init(s_free + i, 4); mbar_init(p_half + i, 4);
         }
         for (int i = 0; i < NST; i++) {
             mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
@@ -390,8 +389,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     np[w]++;
                 };
                 if (SEP) {
-                    score(0); score(1);
-                    product(0); product(1);
+                    score(0); product(0);
+                    score(1); product(1);
                 } else {   // S(i + 1) takes the place of P(i)
                     product(0); score(0);
                     product(1); score(1);
@@ -454,13 +453,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         };
         float base = 0.0f, l = 0.0f;
         bool fresh = true, ok = true;   // fresh: the row has seen nothing yet, base is not set
-        const int n_w = on[w] ? hi[w] - lo[w] : 0;
-        int i = 0, it = 0, turns = 0;   // step, this tile's steps so far, turns waited for
-        while (i < n && !active(w, i)) i++;
+        // (selected, not indexed by w: arrays would go to local memory)
+        const int lo_w = w ? lo[1] : lo[0], hi_w = w ? hi[1] : hi[0], n_w = max(0, hi_w - lo_w);
+        const int lo_o = w ? lo[0] : lo[1], hi_o = w ? hi[0] : hi[1];
+        auto mine = [&](int i) { const int kt = order(i); return kt >= lo_w && kt < hi_w; };
+        auto others = [&](int i) { const int kt = order(i); return i >= 0 && i < n && kt >= lo_o && kt < hi_o; };
+        int i = 0, it = 0;   // step, this tile's steps so far
+        while (i < n && !mine(i)) i++;
         if (n_w > 0) fetch(order(i));
         for (int next; it < n_w; i = next, it++) {
             const int kt = order(i), buf = it & 1;
-            for (next = i + 1; next < n && !active(w, next);) next++;
+            for (next = i + 1; next < n && !mine(next);) next++;
             // all of the tile's distances beyond the table's range on one side: one bias for all
             const int dist_lo = kt * KT - (rb.pos0 + q0 + w * QT) - 127, dist_hi = dist_lo + 254;
             const bool flat = (MODE & TABLE) && (dist_lo >= sh.range || dist_hi <= -sh.range);
@@ -501,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             if (!ok) break;
             tc_fence_after();
             // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
-            if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && active(0, i))) {
+            if (rb.len < a.Sk && rb.len - kt * KT < KT && rb.len > kt * KT && !(w == 1 && others(i))) {
                 const int st = i % NST;
                 ok = __all_sync(0xffffffffu, mbar_wait(v_full + st, (i / NST) & 1, abort_flag, 59, tc.dev_error));
                 if (!ok) break;
@@ -615,11 +618,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                         for (int d = 0; d < DP; d += 32) scale_o(tO + d, alpha);
                     }
                 }
-                // (SEP) The exponentials of the two tiles take turns (side by side both would wait for MUFU,
-                // then both for their products): tile 1 follows tile 0 in each step that both take, tile 0
-                // follows tile 1's step before.
-                if (SEP && active(w ^ 1, i + w - 1))
-                    ok = __all_sync(0xffffffffu, mbar_wait(turn + w, turns++ & 1, abort_flag, 63, tc.dev_error));
                 const uint64_t nb2 = pack2(-base, -base);
                 uint64_t sum2[4] = {0, 0, 0, 0};
                 auto probs = [&](auto arg) {   // arg: two entries of s -> two exponents
@@ -664,8 +662,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 l += (e0 + e1) + (e2 + e3);
                 if (mx != mx) l = mx;   // a NaN score: the row is NaN
             }
-            __syncwarp();
-            if (SEP && lane == 0 && active(w ^ 1, i + w)) mbar_arrive(turn + (w ^ 1));
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
