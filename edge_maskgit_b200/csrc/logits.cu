@@ -4,10 +4,12 @@
 //   z += bias[v];   z = -inf where the token's bit is 0
 //
 // Bound by memory: each logit is read and written once, everything else (a row's history, a shared
-// bias or mask) comes from L2.  One CTA owns kChunk consecutive tokens of one row.  It counts the
-// row's history into shared memory for those tokens only, so counting needs neither a second
-// kernel nor a [R][V] table in global memory: the price is that each of a row's chunks reads the
-// history again, which stays in L2.  The logits' own loads are issued before the count.
+// bias or mask) comes from L2.  One CTA owns a chunk of consecutive tokens of one row.  It counts the
+// row's history into shared memory for those tokens only, so counting needs neither a second kernel
+// nor a [R][V] table in global memory: the price is that each of a row's chunks reads the history
+// again, from L2.  Chunks are up to 8192 tokens, which keeps that small; with few rows they are
+// shorter, so that all SMs have work.  After the count each warp streams its own segments, the next
+// one's logits and bias on their way while it works on this one, with no barrier between warps.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -18,11 +20,11 @@
 namespace mgc {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 
 struct LogitArgs {
     const void* z; long long ld;
-    int R, V, chunks;
+    int R, V, chunks, segs;   // segs: segments of 32 vectors per warp and chunk
     const int32_t* hist; long long ld_hist; int L;
     const int32_t* hist_len;
     const float* pen; long long ld_pen;
@@ -31,12 +33,9 @@ struct LogitArgs {
     void* out; long long ld_out;
 };
 
-// One logit: the formulas above, in f32.
-__device__ __forceinline__ float adjust(float z, uint32_t count, float rep, float freq, float pres, float bias,
-                                        bool allowed) {
-    if (count) z = (z > 0.0f ? z / rep : z * rep) - (freq * (float)count + pres);
-    z += bias;
-    return allowed ? z : -INFINITY;
+// A token that the history holds `count` times.
+__device__ __forceinline__ float penalise(float z, uint32_t count, float rep, float freq, float pres) {
+    return count ? (z > 0.0f ? z / rep : z * rep) - (freq * (float)count + pres) : z;
 }
 
 template <int DT> struct Elem;   // DT: 0 f32, 1 f16, 2 bf16; a 16-byte vector holds N values
@@ -63,104 +62,113 @@ template <bool BF16> struct Elem16 {
 template <> struct Elem<1> : Elem16<false> {};
 template <> struct Elem<2> : Elem16<true> {};
 
-// VPT 16-byte vectors per thread.  A chunk starts at a 16-byte boundary of the logits' memory, so
-// rows that begin in the middle of one (odd V) still load whole vectors: chunk c of a row holds
-// tokens [c * CHUNK - lead, (c + 1) * CHUNK - lead), lead = the values between the boundary below
-// the row's first logit and that logit.
-template <int DT, int VPT, bool HIST, bool BIAS, bool MASK>
-__global__ void __launch_bounds__(kThreads) logits_adjust_kernel(const LogitArgs a) {
+// A chunk starts at a 16-byte boundary of the logits' memory, so rows that begin in the middle of one
+// (odd V) still move whole vectors: chunk c of a row holds tokens [c * chunk - lead, ...), lead = the
+// values between the boundary below the row's first logit and that logit.
+template <int DT, bool HIST, bool BIAS, bool MASK>
+__global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitArgs a) {
     using E = Elem<DT>;
-    constexpr int N = E::N, CHUNK = kThreads * VPT * N;
-    __shared__ __align__(16) uint32_t s_count[HIST ? CHUNK : 4];
-    __shared__ __align__(16) float s_bias[BIAS ? CHUNK : 4];
+    constexpr int N = E::N, SEG = 32 * N;
+    extern __shared__ __align__(16) uint32_t s_count[];   // [chunk]
+    __shared__ __align__(16) float s_bias[BIAS ? kWarps * 2 * SEG : 4];
     griddep_wait();
     griddep_launch();
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int chunk = a.segs * kWarps * SEG;
     const long long r = blockIdx.x / a.chunks;
     const int c = (int)(blockIdx.x % a.chunks);
     const char* zrow = reinterpret_cast<const char*>(a.z) + r * a.ld * E::SIZE;
     char* orow = reinterpret_cast<char*>(a.out) + r * a.ld_out * E::SIZE;
     const int lead = (int)((reinterpret_cast<uintptr_t>(zrow) & 15) / E::SIZE);
     const bool out_vec = ((reinterpret_cast<uintptr_t>(zrow) ^ reinterpret_cast<uintptr_t>(orow)) & 15) == 0;
-    const long long t0 = (long long)c * CHUNK - lead;   // token of the chunk's first value (may be < 0)
+    const long long t0 = (long long)c * chunk - lead;   // token of the chunk's first value (may be < 0)
+    const float* brow = BIAS ? a.bias + r * a.ld_bias : nullptr;
 
-    uint4 v[VPT];
-    auto first = [&](int i) { return t0 + (long long)(i * kThreads + tid) * N; };
+    auto seg_at = [&](int k) { return (k * kWarps + warp) * SEG; };   // segment k's place in the chunk
     auto whole = [&](long long t) { return t >= 0 && t + N <= a.V; };
+    auto fetch = [&](int k, uint4& v) {   // this lane's logits, and the segment's bias
+        const long long t = t0 + seg_at(k) + lane * N;
+        if (whole(t)) v = *reinterpret_cast<const uint4*>(zrow + t * E::SIZE);
+        if (BIAS) {   // 4-byte copies: a row of an odd-sized table starts anywhere
+            float* dst = s_bias + (warp * 2 + (k & 1)) * SEG;
 #pragma unroll
-    for (int i = 0; i < VPT; i++) {
-        const long long t = first(i);
-        if (whole(t)) v[i] = *reinterpret_cast<const uint4*>(zrow + t * E::SIZE);
-    }
-    if (BIAS) {   // 4-byte copies: a row of an odd-sized table starts anywhere
-        const float* b = a.bias + r * a.ld_bias;
-#pragma unroll 4
-        for (int i = tid; i < CHUNK; i += kThreads) {
-            const long long t = t0 + i;
-            if (t >= 0 && t < a.V)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(s_bias + i)), "l"(b + t) : "memory");
+            for (int j = 0; j < N; j++) {
+                const long long x = t0 + seg_at(k) + j * 32 + lane;
+                if (x >= 0 && x < a.V)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst + j * 32 + lane)), "l"(brow + x) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-    }
+    };
+    uint4 next = make_uint4(0, 0, 0, 0);
+    fetch(0, next);
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     bool any = false;
     if (HIST) {
-        for (int i = tid; i < CHUNK / 4; i += kThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
         int n = a.L;
         if (a.hist_len) n = max(0, min(a.L, __ldg(a.hist_len + r)));
         const float* pen = a.pen + r * a.ld_pen;
         rep = __ldg(pen); freq = __ldg(pen + 1); pres = __ldg(pen + 2);
+        for (int i = tid; i < chunk / 4; i += kThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         const int32_t* h = a.hist + r * a.ld_hist;
-#pragma unroll 4
+        const long long end = min(t0 + chunk, (long long)a.V);
+#pragma unroll 8
         for (int i = tid; i < n; i += kThreads) {
             const int tok = __ldg(h + i);
-            const long long at = tok - t0;
-            if (tok >= 0 && tok < a.V && at >= 0 && at < CHUNK) {
-                atomicAdd(s_count + at, 1u);   // integers: the order does not matter
+            if (tok >= 0 && tok >= t0 && tok < end) {
+                atomicAdd(s_count + (tok - t0), 1u);   // integers: the order does not matter
                 any = true;
             }
         }
+        any = __syncthreads_or(any);
     }
-    if (BIAS) cp_async_wait_all();
-    if (HIST) any = __syncthreads_or(any);
-    else if (BIAS) __syncthreads();
 
     const uint32_t* mask = MASK ? a.allowed + r * a.ld_allowed : nullptr;
-#pragma unroll
-    for (int i = 0; i < VPT; i++) {
-        const long long t = first(i);
-        const int at = (i * kThreads + tid) * N;
+#pragma unroll 1
+    for (int k = 0; k < a.segs; k++) {
+        const uint4 v = next;
+        if (k + 1 < a.segs) fetch(k + 1, next);
+        if (BIAS) {
+            if (k + 1 < a.segs) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
+        }
+        const int at = seg_at(k) + lane * N;
+        const long long t = t0 + at;
+        const float* sb = s_bias + (BIAS ? (warp * 2 + (k & 1)) * SEG + lane * N : 0);
         if (whole(t)) {
-            float b[N];
-            uint32_t n[N], bits = ~0u;
-            if (BIAS) {
+            float z[N];
 #pragma unroll
-                for (int j = 0; j < N; j += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(s_bias + at + j);
-                    b[j] = f.x; b[j + 1] = f.y; b[j + 2] = f.z; b[j + 3] = f.w;
-                }
-            }
+            for (int j = 0; j < N; j++) z[j] = E::get(v, j);
             if (HIST && any) {
 #pragma unroll
                 for (int j = 0; j < N; j += 4) {
                     const uint4 u = *reinterpret_cast<const uint4*>(s_count + at + j);
-                    n[j] = u.x; n[j + 1] = u.y; n[j + 2] = u.z; n[j + 3] = u.w;
+                    if (u.x | u.y | u.z | u.w) {
+                        z[j] = penalise(z[j], u.x, rep, freq, pres);
+                        z[j + 1] = penalise(z[j + 1], u.y, rep, freq, pres);
+                        z[j + 2] = penalise(z[j + 2], u.z, rep, freq, pres);
+                        z[j + 3] = penalise(z[j + 3], u.w, rep, freq, pres);
+                    }
                 }
-            } else {
+            }
+            if (BIAS) {
 #pragma unroll
-                for (int j = 0; j < N; j++) n[j] = 0;
+                for (int j = 0; j < N; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(sb + j);
+                    z[j] += f.x; z[j + 1] += f.y; z[j + 2] += f.z; z[j + 3] += f.w;
+                }
             }
             if (MASK) {   // N bits from token t on: at most two words
-                const uint32_t lo = __ldg(mask + (t >> 5));
-                const uint32_t hi = __ldg(mask + ((t + N - 1) >> 5));
-                bits = __funnelshift_r(lo, hi, (uint32_t)(t & 31));
+                const uint32_t lo = __ldg(mask + (t >> 5)), hi = __ldg(mask + ((t + N - 1) >> 5));
+                const uint32_t bits = __funnelshift_r(lo, hi, (uint32_t)(t & 31));
+#pragma unroll
+                for (int j = 0; j < N; j++) z[j] = bits >> j & 1 ? z[j] : -INFINITY;
             }
             uint4 o;
 #pragma unroll
-            for (int j = 0; j < N; j += 2)
-                E::set2(o, j,
-                        adjust(E::get(v[i], j), n[j], rep, freq, pres, BIAS ? b[j] : 0.0f, bits >> j & 1),
-                        adjust(E::get(v[i], j + 1), n[j + 1], rep, freq, pres, BIAS ? b[j + 1] : 0.0f, bits >> (j + 1) & 1));
+            for (int j = 0; j < N; j += 2) E::set2(o, j, z[j], z[j + 1]);
             if (out_vec) *reinterpret_cast<uint4*>(orow + t * E::SIZE) = o;
             else {
 #pragma unroll
@@ -171,35 +179,43 @@ __global__ void __launch_bounds__(kThreads) logits_adjust_kernel(const LogitArgs
             for (int j = 0; j < N; j++) {
                 const long long x = t + j;
                 if (x < 0 || x >= a.V) continue;
-                const bool ok = !MASK || (__ldg(mask + (x >> 5)) >> (x & 31) & 1);
-                E::store(orow, x, adjust(E::load(zrow, x), HIST ? s_count[at + j] : 0, rep, freq, pres,
-                                         BIAS ? s_bias[at + j] : 0.0f, ok));
+                float z = E::load(zrow, x);
+                if (HIST && s_count[at + j]) z = penalise(z, s_count[at + j], rep, freq, pres);
+                if (BIAS) z += sb[j];
+                if (MASK && !(__ldg(mask + (x >> 5)) >> (x & 31) & 1)) z = -INFINITY;
+                E::store(orow, x, z);
             }
         }
+        if (BIAS) __syncwarp();   // the bias was read before its place is filled again
     }
 }
 
-template <int DT, int VPT>
+template <int DT>
 void launch_logits(LogitArgs& a, cudaStream_t st) {
-    constexpr int CHUNK = kThreads * VPT * Elem<DT>::N;
+    constexpr int SEG = 32 * Elem<DT>::N;
+    const int sms = current_sms();
     // a row may start up to N - 1 values past a boundary
-    a.chunks = (int)(((long long)a.V + Elem<DT>::N - 1 + CHUNK - 1) / CHUNK);
+    auto chunks = [&](int segs) { return ((long long)a.V + Elem<DT>::N - 1 + kWarps * segs * SEG - 1) / (kWarps * segs * SEG); };
+    a.segs = 8192 / (kWarps * SEG);
+    while (a.segs > 1 && chunks(a.segs) * a.R < 4LL * sms) a.segs /= 2;
+    a.chunks = (int)chunks(a.segs);
     const long long grid = (long long)a.chunks * a.R;
     if (grid > 0x7fffffffLL) throw std::runtime_error("R * V is too large for one launch");
     const bool h = a.hist, b = a.bias, m = a.allowed;
+    const size_t smem = h ? (size_t)a.segs * kWarps * SEG * 4 : 0;   // at most 32 KB
     auto go = [&](auto kernel) {
         ++g_launch_count;
-        const cudaError_t e = launch_k(kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, a);
+        const cudaError_t e = launch_k(kernel, dim3((unsigned)grid), dim3(kThreads), smem, st, a);
         if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
     };
-    if (h && b && m) go(logits_adjust_kernel<DT, VPT, true, true, true>);
-    else if (h && b) go(logits_adjust_kernel<DT, VPT, true, true, false>);
-    else if (h && m) go(logits_adjust_kernel<DT, VPT, true, false, true>);
-    else if (h) go(logits_adjust_kernel<DT, VPT, true, false, false>);
-    else if (b && m) go(logits_adjust_kernel<DT, VPT, false, true, true>);
-    else if (b) go(logits_adjust_kernel<DT, VPT, false, true, false>);
-    else if (m) go(logits_adjust_kernel<DT, VPT, false, false, true>);
-    else go(logits_adjust_kernel<DT, VPT, false, false, false>);
+    if (h && b && m) go(logits_adjust_kernel<DT, true, true, true>);
+    else if (h && b) go(logits_adjust_kernel<DT, true, true, false>);
+    else if (h && m) go(logits_adjust_kernel<DT, true, false, true>);
+    else if (h) go(logits_adjust_kernel<DT, true, false, false>);
+    else if (b && m) go(logits_adjust_kernel<DT, false, true, true>);
+    else if (b) go(logits_adjust_kernel<DT, false, true, false>);
+    else if (m) go(logits_adjust_kernel<DT, false, false, true>);
+    else go(logits_adjust_kernel<DT, false, false, false>);
 }
 
 }  // namespace
@@ -230,11 +246,11 @@ extern "C" int mgc_logits_adjust(int dtype, const void* z, int64_t ld, int R, in
         need(!bias || ld_bias == 0 || ld_bias >= V, "ld_bias must be 0 or at least V");
         need(!allowed || ld_allowed == 0 || ld_allowed >= ((int64_t)V + 31) / 32,
              "ld_allowed must be 0 or at least (V + 31) / 32");
-        LogitArgs a{z, ld, R, V, 0, hist, ld_hist, L, hist_len, pen, ld_pen, bias, ld_bias, allowed, ld_allowed, out, ld_out};
+        LogitArgs a{z, ld, R, V, 0, 0, hist, ld_hist, L, hist_len, pen, ld_pen, bias, ld_bias, allowed, ld_allowed, out, ld_out};
         if (L == 0) a.hist = nullptr;   // an empty history
         const cudaStream_t st = (cudaStream_t)stream;
-        if (dtype == MGC_F32) launch_logits<0, 4>(a, st);
-        else if (dtype == MGC_F16) launch_logits<1, 2>(a, st);
-        else launch_logits<2, 2>(a, st);
+        if (dtype == MGC_F32) launch_logits<0>(a, st);
+        else if (dtype == MGC_F16) launch_logits<1>(a, st);
+        else launch_logits<2>(a, st);
     });
 }
