@@ -24,7 +24,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 
 struct LogitArgs {
     const void* z; long long ld;
-    int R, V, chunks, segs;   // segs: segments of 32 vectors per warp and chunk
+    int R, V, chunks;
     const int32_t* hist; long long ld_hist; int L;
     const int32_t* hist_len;
     const float* pen; long long ld_pen;
@@ -65,7 +65,9 @@ template <> struct Elem<2> : Elem16<true> {};
 // A chunk starts at a 16-byte boundary of the logits' memory, so rows that begin in the middle of one
 // (odd V) still move whole vectors: chunk c of a row holds tokens [c * chunk - lead, ...), lead = the
 // values between the boundary below the row's first logit and that logit.
-template <int DT, bool HIST, bool BIAS, bool MASK>
+// SEGS: segments of 32 vectors per warp and chunk; their logits are all requested at the start (a
+// warp that fetched one segment ahead kept 16 KB per SM in flight: 2 TB/s).
+template <int DT, int SEGS, bool HIST, bool BIAS, bool MASK>
 __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitArgs a) {
     using E = Elem<DT>;
     constexpr int N = E::N, SEG = 32 * N;
@@ -74,34 +76,36 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitA
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int chunk = a.segs * kWarps * SEG;
+    constexpr int chunk = SEGS * kWarps * SEG;
     const long long r = blockIdx.x / a.chunks;
     const int c = (int)(blockIdx.x % a.chunks);
     const char* zrow = reinterpret_cast<const char*>(a.z) + r * a.ld * E::SIZE;
     char* orow = reinterpret_cast<char*>(a.out) + r * a.ld_out * E::SIZE;
     const int lead = (int)((reinterpret_cast<uintptr_t>(zrow) & 15) / E::SIZE);
     const bool out_vec = ((reinterpret_cast<uintptr_t>(zrow) ^ reinterpret_cast<uintptr_t>(orow)) & 15) == 0;
-    const long long t0 = (long long)c * chunk - lead;   // token of the chunk's first value (may be < 0)
+    const int t0 = c * chunk - lead;   // token of the chunk's first value (may be < 0); V + chunk < 2^31
     const float* brow = BIAS ? a.bias + r * a.ld_bias : nullptr;
 
     auto seg_at = [&](int k) { return (k * kWarps + warp) * SEG; };   // segment k's place in the chunk
-    auto whole = [&](long long t) { return t >= 0 && t + N <= a.V; };
-    auto fetch = [&](int k, uint4& v) {   // this lane's logits, and the segment's bias
-        const long long t = t0 + seg_at(k) + lane * N;
-        if (whole(t)) v = *reinterpret_cast<const uint4*>(zrow + t * E::SIZE);
-        if (BIAS) {   // 4-byte copies: a row of an odd-sized table starts anywhere
-            float* dst = s_bias + (warp * 2 + (k & 1)) * SEG;
+    auto inside = [&](int t) { return t >= 0 && t + SEG <= a.V; };      // a segment without a row's end
+    auto fetch_bias = [&](int k) {   // an inner segment's; 4-byte copies: a row of an odd-sized table starts anywhere
+        const int t = t0 + seg_at(k);
+        if (inside(t)) {
+            const uint32_t dst = smem_u32(s_bias + (warp * 2 + (k & 1)) * SEG + lane);
+            const float* src = brow + t + lane;
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const long long x = t0 + seg_at(k) + j * 32 + lane;
-                if (x >= 0 && x < a.V)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst + j * 32 + lane)), "l"(brow + x) : "memory");
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            for (int j = 0; j < N; j++)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + j * 128), "l"(src + j * 32) : "memory");
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    uint4 next = make_uint4(0, 0, 0, 0);
-    fetch(0, next);
+    uint4 v[SEGS];
+#pragma unroll
+    for (int k = 0; k < SEGS; k++) {
+        const int t = t0 + seg_at(k);
+        if (inside(t)) v[k] = *reinterpret_cast<const uint4*>(zrow + (long long)(t + lane * N) * E::SIZE);
+    }
+    if (BIAS) fetch_bias(0);
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     bool any = false;
     if (HIST) {
@@ -112,11 +116,12 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitA
         for (int i = tid; i < chunk / 4; i += kThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         const int32_t* h = a.hist + r * a.ld_hist;
-        const long long end = min(t0 + chunk, (long long)a.V);
+        const int first = max(t0, 0);
+        const unsigned span = (unsigned)(min(t0 + chunk, a.V) - first);   // > 0
 #pragma unroll 8
         for (int i = tid; i < n; i += kThreads) {
             const int tok = __ldg(h + i);
-            if (tok >= 0 && tok >= t0 && tok < end) {
+            if ((unsigned)tok - (unsigned)first < span) {   // (a negative number is a large one)
                 atomicAdd(s_count + (tok - t0), 1u);   // integers: the order does not matter
                 any = true;
             }
@@ -125,22 +130,23 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitA
     }
 
     const uint32_t* mask = MASK ? a.allowed + r * a.ld_allowed : nullptr;
-#pragma unroll 1
-    for (int k = 0; k < a.segs; k++) {
-        const uint4 v = next;
-        if (k + 1 < a.segs) fetch(k + 1, next);
+#pragma unroll
+    for (int k = 0; k < SEGS; k++) {
         if (BIAS) {
-            if (k + 1 < a.segs) asm volatile("cp.async.wait_group 1;" ::: "memory");
-            else asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (k + 1 < SEGS) {
+                fetch_bias(k + 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
             __syncwarp();
         }
-        const int at = seg_at(k) + lane * N;
-        const long long t = t0 + at;
+        const int at = seg_at(k) + lane * N, t = t0 + at;
         const float* sb = s_bias + (BIAS ? (warp * 2 + (k & 1)) * SEG + lane * N : 0);
-        if (whole(t)) {
+        if (inside(t0 + seg_at(k))) {
             float z[N];
 #pragma unroll
-            for (int j = 0; j < N; j++) z[j] = E::get(v, j);
+            for (int j = 0; j < N; j++) z[j] = E::get(v[k], j);
             if (HIST && any) {
 #pragma unroll
                 for (int j = 0; j < N; j += 4) {
@@ -169,19 +175,19 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitA
             uint4 o;
 #pragma unroll
             for (int j = 0; j < N; j += 2) E::set2(o, j, z[j], z[j + 1]);
-            if (out_vec) *reinterpret_cast<uint4*>(orow + t * E::SIZE) = o;
+            if (out_vec) *reinterpret_cast<uint4*>(orow + (long long)t * E::SIZE) = o;
             else {
 #pragma unroll
                 for (int j = 0; j < N; j++) E::store(orow, t + j, E::get(o, j));
             }
-        } else {   // a row's first or last few logits
+        } else {   // the segment of a row's first or last logits
 #pragma unroll 1
             for (int j = 0; j < N; j++) {
-                const long long x = t + j;
+                const int i = seg_at(k) + j * 32 + lane, x = t0 + i;
                 if (x < 0 || x >= a.V) continue;
                 float z = E::load(zrow, x);
-                if (HIST && s_count[at + j]) z = penalise(z, s_count[at + j], rep, freq, pres);
-                if (BIAS) z += sb[j];
+                if (HIST) z = penalise(z, s_count[i], rep, freq, pres);
+                if (BIAS) z += __ldg(brow + x);
                 if (MASK && !(__ldg(mask + (x >> 5)) >> (x & 31) & 1)) z = -INFINITY;
                 E::store(orow, x, z);
             }
@@ -190,32 +196,37 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitA
     }
 }
 
-template <int DT>
-void launch_logits(LogitArgs& a, cudaStream_t st) {
-    constexpr int SEG = 32 * Elem<DT>::N;
-    const int sms = current_sms();
-    // a row may start up to N - 1 values past a boundary
-    auto chunks = [&](int segs) { return ((long long)a.V + Elem<DT>::N - 1 + kWarps * segs * SEG - 1) / (kWarps * segs * SEG); };
-    a.segs = 8192 / (kWarps * SEG);
-    while (a.segs > 1 && chunks(a.segs) * a.R < 4LL * sms) a.segs /= 2;
-    a.chunks = (int)chunks(a.segs);
-    const long long grid = (long long)a.chunks * a.R;
-    if (grid > 0x7fffffffLL) throw std::runtime_error("R * V is too large for one launch");
+template <int DT, int SEGS>
+void launch_segs(LogitArgs& a, long long chunks, cudaStream_t st) {
+    a.chunks = (int)chunks;
+    if (chunks * a.R > 0x7fffffffLL) throw std::runtime_error("R * V is too large for one launch");
     const bool h = a.hist, b = a.bias, m = a.allowed;
-    const size_t smem = h ? (size_t)a.segs * kWarps * SEG * 4 : 0;   // at most 32 KB
+    const size_t smem = h ? (size_t)SEGS * kWarps * 32 * Elem<DT>::N * 4 : 0;   // at most 32 KB
     auto go = [&](auto kernel) {
         ++g_launch_count;
-        const cudaError_t e = launch_k(kernel, dim3((unsigned)grid), dim3(kThreads), smem, st, a);
+        const cudaError_t e = launch_k(kernel, dim3((unsigned)(chunks * a.R)), dim3(kThreads), smem, st, a);
         if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
     };
-    if (h && b && m) go(logits_adjust_kernel<DT, true, true, true>);
-    else if (h && b) go(logits_adjust_kernel<DT, true, true, false>);
-    else if (h && m) go(logits_adjust_kernel<DT, true, false, true>);
-    else if (h) go(logits_adjust_kernel<DT, true, false, false>);
-    else if (b && m) go(logits_adjust_kernel<DT, false, true, true>);
-    else if (b) go(logits_adjust_kernel<DT, false, true, false>);
-    else if (m) go(logits_adjust_kernel<DT, false, false, true>);
-    else go(logits_adjust_kernel<DT, false, false, false>);
+    if (h && b && m) go(logits_adjust_kernel<DT, SEGS, true, true, true>);
+    else if (h && b) go(logits_adjust_kernel<DT, SEGS, true, true, false>);
+    else if (h && m) go(logits_adjust_kernel<DT, SEGS, true, false, true>);
+    else if (h) go(logits_adjust_kernel<DT, SEGS, true, false, false>);
+    else if (b && m) go(logits_adjust_kernel<DT, SEGS, false, true, true>);
+    else if (b) go(logits_adjust_kernel<DT, SEGS, false, true, false>);
+    else if (m) go(logits_adjust_kernel<DT, SEGS, false, false, true>);
+    else go(logits_adjust_kernel<DT, SEGS, false, false, false>);
+}
+
+// Long chunks read the history less often; short ones give every SM work when there are few rows.
+template <int DT>
+void launch_logits(LogitArgs& a, cudaStream_t st) {
+    constexpr int N = Elem<DT>::N;
+    const long long enough = 4LL * current_sms();
+    // a row may start up to N - 1 values past a boundary
+    auto chunks = [&](int segs) { return ((long long)a.V + N - 1 + kWarps * 32 * N * segs - 1) / (kWarps * 32 * N * segs); };
+    if (chunks(4) * a.R >= enough) launch_segs<DT, 4>(a, chunks(4), st);
+    else if (chunks(2) * a.R >= enough) launch_segs<DT, 2>(a, chunks(2), st);
+    else launch_segs<DT, 1>(a, chunks(1), st);
 }
 
 }  // namespace
@@ -231,6 +242,7 @@ extern "C" int mgc_logits_adjust(int dtype, const void* z, int64_t ld, int R, in
         auto need = [](bool ok, const char* m) { if (!ok) throw std::invalid_argument(m); };
         need(dtype == MGC_F32 || dtype == MGC_F16 || dtype == MGC_BF16, "dtype must be F32, F16 or BF16");
         need(R >= 0 && V >= 0 && L >= 0, "negative size");
+        need(V <= 1 << 30, "V must be at most 2^30");
         if (R == 0 || V == 0) return;
         need(z && out, "logits and out must not be NULL");
         need((hist != nullptr) == (pen != nullptr), "history and penalties are given together");
@@ -246,7 +258,7 @@ extern "C" int mgc_logits_adjust(int dtype, const void* z, int64_t ld, int R, in
         need(!bias || ld_bias == 0 || ld_bias >= V, "ld_bias must be 0 or at least V");
         need(!allowed || ld_allowed == 0 || ld_allowed >= ((int64_t)V + 31) / 32,
              "ld_allowed must be 0 or at least (V + 31) / 32");
-        LogitArgs a{z, ld, R, V, 0, 0, hist, ld_hist, L, hist_len, pen, ld_pen, bias, ld_bias, allowed, ld_allowed, out, ld_out};
+        LogitArgs a{z, ld, R, V, 0, hist, ld_hist, L, hist_len, pen, ld_pen, bias, ld_bias, allowed, ld_allowed, out, ld_out};
         if (L == 0) a.hist = nullptr;   // an empty history
         const cudaStream_t st = (cudaStream_t)stream;
         if (dtype == MGC_F32) launch_logits<0>(a, st);

@@ -172,7 +172,7 @@ int mgc_attention(const mgc_attention_args* args, void* stream);
  * values outside 0..V-1 are skipped.  penalties f32 [R][3]: rep, freq, pres; history and penalties
  * are given together or both NULL.  bias f32 [R][V], allowed [R][(V + 31) / 32], each may be NULL.
  * ld* are row strides in elements; 0 for history, penalties, bias or allowed shares one row among
- * all (with hist_len still [R]).  R = 0 or V = 0 is a no-op. */
+ * all (with hist_len still [R]).  V is at most 2^30; R = 0 or V = 0 is a no-op. */
 int mgc_logits_adjust(int dtype, const void* logits_dev, int64_t ld, int R, int V,
                       const int32_t* history_dev, int64_t ld_history, int L, const int32_t* hist_len_dev,
                       const float* penalties_dev, int64_t ld_penalties, const float* bias_dev, int64_t ld_bias,
