@@ -7,7 +7,7 @@
 // bias or mask) comes from L2.  One CTA owns a chunk of consecutive tokens of one row.  It counts the
 // row's history into shared memory for those tokens only, so counting needs neither a second kernel
 // nor a [R][V] table in global memory: the price is that each of a row's chunks reads the history
-// again, from L2.  Chunks are up to 8192 tokens, which keeps that small; with few rows they are
+// again, from L2.  Chunks are up to 16384 tokens, which keeps that small; with few rows they are
 // shorter, so that all SMs have work.  After the count each warp streams its own segments, the next
 // one's logits and bias on their way while it works on this one, with no barrier between warps.
 #include <cuda_bf16.h>
@@ -20,7 +20,7 @@
 namespace mgc {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 
 struct LogitArgs {
     const void* z; long long ld;
@@ -68,7 +68,7 @@ template <> struct Elem<2> : Elem16<true> {};
 // SEGS: segments of 32 vectors per warp and chunk; their logits are all requested at the start (a
 // warp that fetched one segment ahead kept 16 KB per SM in flight: 2 TB/s).
 template <int DT, int SEGS, bool HIST, bool BIAS, bool MASK>
-__global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) logits_adjust_kernel(const LogitArgs a) {
     using E = Elem<DT>;
     constexpr int N = E::N, SEG = 32 * N;
     extern __shared__ __align__(16) uint32_t s_count[];   // [chunk]
@@ -118,14 +118,22 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitA
         const int32_t* h = a.hist + r * a.ld_hist;
         const int first = max(t0, 0);
         const unsigned span = (unsigned)(min(t0 + chunk, a.V) - first);   // > 0
-#pragma unroll 8
-        for (int i = tid; i < n; i += kThreads) {
-            const int tok = __ldg(h + i);
+        auto count = [&](int tok) {
             if ((unsigned)tok - (unsigned)first < span) {   // (a negative number is a large one)
                 atomicAdd(s_count + (tok - t0), 1u);   // integers: the order does not matter
                 any = true;
             }
+        };
+        // four at a time from the first 16-byte boundary on
+        const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4), quads = (n - head) / 4;
+        if (tid < head) count(__ldg(h + tid));
+#pragma unroll 4
+        for (int i = tid; i < quads; i += kThreads) {
+            const int4 q = __ldg(reinterpret_cast<const int4*>(h + head) + i);
+            count(q.x); count(q.y); count(q.z); count(q.w);
         }
+        const int done = head + quads * 4;
+        if (tid < n - done) count(__ldg(h + done + tid));
         any = __syncthreads_or(any);
     }
 
@@ -196,25 +204,29 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const LogitA
     }
 }
 
+template <int DT, int SEGS, bool HIST, bool BIAS, bool MASK>
+void launch_one(const LogitArgs& a, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto kernel = logits_adjust_kernel<DT, SEGS, HIST, BIAS, MASK>;
+    const uint32_t smem = HIST ? SEGS * kWarps * 32 * Elem<DT>::N * 4 : 0;   // at most 64 KB
+    if (smem) allow_smem(kernel, smem, done);
+    ++g_launch_count;
+    const cudaError_t e = launch_k(kernel, dim3((unsigned)((long long)a.chunks * a.R)), dim3(kThreads), smem, st, a);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+}
 template <int DT, int SEGS>
 void launch_segs(LogitArgs& a, long long chunks, cudaStream_t st) {
     a.chunks = (int)chunks;
     if (chunks * a.R > 0x7fffffffLL) throw std::runtime_error("R * V is too large for one launch");
     const bool h = a.hist, b = a.bias, m = a.allowed;
-    const size_t smem = h ? (size_t)SEGS * kWarps * 32 * Elem<DT>::N * 4 : 0;   // at most 32 KB
-    auto go = [&](auto kernel) {
-        ++g_launch_count;
-        const cudaError_t e = launch_k(kernel, dim3((unsigned)(chunks * a.R)), dim3(kThreads), smem, st, a);
-        if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
-    };
-    if (h && b && m) go(logits_adjust_kernel<DT, SEGS, true, true, true>);
-    else if (h && b) go(logits_adjust_kernel<DT, SEGS, true, true, false>);
-    else if (h && m) go(logits_adjust_kernel<DT, SEGS, true, false, true>);
-    else if (h) go(logits_adjust_kernel<DT, SEGS, true, false, false>);
-    else if (b && m) go(logits_adjust_kernel<DT, SEGS, false, true, true>);
-    else if (b) go(logits_adjust_kernel<DT, SEGS, false, true, false>);
-    else if (m) go(logits_adjust_kernel<DT, SEGS, false, false, true>);
-    else go(logits_adjust_kernel<DT, SEGS, false, false, false>);
+    if (h && b && m) launch_one<DT, SEGS, true, true, true>(a, st);
+    else if (h && b) launch_one<DT, SEGS, true, true, false>(a, st);
+    else if (h && m) launch_one<DT, SEGS, true, false, true>(a, st);
+    else if (h) launch_one<DT, SEGS, true, false, false>(a, st);
+    else if (b && m) launch_one<DT, SEGS, false, true, true>(a, st);
+    else if (b) launch_one<DT, SEGS, false, true, false>(a, st);
+    else if (m) launch_one<DT, SEGS, false, false, true>(a, st);
+    else launch_one<DT, SEGS, false, false, false>(a, st);
 }
 
 // Long chunks read the history less often; short ones give every SM work when there are few rows.

@@ -198,6 +198,26 @@ def test_logits_parts_shared_rows_in_place(dt, hist, bias, mask):
     assert torch.equal(again, want)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("parts", range(8))
+def test_logits_many_rows_of_many_tokens(dt, parts):
+    """Every combination of parts at a size where each row is cut into its longest chunks."""
+    from edge_maskgit_b200 import runtime as rt
+    R, V = 200, 60001
+    kw = {}
+    if parts & 1:
+        kw.update(history=ints(0, V, R, 33, seed=36), penalties=torch.tensor([1.4, 0.3, 0.2], device="cuda"))
+    if parts & 2:
+        kw.update(bias=randn(V, dtype=F32, seed=37))
+    if parts & 4:
+        kw.update(allowed=ints(-2 ** 31, 2 ** 31 - 1, R, (V + 31) // 32, seed=38))
+    z = randn(R, V, dtype=dt, seed=39, std=3.0)
+    y = rt.logits_adjust(z, **kw)
+    rows = [0, 1, 2, 7, 77, R - 1]
+    pick = {k: (v[rows] if v.dim() == 2 else v) for k, v in kw.items()}
+    within(y[rows], *logits_ref(z[rows], **pick))
+
+
 @pytest.mark.parametrize("dt", [F32, F16])
 def test_logits_strided_rows(dt):
     R, V = 4, 1003
