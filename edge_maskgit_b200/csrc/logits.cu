@@ -8,8 +8,8 @@
 // row's history into shared memory for those tokens only, so counting needs neither a second kernel
 // nor a [R][V] table in global memory: the price is that each of a row's chunks reads the history
 // again, from L2.  Chunks are up to 16384 tokens, which keeps that small; with few rows they are
-// shorter, so that all SMs have work.  After the count each warp streams its own segments, the next
-// one's logits and bias on their way while it works on this one, with no barrier between warps.
+// shorter, so that all SMs have work.  After the count each warp works on its own segments, with no barrier
+// between warps.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,6 +33,11 @@ struct LogitArgs {
     void* out; long long ld_out;
 };
 
+template <int N, int SHIFT>
+__device__ __forceinline__ void add_at(float (&z)[N], const float (&x)[N + 4]) {
+#pragma unroll
+    for (int j = 0; j < N; j++) z[j] += x[j + SHIFT];
+}
 // A token that the history holds `count` times.
 __device__ __forceinline__ float penalise(float z, uint32_t count, float rep, float freq, float pres) {
     return count ? (z > 0.0f ? z / rep : z * rep) - (freq * (float)count + pres) : z;
@@ -72,7 +77,6 @@ __global__ void __launch_bounds__(kThreads, 2) logits_adjust_kernel(const LogitA
     using E = Elem<DT>;
     constexpr int N = E::N, SEG = 32 * N;
     extern __shared__ __align__(16) uint32_t s_count[];   // [chunk]
-    __shared__ __align__(16) float s_bias[BIAS ? kWarps * 2 * SEG : 4];
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -87,25 +91,14 @@ __global__ void __launch_bounds__(kThreads, 2) logits_adjust_kernel(const LogitA
     const float* brow = BIAS ? a.bias + r * a.ld_bias : nullptr;
 
     auto seg_at = [&](int k) { return (k * kWarps + warp) * SEG; };   // segment k's place in the chunk
-    auto inside = [&](int t) { return t >= 0 && t + SEG <= a.V; };      // a segment without a row's end
-    auto fetch_bias = [&](int k) {   // an inner segment's; 4-byte copies: a row of an odd-sized table starts anywhere
-        const int t = t0 + seg_at(k);
-        if (inside(t)) {
-            const uint32_t dst = smem_u32(s_bias + (warp * 2 + (k & 1)) * SEG + lane);
-            const float* src = brow + t + lane;
-#pragma unroll
-            for (int j = 0; j < N; j++)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + j * 128), "l"(src + j * 32) : "memory");
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+    // a segment without a row's end (nor, where bias is read in aligned pieces, its neighbourhood)
+    auto inside = [&](int t) { return t >= (BIAS ? 4 : 0) && t + SEG + (BIAS ? 4 : 0) <= a.V; };
     uint4 v[SEGS];
 #pragma unroll
     for (int k = 0; k < SEGS; k++) {
         const int t = t0 + seg_at(k);
         if (inside(t)) v[k] = *reinterpret_cast<const uint4*>(zrow + (long long)(t + lane * N) * E::SIZE);
     }
-    if (BIAS) fetch_bias(0);
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     bool any = false;
     if (HIST) {
@@ -140,17 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_adjust_kernel(const LogitA
     const uint32_t* mask = MASK ? a.allowed + r * a.ld_allowed : nullptr;
 #pragma unroll
     for (int k = 0; k < SEGS; k++) {
-        if (BIAS) {
-            if (k + 1 < SEGS) {
-                fetch_bias(k + 1);
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
-            __syncwarp();
-        }
         const int at = seg_at(k) + lane * N, t = t0 + at;
-        const float* sb = s_bias + (BIAS ? (warp * 2 + (k & 1)) * SEG + lane * N : 0);
         if (inside(t0 + seg_at(k))) {
             float z[N];
 #pragma unroll
@@ -168,10 +151,22 @@ __global__ void __launch_bounds__(kThreads, 2) logits_adjust_kernel(const LogitA
                 }
             }
             if (BIAS) {
+                // aligned loads around the N values, which start at one of four places (the same for the warp)
+                const int shift = (int)(reinterpret_cast<uintptr_t>(brow + t) >> 2 & 3);
+                const float4* q = reinterpret_cast<const float4*>(brow + t - shift);
+                float x[N + 4];
 #pragma unroll
-                for (int j = 0; j < N; j += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(sb + j);
-                    z[j] += f.x; z[j + 1] += f.y; z[j + 2] += f.z; z[j + 3] += f.w;
+                for (int j = 0; j < N / 4; j++) {
+                    const float4 f = __ldg(q + j);
+                    x[4 * j] = f.x; x[4 * j + 1] = f.y; x[4 * j + 2] = f.z; x[4 * j + 3] = f.w;
+                }
+                if (shift == 0) add_at<N, 0>(z, x);
+                else {
+                    const float4 f = __ldg(q + N / 4);
+                    x[N] = f.x; x[N + 1] = f.y; x[N + 2] = f.z; x[N + 3] = f.w;
+                    if (shift == 1) add_at<N, 1>(z, x);
+                    else if (shift == 2) add_at<N, 2>(z, x);
+                    else add_at<N, 3>(z, x);
                 }
             }
             if (MASK) {   // N bits from token t on: at most two words
@@ -200,7 +195,6 @@ __global__ void __launch_bounds__(kThreads, 2) logits_adjust_kernel(const LogitA
                 E::store(orow, x, z);
             }
         }
-        if (BIAS) __syncwarp();   // the bias was read before its place is filled again
     }
 }
 
