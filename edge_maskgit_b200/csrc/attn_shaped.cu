@@ -105,16 +105,25 @@ Plan plan(const mgc_attention_args& args) {
     } else {
         const long long heads = (long long)a.B * a.Hkv * ((rows + 15) / 16);
         const long long want = std::max<long long>(1, (4LL * sms + heads - 1) / heads);
+        // With few heads a cluster of up to 16 CTAs per head reads its keys and joins them in one launch,
+        // as long as that leaves no CTA more than 512 keys; else ranges of up to 1024 keys, as many
+        // as there are, are joined by a second kernel.
+        const long long wide = std::min<long long>(16, std::min<long long>(want, (a.Sk + 63) / 64));
+        const long long each = wide > 0 ? ((a.Sk + wide - 1) / wide + 63) / 64 * 64 : 0;
         long long chunk = ((a.Sk + want - 1) / want + 63) / 64 * 64;
         chunk = std::max<long long>(128, std::min<long long>(1024, chunk));
         if (heads >= 4LL * sms && a.Sk <= 4096) chunk = (a.Sk + 63) / 64 * 64;
-        if (a.Sk > chunk) {
+        if (wide > 1 && each <= 512) {
+            p.c.chunk = (int)each;
+            p.c.nsplit = (int)((a.Sk + each - 1) / each);
+            p.c.cluster = p.c.nsplit > 1;
+        } else if (a.Sk > chunk) {
             p.c.chunk = (int)chunk;
             p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);
         }
     }
     p.bytes = p.doc_bytes;
-    if (p.c.nsplit > 1) {
+    if (p.c.nsplit > 1 && !p.c.cluster) {
         const uint64_t all = (uint64_t)a.B * a.Sq * a.Hq * p.c.nsplit;
         p.opart_bytes = (all * a.D * 4 + 15) / 16 * 16;
         p.bytes += p.opart_bytes + all * 8;
@@ -180,7 +189,7 @@ int mgc_attention(const mgc_attention_args* args, void* stream) {
         const cudaStream_t st = (cudaStream_t)stream;
         if (p.tile) run_tile(p, st);
         else launch_attn_step(p.c, st);
-        if (p.c.nsplit > 1) launch_attn_combine(p.c, st);
+        if (p.c.nsplit > 1 && !p.c.cluster) launch_attn_combine(p.c, st);
     });
 }
 

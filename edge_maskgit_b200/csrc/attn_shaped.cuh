@@ -17,6 +17,7 @@ struct AttnCall {
     mgc_attention_args a;
     int g;                 // query heads per key head
     int nsplit, chunk;     // splits of the key range; keys per split (a multiple of the key tile)
+    int cluster;           // few queries: the splits are one cluster, joined in distributed shared memory
     float* opart;
     float2* mlpart;
 };

@@ -6,7 +6,9 @@
 // tile is memory-bound by an order of magnitude, so the tcgen05 path with its 128-row tile would
 // add nothing).  The key range is split over CTAs, and inside a CTA over four warps.  Each warp has
 // its own ring of 16-key stages filled by cp.async, so the main loop has no CTA-wide barrier; the
-// online softmax keeps (max, sum, output) in registers, and warps and CTAs are joined at the end.
+// online softmax keeps (max, sum, output) in registers, and warps and CTAs are joined at the end: up to
+// 16 CTAs are one cluster and join in distributed shared memory, more leave partial results in the
+// workspace for a second kernel.
 #include <stdexcept>
 
 #include "attn_shaped.cuh"
@@ -19,7 +21,10 @@ template <int DP> constexpr int row_bytes() { return DP * 2 + 16; }   // odd in 
 template <int DP> constexpr int stage_bytes() { return 2 * KT * row_bytes<DP>(); }
 template <int DP> constexpr int ring_bytes() { return WARPS * STAGES * stage_bytes<DP>(); }
 template <int DP> constexpr int join_bytes() { return WARPS * 16 * (DP * 4 + 8); }
-template <int DP> constexpr int smem_bytes() { return ring_bytes<DP>() > join_bytes<DP>() ? ring_bytes<DP>() : join_bytes<DP>(); }
+template <int DP> constexpr int part_bytes() { return 16 * (DP * 4 + 8); }   // a CTA's own result, for its cluster
+template <int DP> constexpr int smem_bytes() {
+    return ring_bytes<DP>() > join_bytes<DP>() + part_bytes<DP>() ? ring_bytes<DP>() : join_bytes<DP>() + part_bytes<DP>();
+}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -206,6 +211,8 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
         for (int d = 0; d < DP / 8; d++)
             *reinterpret_cast<float2*>(so + (warp * 16 + qr + 8 * u) * DP + d * 8 + qc) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
     }
+    float* po = reinterpret_cast<float*>(smem + join_bytes<DP>());   // [16][DP]
+    float2* pml = reinterpret_cast<float2*>(po + 16 * DP);            // [16]
     __syncthreads();
     for (int r = warp; r < 16 && blk * 16 + r < rows; r += WARPS) {
         float mm = -INFINITY;
@@ -223,7 +230,12 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
                 if (lane + 32 * u < DP) acc[u] += so[(w * 16 + r) * DP + lane + 32 * u] * f;
         }
         const int gr = blk * 16 + r, i = gr / c.g, h = hk * c.g + gr % c.g;
-        if (c.nsplit == 1) {
+        if (c.cluster) {
+            if (lane == 0) pml[r] = make_float2(mm, ll);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (lane + 32 * u < DP) po[r * DP + lane + 32 * u] = acc[u];
+        } else if (c.nsplit == 1) {
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
             for (int u = 0; u < 4; u++) acc[u] = ll == 0.0f ? 0.0f : acc[u] * inv;
@@ -237,6 +249,39 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
                 if (lane + 32 * u < a.D) c.opart[id * a.D + lane + 32 * u] = acc[u];
         }
     }
+    if (!c.cluster) return;
+    __syncwarp();
+    cluster_sync_all();
+    for (int r = warp * c.nsplit + split; r < 16 && blk * 16 + r < rows; r += WARPS * c.nsplit) {   // this CTA's rows
+        float2 ml = make_float2(-INFINITY, 0.0f);   // lane = split
+        if (lane < c.nsplit) {
+            const uint32_t at = mapa_u32(pml + r, lane);
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(at) : "memory");
+        }
+        float mm = ml.x;
+        for (int k = 16; k; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
+        const float f = ex2_approx(ml.x - (mm == -INFINITY ? 0.0f : mm));
+        float ll = ml.y * f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 16; k; k >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, k);
+#pragma unroll 4
+        for (int p = 0; p < c.nsplit; p++) {
+            const uint32_t at = mapa_u32(po + r * DP + lane, p);
+            const float w = __shfl_sync(0xffffffffu, f, p);
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                float x = 0.0f;
+                if (lane + 32 * u < DP) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at + 128 * u) : "memory");
+                acc[u] = fmaf(x, w, acc[u]);
+            }
+        }
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+        for (int u = 0; u < 4; u++) acc[u] = ll == 0.0f ? 0.0f : acc[u] * inv;
+        const int gr = blk * 16 + r;
+        write_row<BF16>(c, b, hk * c.g + gr % c.g, gr / c.g, acc);
+    }
+    __syncwarp();
+    cluster_sync_all();   // partial results live until every CTA has read them
 }
 
 // Joins the splits of one row per warp, in split order; lane = four dims.
@@ -300,6 +345,12 @@ void launch_step(const AttnCall& c, cudaStream_t st) {
     allow_smem(kernel, smem_bytes<DP>(), done);
     const long long blocks = (long long)c.a.B * c.a.Hkv * ((c.a.Sq * c.g + 15) / 16) * c.nsplit;
     if (blocks > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
+    if (c.cluster) {
+        static std::atomic<uint64_t> wide{0};
+        if (c.nsplit > 8) allow_wide_clusters(kernel, wide);
+        launch_clusters(kernel, (unsigned)blocks, WARPS * 32, smem_bytes<DP>(), c.nsplit, st, c);
+        return;
+    }
     ++g_launch_count;
     const cudaError_t e = launch_k(kernel, dim3((unsigned)blocks), dim3(WARPS * 32), smem_bytes<DP>(), st, c);
     if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
@@ -329,11 +380,8 @@ void launch_attn_step(const AttnCall& c, cudaStream_t st) {
 void launch_attn_combine(const AttnCall& c, cudaStream_t st) {
     const long long all = (long long)c.a.B * c.a.Sq * c.a.Hq, blocks = (all + 3) / 4;
     if (blocks > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
-    ++g_launch_count;
-    const cudaError_t e = c.a.dtype == MGC_BF16
-                              ? launch_k(attn_combine_kernel<true>, dim3((unsigned)blocks), dim3(128), 0, st, c)
-                              : launch_k(attn_combine_kernel<false>, dim3((unsigned)blocks), dim3(128), 0, st, c);
-    if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+    // (launched while the partial results are still being made: the kernel waits for them itself)
+    launch_after(c.a.dtype == MGC_BF16 ? attn_combine_kernel<true> : attn_combine_kernel<false>, (unsigned)blocks, 128, st, c);
 }
 
 }  // namespace mgc

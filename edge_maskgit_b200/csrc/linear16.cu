@@ -431,27 +431,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lp::THREADS, 1)
 }
 
 // ------------------------------------------------------------------ host
-template <class K, class... Args>
-void launch_cluster(K kernel, unsigned grid, unsigned block, uint32_t smem, unsigned cluster, cudaStream_t st, Args... args) {
-    ++g_launch_count;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster ? 1 : 0;   // 0: the kernel fixes its own
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
-    }
-}
-
 CUtensorMap operand_map(const void* p, bool bf16, int rows, int K, long long ld, int box_rows) {
     const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows}, strides[1] = {(uint64_t)ld};
     const uint32_t box[2] = {BK, (uint32_t)box_rows};
@@ -466,7 +445,7 @@ void run_split(const void* w, long long ldw, const void* x, long long ldx, const
     const CUtensorMap mw = operand_map(w, BF16, a.N, a.K, ldw, TILE_N), mx = operand_map(x, BF16, a.M, a.K, ldx, BN);
     const long long tiles = (long long)((a.N + TILE_N - 1) / TILE_N) * ((a.M + BN - 1) / BN);
     if (tiles * split > 0x7fffffffLL) throw std::runtime_error("M * N is too large for one launch");
-    launch_cluster(kernel, (unsigned)(tiles * split), ls::THREADS, ls::smem<BN>(), split, st, mw, mx, a, split);
+    launch_clusters(kernel, (unsigned)(tiles * split), ls::THREADS, ls::smem<BN>(), split, st, mw, mx, a, split);
 }
 
 template <bool BF16>
@@ -482,7 +461,7 @@ void run_linear(const void* w, long long ldw, const void* x, long long ldx, cons
         static std::atomic<uint64_t> done[2];
         auto kernel = rows ? linear_pair_kernel<BF16, true> : linear_pair_kernel<BF16, false>;
         allow_smem(kernel, lp::SMEM, done[rows]);
-        launch_cluster(kernel, 2 * pairs, lp::THREADS, lp::SMEM, 0, st, mw, mx, a);
+        launch_clusters(kernel, 2 * pairs, lp::THREADS, lp::SMEM, 0, st, mw, mx, a);
         return;
     }
     const int bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;

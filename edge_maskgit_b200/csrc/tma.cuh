@@ -10,6 +10,7 @@
 #include <stdexcept>
 #include <string>
 
+#include "kernels.h"
 #include "ptx.cuh"
 
 namespace mgc {
@@ -33,6 +34,60 @@ void allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t>& done) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) throw std::runtime_error(std::string("cannot set the shared-memory limit: ") + cudaGetErrorString(e));
     done.fetch_or(1ull << dev);
+}
+
+// Lets a kernel run in clusters of more than 8 CTAs, once per device.
+template <class K>
+void allow_wide_clusters(K kernel, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev > 63) throw std::runtime_error("no usable current device");
+    if (done.load() >> dev & 1) return;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("cannot allow clusters of 16: ") + cudaGetErrorString(e));
+    done.fetch_or(1ull << dev);
+}
+
+inline void launch_checked(const cudaLaunchConfig_t& cfg, const void* kernel, void** args) {
+    ++g_launch_count;
+    const cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+    }
+}
+// Launch in clusters of `cluster` CTAs along x (0: the size that the kernel itself declares).
+template <class... P, class... Args>
+void launch_clusters(void (*kernel)(P...), unsigned grid, unsigned block, uint32_t smem, unsigned cluster, cudaStream_t st,
+                     Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster ? 1 : 0;
+    void* p[] = {(void*)&args...};
+    launch_checked(cfg, (const void*)kernel, p);
+}
+// Launch that may begin before the kernel ahead of it on the stream has ended; `kernel` calls
+// griddep_wait() before it reads anything.
+template <class... P, class... Args>
+void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    void* p[] = {(void*)&args...};
+    launch_checked(cfg, (const void*)kernel, p);
 }
 
 // Runs f, turning any exception into mgc_last_error() and -1.
