@@ -62,6 +62,8 @@ void check_pointers(const mgc_attention_args& a) {
                  ok(a.out_stride[i], sizes_q[i]),
              "strides must be multiples of 8, not negative");
         need(sizes_q[i] <= 1 || a.out_stride[i] >= a.D, "out's strides must be at least D");
+        need(i != 1 || a.Sk <= 1 || (a.k_stride[1] < (1LL << 31) && a.v_stride[1] < (1LL << 31)),
+             "k's and v's position strides must be below 2^31");
     }
 }
 

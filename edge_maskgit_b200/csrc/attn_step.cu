@@ -20,7 +20,8 @@ constexpr int WARPS = 4, KT = 16, STAGES = 3;
 template <int DP> constexpr int row_bytes() { return DP * 2 + 16; }   // odd in 16-byte units: ldmatrix without conflicts
 template <int DP> constexpr int stage_bytes() { return 2 * KT * row_bytes<DP>(); }
 template <int DP> constexpr int ring_bytes() { return WARPS * STAGES * stage_bytes<DP>(); }
-template <int DP> constexpr int join_bytes() { return WARPS * 16 * (DP * 4 + 8); }
+template <int DP> constexpr int join_row() { return DP + 8; }   // floats: eight rows' writes meet no bank twice
+template <int DP> constexpr int join_bytes() { return WARPS * 16 * (join_row<DP>() * 4 + 8); }
 template <int DP> constexpr int part_bytes() { return 16 * (DP * 4 + 8); }   // a CTA's own result, for its cluster
 template <int DP> constexpr int smem_bytes() {
     return ring_bytes<DP>() > join_bytes<DP>() + part_bytes<DP>() ? ring_bytes<DP>() : join_bytes<DP>() + part_bytes<DP>();
@@ -45,6 +46,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // 16 bytes global -> shared, or zeros
 __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool copy) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(copy ? 16 : 0) : "memory");
@@ -64,6 +68,21 @@ __device__ __forceinline__ void write_row(const AttnCall& c, int b, int h, int i
         if (lane + 32 * u < c.a.D) store16<BF16>(c.a.out, at + lane + 32 * u, o[u]);
 }
 
+// The same from sums of unnormalised values: o = dims 4 lane .. 4 lane + 3, l their sum of probabilities.
+template <bool BF16>
+__device__ __forceinline__ void write_row4(const AttnCall& c, int b, int h, int i, float4 o, float l) {
+    const int lane = threadIdx.x & 31;
+    const bool dims = lane * 4 < c.a.D;
+    if (__any_sync(0xffffffffu, dims && (isnan(o.x) || isnan(o.y) || isnan(o.z) || isnan(o.w) || isnan(l)))) {
+        float nan[4] = {NAN, NAN, NAN, NAN};
+        write_row<BF16>(c, b, h, i, nan);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(c.a.out) + b * c.a.out_stride[0] + i * c.a.out_stride[1] + h * c.a.out_stride[2];
+    if (dims) reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<BF16>(o.x * inv, o.y * inv), pack16<BF16>(o.z * inv, o.w * inv));
+}
+
 // grid: splits x (batch row, key head, 16-row block), splits fastest
 template <bool BF16, int DP>
 __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_constant__ AttnCall c) {
@@ -73,25 +92,24 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
     griddep_launch();
     const mgc_attention_args& a = c.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qr = lane >> 2, qc = (lane & 3) * 2;
-    const int split = blockIdx.x % c.nsplit;
-    long long rest = blockIdx.x / c.nsplit;
-    const int rows = a.Sq * c.g, blocks = (rows + 15) / 16;
+    const unsigned blocks = (unsigned)(a.Sq * c.g + 15) / 16;
+    unsigned rest = blockIdx.x / (unsigned)c.nsplit;
+    const int rows = a.Sq * c.g, split = (int)(blockIdx.x - rest * c.nsplit);
     const int blk = (int)(rest % blocks); rest /= blocks;
-    const int hk = (int)(rest % a.Hkv), b = (int)(rest / a.Hkv);
+    const int hk = (int)(rest % (unsigned)a.Hkv), b = (int)(rest / (unsigned)a.Hkv);
     const RowBounds rb = row_bounds(a, b);
 
     // rows of this lane's fragments: blk * 16 + qr and + 8; row = query i * g + (h - hk * g)
-    int row[2], qi[2], head[2], doc[2], end[2];
-    ScoreShape sh[2];
+    int row[2], qi[2], head[2], doc[2], end[2], pos[2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         row[u] = blk * 16 + qr + 8 * u;
         const int rr = min(row[u], rows - 1);
         qi[u] = rr / c.g;
-        head[u] = hk * c.g + rr % c.g;
-        sh[u] = score_shape(a, head[u]);
+        head[u] = hk * c.g + (rr - qi[u] * c.g);
+        pos[u] = rb.pos0 + qi[u];
         doc[u] = a.doc_q ? __ldg(a.doc_q + (long long)b * a.Sq + qi[u]) : 0;
-        end[u] = row[u] < rows && doc[u] >= 0 ? key_end(rb, rb.pos0 + qi[u]) : 0;
+        end[u] = row[u] < rows && doc[u] >= 0 ? key_end(rb, pos[u]) : 0;
     }
     uint32_t qf[NK][4];
 #pragma unroll
@@ -112,22 +130,34 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
     const uint32_t ring = smem_u32(smem) + warp * STAGES * SB;
     const int mine = tiles > warp ? (tiles - warp + WARPS - 1) / WARPS : 0;   // tiles warp, warp + 4, ...
 
+    const int ks = (int)a.k_stride[1], vs = (int)a.v_stride[1];   // (below 2^31: checked)
     auto load = [&](int n) {   // stage n % STAGES <- the warp's n-th tile; keys past the end read as zeros
         if (n < mine) {
             const int j0 = k_lo + (warp + n * WARPS) * KT;
             const uint32_t s = ring + (n % STAGES) * SB;
+            const uint16_t* kt = kp + (long long)j0 * ks;
+            const uint16_t* vt = vp + (long long)j0 * vs;
+            if (a.D == DP && j0 + KT <= k_hi) {
 #pragma unroll
-            for (int x = lane; x < KT * CH; x += 32) {
-                const int r = x / CH, ch = x % CH, j = j0 + r;
-                const bool in = j < k_hi && ch * 8 < a.D;
-                const long long jj = in ? j : 0;
-                const int d = in ? ch * 8 : 0;
-                cp16_or_zero(s + r * RB + ch * 16, kp + jj * a.k_stride[1] + d, in);
-                cp16_or_zero(s + KT * RB + r * RB + ch * 16, vp + jj * a.v_stride[1] + d, in);
+                for (int i = 0; i < KT * CH / 32; i++) {
+                    const int x = lane + 32 * i, r = x / CH, ch = x % CH;
+                    cp16(s + r * RB + ch * 16, kt + (long long)r * ks + ch * 8);
+                    cp16(s + KT * RB + r * RB + ch * 16, vt + (long long)r * vs + ch * 8);
+                }
+            } else {
+#pragma unroll 1
+                for (int x = lane; x < KT * CH; x += 32) {
+                    const int r = x / CH, ch = x % CH;
+                    const bool in = j0 + r < k_hi && ch * 8 < a.D;
+                    cp16_or_zero(s + r * RB + ch * 16, in ? kt + (long long)r * ks + ch * 8 : kp, in);
+                    cp16_or_zero(s + KT * RB + r * RB + ch * 16, in ? vt + (long long)r * vs + ch * 8 : vp, in);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // score constants of the two rows (ScoreShape, branches on the call's own values only)
+    const ScoreShape s0 = score_shape(a, head[0]), s1 = score_shape(a, head[1]);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[DP / 8][4];
 #pragma unroll
     for (int d = 0; d < DP / 8; d++)
@@ -148,17 +178,29 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
             mma16816<BF16>(sc[0], qf[k], kf[0], kf[2]);
             mma16816<BF16>(sc[1], qf[k], kf[1], kf[3]);
         }
+        // ---- shape; one branch for all eight scores at a time
+        auto each = [&](auto f) {   // f(score, row 0 / 1, key)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) f(sc[t][e], e >> 1, j0 + t * 8 + qc + (e & 1));
+        };
+        if (a.cap > 0.0f) each([&](float& x, int, int) { x = capped(x, s0.c1, s0.cap2); });
+        else each([&](float& x, int, int) { x *= s0.c1; });
+        if (a.slopes) each([&](float& x, int u, int j) { x = fmaf(u ? -s1.slope2 : -s0.slope2, fabsf((float)(j - pos[u])), x); });
+        if (a.dist_bias)
+            each([&](float& x, int u, int j) {
+                x += bias2(__ldg((u ? s1.table : s0.table) + max(-s0.range, min(s0.range, j - pos[u]))));
+            });
+        if (a.doc_k)
+            each([&](float& x, int u, int j) {
+                if (__ldg(a.doc_k + (long long)b * a.Sk + min(j, a.Sk - 1)) != doc[u]) x = -INFINITY;
+            });
         float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int u = e >> 1, j = j0 + t * 8 + qc + (e & 1);
-                bool seen = j < end[u];
-                if (a.doc_k) seen = seen && __ldg(a.doc_k + (long long)b * a.Sk + min(j, a.Sk - 1)) == doc[u];
-                sc[t][e] = seen ? shaped(sc[t][e], sh[u], j - (rb.pos0 + qi[u])) : -INFINITY;
-                mx[u] = fmaxf(mx[u], sc[t][e]);
-            }
+        each([&](float& x, int u, int j) {
+            x = j < end[u] ? x : -INFINITY;
+            mx[u] = fmaxf(mx[u], x);
+        });
         float alpha[2], base[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -200,16 +242,18 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();   // the ring is free: join the warps through it
-    float* so = reinterpret_cast<float*>(smem);                    // [WARPS][16][DP]
-    float2* sml = reinterpret_cast<float2*>(so + WARPS * 16 * DP);  // [WARPS][16]
+    constexpr int JR = join_row<DP>();
+    float* so = reinterpret_cast<float*>(smem);                    // [WARPS][16][JR]
+    float2* sml = reinterpret_cast<float2*>(so + WARPS * 16 * JR);  // [WARPS][16]
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
         l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
         if ((lane & 3) == 0) sml[warp * 16 + qr + 8 * u] = make_float2(m[u], l[u]);
+        if (row[u] >= rows) continue;
 #pragma unroll
         for (int d = 0; d < DP / 8; d++)
-            *reinterpret_cast<float2*>(so + (warp * 16 + qr + 8 * u) * DP + d * 8 + qc) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
+            *reinterpret_cast<float2*>(so + (warp * 16 + qr + 8 * u) * JR + d * 8 + qc) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
     }
     float* po = reinterpret_cast<float*>(smem + join_bytes<DP>());   // [16][DP]
     float2* pml = reinterpret_cast<float2*>(po + 16 * DP);            // [16]
@@ -227,7 +271,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
             ll += ml.y * f;
 #pragma unroll
             for (int u = 0; u < 4; u++)
-                if (lane + 32 * u < DP) acc[u] += so[(w * 16 + r) * DP + lane + 32 * u] * f;
+                if (lane + 32 * u < DP) acc[u] += so[(w * 16 + r) * JR + lane + 32 * u] * f;
         }
         const int gr = blk * 16 + r, i = gr / c.g, h = hk * c.g + gr % c.g;
         if (c.cluster) {
@@ -261,24 +305,23 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
         float mm = ml.x;
         for (int k = 16; k; k >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, k));
         const float f = ex2_approx(ml.x - (mm == -INFINITY ? 0.0f : mm));
-        float ll = ml.y * f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float ll = ml.y * f;
         for (int k = 16; k; k >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, k);
-#pragma unroll 4
-        for (int p = 0; p < c.nsplit; p++) {
-            const uint32_t at = mapa_u32(po + r * DP + lane, p);
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // dims 4 lane ..
+        const bool dims = lane * 4 < DP;
+#pragma unroll
+        for (int p = 0; p < 16; p++) {   // all remote reads in flight
+            if (p >= c.nsplit) break;
             const float w = __shfl_sync(0xffffffffu, f, p);
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                float x = 0.0f;
-                if (lane + 32 * u < DP) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at + 128 * u) : "memory");
-                acc[u] = fmaf(x, w, acc[u]);
-            }
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (dims)
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(mapa_u32(po + r * DP + lane * 4, p)) : "memory");
+            acc.x = fmaf(x.x, w, acc.x); acc.y = fmaf(x.y, w, acc.y);
+            acc.z = fmaf(x.z, w, acc.z); acc.w = fmaf(x.w, w, acc.w);
         }
-        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-#pragma unroll
-        for (int u = 0; u < 4; u++) acc[u] = ll == 0.0f ? 0.0f : acc[u] * inv;
         const int gr = blk * 16 + r;
-        write_row<BF16>(c, b, hk * c.g + gr % c.g, gr / c.g, acc);
+        write_row4<BF16>(c, b, hk * c.g + gr % c.g, gr / c.g, acc, ll);
     }
     __syncwarp();
     cluster_sync_all();   // partial results live until every CTA has read them
@@ -322,20 +365,8 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const __grid_constant
             }
         }
     }
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-    const int h = (int)(id % a.Hq);
     const long long bi = id / a.Hq;
-    const int b = (int)(bi / a.Sq), i = (int)(bi % a.Sq);
-    const bool bad = dims && (isnan(acc.x) || isnan(acc.y) || isnan(acc.z) || isnan(acc.w) || isnan(ll));
-    if (__any_sync(0xffffffffu, bad)) {
-        float o[4] = {NAN, NAN, NAN, NAN};   // write_row repairs
-        write_row<BF16>(c, b, h, i, o);
-        return;
-    }
-    if (dims) {
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b * a.out_stride[0] + i * a.out_stride[1] + h * a.out_stride[2];
-        reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
-    }
+    write_row4<BF16>(c, (int)(bi / a.Sq), (int)(id % a.Hq), (int)(bi % a.Sq), acc, ll);
 }
 
 template <bool BF16, int DP>

@@ -282,11 +282,17 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
     doc_k[b][j] >= 0 if given.  A query that sees no key gives zeros.  scale defaults to D ** -0.5;
     slopes f32 [Hq]; prefix, k_len, q_pos int32 [B]; doc_q, doc_k int32 [B][Sq], [B][Sk]."""
     import torch
-    code = _code_of(q, "q")
+    code = _CODE.get(getattr(q, "dtype", None)) or _code_of(q, "q")
     dt, index = q.dtype, q.get_device()
-    qs, ks, vs = _heads(q, "q", dt, index), _heads(k, "k", dt, index), _heads(v, "v", dt, index)
+    if index < 0 or not (k.dtype is dt and v.dtype is dt and k.get_device() == index and v.get_device() == index) or \
+            q.requires_grad or k.requires_grad or v.requires_grad or not (q.dim() == k.dim() == v.dim() == 4):
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            _heads(t, name, dt, index)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
     B, Sq, Hq, D = q.shape
     Bk, Sk, Hkv, Dk = k.shape
+    if (qs[3] != 1 or ks[3] != 1 or vs[3] != 1) and D > 1:
+        raise MgcError("the last axes of q, k and v must be contiguous")
     if k.shape != v.shape or Bk != B or Dk != D:
         raise MgcError(f"k and v must be [{B}][Sk][Hkv][{D}], not {list(k.shape)} and {list(v.shape)}")
     i32, reach = torch.int32, 0

@@ -143,7 +143,8 @@ typedef struct mgc_attention_args {
     const void* v;              /* dev [B][Sk][Hkv][D] */
     void* out;                  /* dev [B][Sq][Hq][D], no overlap with q, k, v */
     int64_t q_stride[3];        /* elements from one batch row, position and head to the next: >= 0, */
-    int64_t k_stride[3];        /* multiples of 8 (the D axis is contiguous); 0 repeats (not in out) */
+    int64_t k_stride[3];        /* multiples of 8 (the D axis is contiguous), positions' below 2^31; 0
+                                   repeats (not in out) */
     int64_t v_stride[3];
     int64_t out_stride[3];
     float scale;
