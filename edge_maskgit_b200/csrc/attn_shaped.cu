@@ -106,22 +106,18 @@ Plan plan(const mgc_attention_args& args) {
         if (a.doc_k) p.doc_bytes = ((uint64_t)a.B * nkt * sizeof(int2) + 15) / 16 * 16;
     } else {
         const long long heads = (long long)a.B * a.Hkv * ((rows + 15) / 16);
-        const long long want = std::max<long long>(1, (4LL * sms + heads - 1) / heads);
-        // With few heads a cluster of up to 16 CTAs per head reads its keys and joins them in one launch,
-        // as long as that leaves no CTA more than 512 keys; else ranges of up to 1024 keys, as many
-        // as there are, are joined by a second kernel.
-        const long long wide = std::min<long long>(16, std::min<long long>(want, (a.Sk + 63) / 64));
-        const long long each = wide > 0 ? ((a.Sk + wide - 1) / wide + 63) / 64 * 64 : 0;
-        long long chunk = ((a.Sk + want - 1) / want + 63) / 64 * 64;
-        chunk = std::max<long long>(128, std::min<long long>(1024, chunk));
-        if (heads >= 4LL * sms && a.Sk <= 4096) chunk = (a.Sk + 63) / 64 * 64;
-        if (wide > 1 && each <= 512) {
-            p.c.chunk = (int)each;
-            p.c.nsplit = (int)((a.Sk + each - 1) / each);
-            p.c.cluster = p.c.nsplit > 1;
-        } else if (a.Sk > chunk) {
+        // As many ranges of keys as run at once (two blocks an SM with large heads, three with small ones),
+        // of 128 keys at least; where that leaves more than 2048 keys each, ranges of 1024, so that
+        // rows of unequal length balance.  Up to 8 ranges are one cluster and join in one launch
+        // (4 rows x 4096 keys x 8 heads of 128: 17.5 us, by a second kernel 20; clusters of 16 took 35).
+        const long long slots = (long long)sms * (a.D > 64 ? 2 : 3);
+        const long long n = std::max<long long>(1, slots / heads);
+        long long chunk = std::max<long long>(128, ((a.Sk + n - 1) / n + 63) / 64 * 64);
+        if (chunk > 2048) chunk = 1024;
+        if (a.Sk > chunk) {
             p.c.chunk = (int)chunk;
             p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);
+            p.c.cluster = p.c.nsplit <= 8;
         }
     }
     p.bytes = p.doc_bytes;

@@ -7,7 +7,7 @@
 // add nothing).  The key range is split over CTAs, and inside a CTA over four warps.  Each warp has
 // its own ring of 16-key stages filled by cp.async, so the main loop has no CTA-wide barrier; the
 // online softmax keeps (max, sum, output) in registers, and warps and CTAs are joined at the end: up to
-// 16 CTAs are one cluster and join in distributed shared memory, more leave partial results in the
+// 8 CTAs are one cluster and join in distributed shared memory, more leave partial results in the
 // workspace for a second kernel.
 #include <stdexcept>
 
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // dims 4 lane ..
         const bool dims = lane * 4 < DP;
 #pragma unroll
-        for (int p = 0; p < 16; p++) {   // all remote reads in flight
+        for (int p = 0; p < 8; p++) {   // all remote reads in flight
             if (p >= c.nsplit) break;
             const float w = __shfl_sync(0xffffffffu, f, p);
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -377,8 +377,6 @@ void launch_step(const AttnCall& c, cudaStream_t st) {
     const long long blocks = (long long)c.a.B * c.a.Hkv * ((c.a.Sq * c.g + 15) / 16) * c.nsplit;
     if (blocks > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
     if (c.cluster) {
-        static std::atomic<uint64_t> wide{0};
-        if (c.nsplit > 8) allow_wide_clusters(kernel, wide);
         launch_clusters(kernel, (unsigned)blocks, WARPS * 32, smem_bytes<DP>(), c.nsplit, st, c);
         return;
     }

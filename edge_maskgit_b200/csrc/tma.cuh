@@ -36,17 +36,6 @@ void allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t>& done) {
     done.fetch_or(1ull << dev);
 }
 
-// Lets a kernel run in clusters of more than 8 CTAs, once per device.
-template <class K>
-void allow_wide_clusters(K kernel, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev > 63) throw std::runtime_error("no usable current device");
-    if (done.load() >> dev & 1) return;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) throw std::runtime_error(std::string("cannot allow clusters of 16: ") + cudaGetErrorString(e));
-    done.fetch_or(1ull << dev);
-}
-
 inline void launch_checked(const cudaLaunchConfig_t& cfg, const void* kernel, void** args) {
     ++g_launch_count;
     const cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
