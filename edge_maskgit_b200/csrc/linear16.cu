@@ -68,8 +68,9 @@ __device__ __forceinline__ void act16_all(float (&v)[N], int a) {
 // 32 accumulators of one output n, for x rows m .. m + 31: a warp moves 32 consecutive n of a row
 // at a time, 2 bytes a lane.
 template <bool BF16>
-__device__ __forceinline__ void finish_cols(const uint32_t (&acc)[32], const LinArgs& a, int m, int n, float bias) {
-    const int rows = min(32, a.M - m);
+__device__ __forceinline__ void finish_cols(const uint32_t (&acc)[32], const LinArgs& a, int m, int n, float bias,
+                                            int cols = 32) {
+    const int rows = min(cols, a.M - m);   // (a 16-column tile has 16)
     uint16_t* y = reinterpret_cast<uint16_t*>(a.y) + m * a.ldy + n;
     const uint16_t* r = a.resid ? reinterpret_cast<const uint16_t*>(a.resid) + m * a.ldr + n : nullptr;
     float v[32], res[32];
@@ -94,8 +95,8 @@ __device__ __forceinline__ void finish_cols(const uint32_t (&acc)[32], const Lin
     }
 }
 
-// 32 accumulators of one x row m, for outputs n .. n + 31 (N a multiple of 8, y and resid rows
-// 16-byte aligned): 16 bytes a move.
+// 32 accumulators of one x row m, for outputs n .. n + 31 (N a multiple of 8; bias, and the rows of y
+// and resid, 16-byte aligned): 16 bytes a move.
 template <bool BF16>
 __device__ __forceinline__ void finish_row(const uint32_t (&acc)[32], const LinArgs& a, int m, int n) {
     const int groups = min(4, (a.N - n) / 8);
@@ -110,10 +111,10 @@ __device__ __forceinline__ void finish_row(const uint32_t (&acc)[32], const LinA
 #pragma unroll
         for (int g = 0; g < 4; g++) {
             float4 b0 = make_float4(0, 0, 0, 0), b1 = b0;
-            if (g < groups) {   // (bias is only 4-byte aligned)
-                const float* b = a.bias + n + 8 * g;
-                b0 = make_float4(__ldg(b), __ldg(b + 1), __ldg(b + 2), __ldg(b + 3));
-                b1 = make_float4(__ldg(b + 4), __ldg(b + 5), __ldg(b + 6), __ldg(b + 7));
+            if (g < groups) {
+                const float4* b = reinterpret_cast<const float4*>(a.bias + n + 8 * g);
+                b0 = __ldg(b);
+                b1 = __ldg(b + 1);
             }
             const float b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
 #pragma unroll
@@ -176,13 +177,19 @@ __global__ void __launch_bounds__(ls::THREADS) linear_split_kernel(const __grid_
     const int ks = (a.K + BK - 1) / BK;
     const int k0 = (int)((long long)ks * rank / split), nk = (int)((long long)ks * (rank + 1) / split) - k0;
 
+    auto load = [&](int i) {
+        const int s = i % ST;
+        mbar_arrive_expect_tx(full + s, SB);
+        tma_load_2d(sm + s * SB, &mw, (k0 + i) * BK, n0, full + s);
+        tma_load_2d(sm + s * SB + A_BYTES, &mx, (k0 + i) * BK, m0, full + s);
+    };
     if (tid == 0) {
         for (int i = 0; i < ST; i++) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         mbar_init(done, 1);
         *abort_flag = 0;
         mbar_fence_init();
-        tma_prefetch_map(&mw);
-        tma_prefetch_map(&mx);
+        griddep_wait();
+        for (int i = 0; i < min(ST, nk); i++) load(i);   // under the rest of the set-up
     }
     if (warp == 1) tmem_alloc(tmem_slot, COLS);
     griddep_wait();
@@ -193,13 +200,10 @@ __global__ void __launch_bounds__(ls::THREADS) linear_split_kernel(const __grid_
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0 && lane == 0) {
-        int i = 0;
+        int i = min(ST, nk);
         for (; i < nk; i++) {
-            const int s = i % ST;
-            if (i >= ST && !mbar_wait(empty + s, (i / ST - 1) & 1, abort_flag, 41)) break;
-            mbar_arrive_expect_tx(full + s, SB);
-            tma_load_2d(sm + s * SB, &mw, (k0 + i) * BK, n0, full + s);
-            tma_load_2d(sm + s * SB + A_BYTES, &mx, (k0 + i) * BK, m0, full + s);
+            if (!mbar_wait(empty + i % ST, (i / ST - 1) & 1, abort_flag, 41)) break;
+            load(i);
         }
         if (i < nk) {   // gave up: let the copies in flight land
             volatile int never = 0;
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(ls::THREADS) linear_split_kernel(const __grid_
                 else tmem_ld16(t_row + c, acc);
                 tmem_ld_wait();
                 if (BN < 32) for (int j = 16; j < 32; j++) acc[j] = 0;
-                if (n < a.N) finish_cols<BF16>(acc, a, m0 + c, n, bias);
+                if (n < a.N) finish_cols<BF16>(acc, a, m0 + c, n, bias, min(32, BN));
             }
         }
     } else {
@@ -452,8 +456,32 @@ template <bool BF16>
 void run_linear(const void* w, long long ldw, const void* x, long long ldx, const LinArgs& a, cudaStream_t st) {
     const int sms = current_sms();
     const long long big = (long long)((a.N + lp::TN - 1) / lp::TN) * ((a.M + lp::TM - 1) / lp::TM);
-    if (a.M > 128 && big >= sms / 4) {
-        const bool rows = a.N % 8 == 0 && a.ldy % 8 == 0 && (uintptr_t)a.y % 16 == 0 &&
+    const int ks = (a.K + BK - 1) / BK;
+    // The kernel, tile and split of the least estimated time, in us, from measurements on a B200: a tile
+    // of bn columns takes 16 KB + 128 bn bytes a k step, which an SM gets from L2 at about 55 bytes a
+    // clock; set-up and launch 3.5 us; a split adds its join.  Measured against the estimate: 257 x
+    // 768 x 2304 in 64 columns 7.3 (7.1), in 128 8.0 (8.3), in 128 split in two 12.5 (10.6), in
+    // pairs 13.4 (12.5); 100 x 2048 x 2048 in 64 split in four 9.8 (9.5); 4097 x 768 x 768 in 128 16.0
+    // (13.2), in pairs 14.1 (12.5); 1 x 4096 x 4096 in 16 split in four 10.9 (8.5), in two 14.2 (9.7).
+    const long long pair_waves = (big + sms / 2 - 1) / (sms / 2);
+    double best = 9.0 + ks * 0.29 + (double)(pair_waves - 1) * std::max(ks * 0.29, 5.0);
+    int bn = 256, split = 1;
+    for (int n = 16; n <= 128; n *= 2) {
+        if (n > 16 && n / 2 >= a.M) break;   // no wider than the rows need
+        const long long tiles = (long long)((a.N + TILE_N - 1) / TILE_N) * ((a.M + n - 1) / n);
+        const int per_sm = n <= 32 ? 2 : 1;   // blocks whose shared memory fits an SM
+        for (int sp = 1; sp <= 8 && ks / sp >= 2; sp *= 2) {
+            const long long ctas = tiles * sp;
+            if (sp > 1 && (ctas > sms * per_sm || sp > 4 * per_sm)) break;   // (8 CTAs with an SM each rarely fit a GPC)
+            const long long side = std::min<long long>(per_sm, (ctas + sms - 1) / sms);   // that share an SM
+            const long long waves = (ctas + sms * per_sm - 1) / (sms * per_sm);
+            const double step = (16384 + 128 * n) / 55.0 / 1850.0 * side;
+            const double us = 3.5 + waves * ((double)((ks + sp - 1) / sp) * step + 0.2 + 0.006 * n) + (sp > 1 ? 0.8 + 0.03 * n : 0.0);
+            if (us < best) { best = us; bn = n; split = sp; }
+        }
+    }
+    if (bn == 256) {
+        const bool rows = a.N % 8 == 0 && a.ldy % 8 == 0 && ((uintptr_t)a.y | (uintptr_t)a.bias) % 16 == 0 &&
                           (!a.resid || (a.ldr % 8 == 0 && (uintptr_t)a.resid % 16 == 0));
         if (big > 0x7fffffffLL) throw std::runtime_error("M * N is too large for one launch");
         const CUtensorMap mw = operand_map(w, BF16, a.N, a.K, ldw, 128), mx = operand_map(x, BF16, a.M, a.K, ldx, 128);
@@ -464,11 +492,6 @@ void run_linear(const void* w, long long ldw, const void* x, long long ldx, cons
         launch_clusters(kernel, 2 * pairs, lp::THREADS, lp::SMEM, 0, st, mw, mx, a);
         return;
     }
-    const int bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-    const long long tiles = (long long)((a.N + TILE_N - 1) / TILE_N) * ((a.M + bn - 1) / bn);
-    const int ks = (a.K + BK - 1) / BK;
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= sms && ks / (split * 2) >= 2) split *= 2;
     if (bn == 16) run_split<BF16, 16>(w, ldw, x, ldx, a, split, st);
     else if (bn == 32) run_split<BF16, 32>(w, ldw, x, ldx, a, split, st);
     else if (bn == 64) run_split<BF16, 64>(w, ldw, x, ldx, a, split, st);
