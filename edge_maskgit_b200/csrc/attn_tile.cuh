@@ -140,8 +140,10 @@ __device__ __forceinline__ void shape32(uint32_t* s, const RowTile& x, int first
 // Unseen keys' scores become -inf.
 __device__ __forceinline__ void mask32(uint32_t* s, const RowTile& x, int first) {
     const int lim = x.lim - first;
+    if (x.lim < KT) {
 #pragma unroll
-    for (int j = 0; j < 32; j++) s[j] = j < lim ? s[j] : 0xFF800000u;
+        for (int j = 0; j < 32; j++) s[j] = j < lim ? s[j] : 0xFF800000u;
+    }
     if (x.docs) {
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
@@ -201,44 +203,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     const AttnCall& c = tc.c;
     const mgc_attention_args& a = c.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x % c.nsplit;
-    long long rest = blockIdx.x / c.nsplit;
+    unsigned rest = blockIdx.x / (unsigned)c.nsplit;
+    const int split = (int)(blockIdx.x - rest * c.nsplit);
     int qb, h, b;
     if (tc.q_outer) {
-        h = (int)(rest % a.Hq); rest /= a.Hq;
-        b = (int)(rest % a.B);
-        qb = tc.qblocks - 1 - (int)(rest / a.B);
+        h = (int)(rest % (unsigned)a.Hq); rest /= (unsigned)a.Hq;
+        b = (int)(rest % (unsigned)a.B);
+        qb = tc.qblocks - 1 - (int)(rest / (unsigned)a.B);
     } else {
-        qb = (int)(rest % tc.qblocks); rest /= tc.qblocks;
-        h = (int)(rest % a.Hq);
-        b = (int)(rest / a.Hq);
+        qb = (int)(rest % (unsigned)tc.qblocks); rest /= (unsigned)tc.qblocks;
+        h = (int)(rest % (unsigned)a.Hq);
+        b = (int)(rest / (unsigned)a.Hq);
     }
     const int hk = h / c.g, q0 = qb * tc.tiles_per_cta * QT;
-    const RowBounds rb = row_bounds(a, b);
-    const int nkt = (a.Sk + KT - 1) / KT;
-
-    if (tid == 0) {
-        for (int i = 0; i < 2; i++) {
-            mbar_init(q_full + i, 1); mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(o_full + i, 1);
-            mbar_init(s_free + i, 4); mbar_init(p_half + i, 4);
-        }
-        for (int i = 0; i < NST; i++) {
-            mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
-        }
-        *abort_flag = 0;
-        mbar_fence_init();
-        tma_prefetch_map(&mq); tma_prefetch_map(&mk); tma_prefetch_map(&mv);
-    }
-    if (tid < 2) {
-        range[tid] = INT_MAX; range[2 + tid] = 0; range[4 + tid] = INT_MAX; range[6 + tid] = -1;
-    }
-    if (warp == 9) tmem_alloc(tmem_slot, 512);
     griddep_wait();
     griddep_launch();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const RowBounds rb = row_bounds(a, b);
+    const int nkt = (a.Sk + KT - 1) / KT;
 
     // ---- the key tiles [lo, hi) of each query tile
     const int kt_first = split * (c.chunk / KT), kt_last = min(nkt, kt_first + c.chunk / KT);
@@ -250,6 +231,63 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         hi[w] = w < tc.tiles_per_cta && last >= first
                     ? max(lo[w], min(kt_last, (key_end(rb, rb.pos0 + last) + KT - 1) / KT)) : lo[w];
     }
+    // Step i works on key tile order(i): from the diagonal (the last query's position) down to the first,
+    // then up from there.  A bias that falls with the distance has its largest values first, so bases
+    // are not moved from tile to tile, and causally the tile with the mask comes first.
+    bool on[2];
+    int lo_all, n, centre;
+    auto steps = [&] {
+        on[0] = hi[0] > lo[0];
+        on[1] = hi[1] > lo[1];
+        lo_all = min(on[0] ? lo[0] : INT_MAX, on[1] ? lo[1] : INT_MAX);
+        const int hi_all = max(on[0] ? hi[0] : 0, on[1] ? hi[1] : 0);
+        n = hi_all > lo_all ? hi_all - lo_all : 0;
+        centre = max(lo_all, min(hi_all - 1, (rb.pos0 + min(q0 + tc.tiles_per_cta * QT, a.Sq) - 1) >> 7));
+    };
+    auto order = [&](int i) { return i <= centre - lo_all ? centre - i : lo_all + i; };
+    auto active = [&](int w, int i) {
+        const int kt = order(i);
+        return on[w] && i >= 0 && i < n && kt >= lo[w] && kt < hi[w];
+    };
+    // ---- copies (by one thread)
+    auto copy = [&](uint8_t* dst, const CUtensorMap* map, int pos, int head, int batch, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, TB);
+#pragma unroll
+        for (int s = 0; s < NSLAB; s++) tma_load_4d(dst + s * SLAB, map, s * 64, pos, head, batch, bar);
+    };
+    auto copy_k = [&](int i) { copy(sK + i % NST * TB, &mk, order(i) * KT, hk * tc.kmul[2], b * tc.kmul[0], k_full + i % NST); };
+    auto copy_v = [&](int i) { copy(sV + i % NST * TB, &mv, order(i) * KT, hk * tc.vmul[2], b * tc.vmul[0], v_full + i % NST); };
+    auto first_copies = [&] {   // both query tiles and a ring of key tiles
+        for (int i = 0; i < min(n, NST); i++) {
+            if (i == 0 && on[0]) copy(sQ, &mq, q0, h * tc.qmul[2], b * tc.qmul[0], q_full);
+            copy_k(i);
+            if (i == 0 && on[1]) copy(sQ + TB, &mq, q0 + QT, h * tc.qmul[2], b * tc.qmul[0], q_full + 1);
+            copy_v(i);
+        }
+    };
+    steps();
+
+    if (tid == 256) {   // (warp 8, which issues the copies)
+        for (int i = 0; i < 2; i++) {
+            mbar_init(q_full + i, 1); mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(o_full + i, 1);
+            mbar_init(s_free + i, 4); mbar_init(p_half + i, 4);
+        }
+        for (int i = 0; i < NST; i++) {
+            mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+        if (!a.doc_q) first_copies();   // under the rest of the set-up
+    }
+    if (tid < 2) {
+        range[tid] = INT_MAX; range[2 + tid] = 0; range[4 + tid] = INT_MAX; range[6 + tid] = -1;
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
     if (a.doc_q) {   // only tiles that share a document number with the queries (sorted or not)
         if (warp < 8) {
             const int w = warp >> 2, i = q0 + w * QT + (tid & 127);
@@ -274,20 +312,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             lo[w] = max(lo[w], range[w]);
             hi[w] = min(hi[w], range[2 + w]);
         }
+        steps();
+        if (tid == 256) first_copies();
     }
-    const bool on[2] = {hi[0] > lo[0], hi[1] > lo[1]};
-    const int lo_all = min(on[0] ? lo[0] : INT_MAX, on[1] ? lo[1] : INT_MAX);
-    const int hi_all = max(on[0] ? hi[0] : 0, on[1] ? hi[1] : 0);
-    const int n = hi_all > lo_all ? hi_all - lo_all : 0;
-    // Step i works on key tile order(i): from the diagonal (the last query's position) down to the first,
-    // then up from there.  A bias that falls with the distance has its largest values first, so bases
-    // are not moved from tile to tile, and causally the tile with the mask comes first.
-    const int centre = max(lo_all, min(hi_all - 1, (rb.pos0 + min(q0 + tc.tiles_per_cta * QT, a.Sq) - 1) >> 7));
-    auto order = [&](int i) { return i <= centre - lo_all ? centre - i : lo_all + i; };
-    auto active = [&](int w, int i) {
-        const int kt = order(i);
-        return on[w] && i >= 0 && i < n && kt >= lo[w] && kt < hi[w];
-    };
 
     // Registers: 384 threads start with 168 each (64512); the 256 softmax threads take 216, the
     // other warpgroup keeps 72: 256 * 216 + 128 * 72 = 64512, all of the launch's own.
@@ -297,24 +324,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     if (warp == 8) {
         // ---------------------------------------------------------------- copies
         if (lane == 0 && n > 0) {
-            auto load = [&](uint8_t* dst, const CUtensorMap* map, int pos, int head, int batch, uint64_t* bar) {
-                mbar_arrive_expect_tx(bar, TB);
-#pragma unroll
-                for (int s = 0; s < NSLAB; s++) tma_load_4d(dst + s * SLAB, map, s * 64, pos, head, batch, bar);
-            };
-            auto load_q = [&](int w) {
-                if (on[w]) load(sQ + w * TB, &mq, q0 + w * QT, h * tc.qmul[2], b * tc.qmul[0], q_full + w);
-            };
             bool ok = true;
-            int i = 0;
+            int i = min(n, NST);   // (the first ring is under way)
             for (; i < n; i++) {
-                const int s = i % NST, par = (i / NST - 1) & 1;
-                if (i == 0) load_q(0);
-                if (i >= NST && !(ok = mbar_wait(k_empty + s, par, abort_flag, 51, tc.dev_error))) break;
-                load(sK + s * TB, &mk, order(i) * KT, hk * tc.kmul[2], b * tc.kmul[0], k_full + s);
-                if (i == 0) load_q(1);
-                if (i >= NST && !(ok = mbar_wait(v_empty + s, par, abort_flag, 52, tc.dev_error))) break;
-                load(sV + s * TB, &mv, order(i) * KT, hk * tc.vmul[2], b * tc.vmul[0], v_full + s);
+                const int par = (i / NST - 1) & 1;
+                if (!(ok = mbar_wait(k_empty + i % NST, par, abort_flag, 51, tc.dev_error))) break;
+                copy_k(i);
+                if (!(ok = mbar_wait(v_empty + i % NST, par, abort_flag, 52, tc.dev_error))) break;
+                copy_v(i);
             }
             if (!ok) {   // gave up: let the copies in flight land (tile i may have K only)
                 volatile int never = 0;
@@ -429,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         x.flip = sh.c1 < 0.0f ? 0x80000000u : 0u;   // a negative scale
         x.cap2 = sh.cap2;
         x.slope2 = sh.slope2;
-        x.doc = doc;
+        x.doc = doc < 0 ? -2 : doc;   // (a padding query matches no key, not a padding key either)
         x.k0 = 0.999997882f * x.cap2 * x.c1;
         x.k1 = -0.332985124f * x.cap2 * x.c1 * x.c1 * x.c1;
         x.k2 = 0.124804431f * x.cap2 * x.c1 * x.c1 * x.c1 * x.c1 * x.c1;
@@ -443,13 +460,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         // bias window and documents of key tile kt: fetched a tile ahead
         float pre_b[2] = {0.0f, 0.0f};
         int pre_d = 0;
+        int2 pre_r = make_int2(0, 0);
         auto fetch = [&](int kt) {
             if (MODE & TABLE) {
                 const int d0 = kt * KT - (rb.pos0 + q0 + w * QT) - 127;   // distance of window entry 0
 #pragma unroll
                 for (int u = 0; u < 2; u++) pre_b[u] = __ldg(sh.table + max(-sh.range, min(sh.range, d0 + r + 128 * u)));
             }
-            if (a.doc_k) pre_d = kt * KT + r < a.Sk ? __ldg(a.doc_k + (long long)b * a.Sk + kt * KT + r) : -1;
+            if (a.doc_k) {   // (keys past the length get a number that no query has)
+                pre_d = kt * KT + r < rb.len ? __ldg(a.doc_k + (long long)b * a.Sk + kt * KT + r) : -1;
+                pre_r = __ldg(tc.doc_range + (long long)b * nkt + kt);
+            }
         };
         float base = 0.0f, l = 0.0f;
         bool fresh = true, ok = true;   // fresh: the row has seen nothing yet, base is not set
@@ -490,15 +511,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 x.lin_b = x.d0 >= 0.0f ? -x.slope2 : x.slope2;
                 x.lin_a = ((MODE & SLOPE) ? x.lin_b * x.d0 : 0.0f) + (flat ? bias2(pre_b[0]) : 0.0f);
             }
-            if (((MODE & TABLE) || a.doc_k) && next < n) fetch(order(next));
             x.win = win + (buf * 4 + ((127 - r) & 3)) * WIN + ((127 - r) & ~3);
             x.lim = end - kt * KT;
             x.docs = nullptr;
+            bool none = x.lim <= 0;   // this row sees nothing of the tile
             if (a.doc_k) {
-                const int2 dr = __ldg(tc.doc_range + (long long)b * nkt + kt);
-                if (!__all_sync(0xffffffffu, dr.x == dr.y && doc == dr.x)) x.docs = reinterpret_cast<const int4*>(sdoc + buf * 128);
+                if (!__all_sync(0xffffffffu, pre_r.x == pre_r.y && doc == pre_r.x)) x.docs = reinterpret_cast<const int4*>(sdoc + buf * 128);
+                none = none || doc > pre_r.y || doc < (pre_r.x & INT_MAX);
+                // (the document numbers hide the keys past the length too)
+                if (x.docs && !a.causal) x.lim = KT;
             }
             const bool masked = x.docs || !__all_sync(0xffffffffu, x.lim >= KT);
+            const bool skip = idle || __all_sync(0xffffffffu, none);
+            if (((MODE & TABLE) || a.doc_k) && next < n) fetch(order(next));
 
             ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, it & 1, abort_flag, 58, tc.dev_error));
             if (!ok) break;
@@ -535,9 +560,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_half + w);
             };
-            if (idle) {
+            if (skip) {   // no scores to look at: probabilities of 0
                 s_is_read();
                 wait_product();
+                uint32_t zero[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) zero[e] = 0;
+#pragma unroll
+                for (int q = 0; q < 4; q++) tmem_st16(tP + q * 16, zero);
                 if (!SEP) half_done();
             } else {
                 uint32_t s[128];
