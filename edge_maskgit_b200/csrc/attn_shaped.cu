@@ -46,7 +46,7 @@ void check(const mgc_attention_args& a) {
     need(a.dist_range >= 0 && a.dist_range <= (1 << 30), "dist_range must be from 0 to 2^30");
     need((a.doc_q != nullptr) == (a.doc_k != nullptr), "doc_q and doc_k are given together");
     need(a.reserved == 0, "reserved must be 0");
-    need((long long)a.Sq * (a.Hq / a.Hkv) < (1LL << 30) && a.Sk < (1 << 30), "Sq or Sk is too large");
+    need((long long)a.Sq * (a.Hq / a.Hkv) < (1LL << 28) && a.Sk < (1 << 28), "Sq or Sk is too large");
 }
 
 void check_pointers(const mgc_attention_args& a) {
@@ -112,13 +112,15 @@ Plan plan(const mgc_attention_args& args) {
     } else {
         const long long heads = (long long)a.B * a.Hkv * ((rows + 15) / 16);
         // As many ranges of keys as run at once (two blocks an SM with large heads, three with small ones),
-        // of 128 keys at least; where that leaves more than 2048 keys each, ranges of 1024, so that
-        // rows of unequal length balance.  Up to 8 ranges are one cluster and join in one launch
-        // (4 rows x 4096 keys x 8 heads of 128: 17.5 us, by a second kernel 20; clusters of 16 took 35).
+        // of 128 keys at least.  Long ones of several rows are cut to 1024 keys (at most 32 ranges), so
+        // that rows of unequal length balance, unless there are several rounds of blocks anyway.  Up to
+        // 8 ranges are one cluster and join in one launch (4 rows x 4096 keys x 8 heads of 128: 17.5 us,
+        // by a second kernel 20; clusters of 16 took 35).
         const long long slots = (long long)sms * (a.D > 64 ? 2 : 3);
         const long long n = std::max<long long>(1, slots / heads);
-        long long chunk = std::max<long long>(128, ((a.Sk + n - 1) / n + 63) / 64 * 64);
-        if (chunk > 2048) chunk = 1024;
+        auto up64 = [](long long x) { return (x + 63) / 64 * 64; };
+        long long chunk = std::max<long long>(128, up64((a.Sk + n - 1) / n));
+        if (chunk > 2048 && a.B > 1 && heads < 4 * slots) chunk = std::max<long long>(1024, up64((a.Sk + 31) / 32));
         if (a.Sk > chunk) {
             p.c.chunk = (int)chunk;
             p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);

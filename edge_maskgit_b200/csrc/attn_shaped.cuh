@@ -66,7 +66,7 @@ struct RowBounds { int len, pos0, prefix; };
 __device__ __forceinline__ RowBounds row_bounds(const mgc_attention_args& a, int b) {
     RowBounds r;
     r.len = a.k_len ? max(0, min(a.Sk, __ldg(a.k_len + b))) : a.Sk;
-    r.pos0 = a.q_pos ? max(-(1 << 30), min(1 << 30, __ldg(a.q_pos + b))) : a.Sk - a.Sq;
+    r.pos0 = a.q_pos ? max(-(1 << 29), min(1 << 29, __ldg(a.q_pos + b))) : a.Sk - a.Sq;
     r.prefix = a.causal ? (a.prefix ? max(0, __ldg(a.prefix + b)) : 0) : a.Sk;
     return r;
 }

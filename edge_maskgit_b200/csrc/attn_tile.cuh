@@ -485,9 +485,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         for (int next; it < n_w; i = next, it++) {
             const int kt = order(i), buf = it & 1;
             for (next = i + 1; next < n && !mine(next);) next++;
-            // all of the tile's distances beyond the table's range on one side: one bias for all
+            // All of the tile's distances beyond the table's range on one side: one bias for all.  (Then they
+            // have one sign too, so the tile is linear and does not look at the window.  Capped scores
+            // do: for them the window is always filled.)
             const int dist_lo = kt * KT - (rb.pos0 + q0 + w * QT) - 127, dist_hi = dist_lo + 254;
-            const bool flat = (MODE & TABLE) && (dist_lo >= sh.range || dist_hi <= -sh.range);
+            const bool flat = (MODE & TABLE) && !(MODE & CAP) && (dist_lo >= sh.range || dist_hi <= -sh.range);
             if (((MODE & TABLE) && !flat) || a.doc_k) {
                 if ((MODE & TABLE) && !flat) {   // four copies, each shifted by one entry: every row reads aligned vectors
 #pragma unroll

@@ -308,7 +308,9 @@ namespace lp {
 constexpr int ST = 6, THREADS = 384;   // warp 0 copies, warp 1 issues MMAs, warps 4-11 read results
 constexpr int TN = 256, TM = 256;
 constexpr uint32_t SB = 2 * A_BYTES, RING = ST * SB, SMEM = 1024 + RING + 256;
-constexpr int GROUP = 8;   // tiles walk 8 m-tiles before the next n-tile: both operands stay in L2
+// tiles walk 16 m-tiles before the next n-tile, so that both operands come from L2 (8192 x 4096 x 14336:
+// 727 us; 8 m-tiles 738, 4 769, 32 776)
+constexpr int GROUP = 16;
 }  // namespace lp
 
 // ROWS: x's rows are the lanes (a thread holds consecutive n of one row and moves 16 bytes at a
@@ -518,6 +520,7 @@ extern "C" int mgc_linear(int dtype, const void* x, int64_t ldx, const void* w, 
         need((M == 1 || (ldx >= K && ldx % 8 == 0)) && (N == 1 || (ldw >= K && ldw % 8 == 0)),
              "ldx and ldw must be multiples of 8 and at least K");
         need(M == 1 || (ldy >= N && (!resid || ldr >= N)), "ldy and ldr must be at least N");
+        need(y != resid || ldy == ldr || M == 1, "in place, ldy must be ldr");
         LinArgs a{M, N, K, bias, resid, ldr, y, ldy, act};
         if (dtype == MGC_BF16) run_linear<true>(w, ldw, x, ldx, a, (cudaStream_t)stream);
         else run_linear<false>(w, ldw, x, ldx, a, (cudaStream_t)stream);

@@ -155,7 +155,8 @@ typedef struct mgc_attention_args {
     int32_t reserved;           /* 0 */
     const int32_t* prefix;      /* dev [B] or NULL (0); read only where causal */
     const int32_t* k_len;       /* dev [B] or NULL (Sk); values are clamped to 0..Sk */
-    const int32_t* q_pos;       /* dev [B] or NULL (Sk - Sq: the queries are the last positions) */
+    const int32_t* q_pos;       /* dev [B] or NULL (Sk - Sq: the queries are the last positions); values
+                                   are clamped to +-2^29.  Sk and Sq * Hq / Hkv are below 2^28 */
     const int32_t* doc_q;       /* dev [B][Sq] document numbers, with doc_k, or NULL; < 0 = padding */
     const int32_t* doc_k;       /* dev [B][Sk] */
     void* workspace;            /* dev, 16-byte aligned, mgc_attention_workspace bytes; the call's own */
@@ -232,7 +233,8 @@ void* mgc_runtime_stream(mgc_runtime* rt);
 int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_t* seeds,
                  int steps, float temperature, int32_t* tokens_out);
 
-/* mgc_generate with its logits adjusted (mgc_logits_adjust) before every draw.  All host pointers. */
+/* mgc_generate with its logits adjusted (mgc_logits_adjust) before every draw (controls NULL: not
+ * adjusted).  All host pointers. */
 typedef struct mgc_logit_controls {
     float repetition, frequency, presence;   /* against the codes an image already holds; 1, 0, 0 = none */
     const float* bias;                       /* [codebook] added to every position's logits, or NULL */

@@ -322,6 +322,10 @@ SIZES = [(1, 1, 1, 1, 1, 8), (2, 1, 17, 4, 2, 64), (1, 1, 1000, 8, 1, 128), (3, 
          (2, 127, 127, 2, 1, 64), (1, 128, 128, 1, 1, 128), (1, 129, 257, 3, 3, 48), (1, 257, 257, 4, 4, 48),
          (2, 300, 300, 4, 2, 128), (1, 513, 700, 2, 1, 104), (1, 700, 90, 2, 2, 32), (2, 33, 2000, 14, 2, 64),
          (1, 1, 5000, 16, 1, 40)]
+# enough rows and keys for the 128-row tiles, with small and large heads
+SIZES += [(40, 129, 257, 3, 3, 48), (16, 257, 257, 4, 4, 48), (10, 300, 300, 4, 2, 64), (6, 513, 700, 2, 2, 64),
+          (6, 129, 1000, 4, 4, 32), (1, 1500, 1500, 3, 1, 8), (6, 129, 257, 3, 3, 128), (12, 700, 90, 2, 2, 104),
+          (3, 400, 2100, 2, 2, 72), (1, 2000, 130, 8, 8, 64)]
 
 
 @pytest.mark.parametrize("dt", [F16, BF16])
@@ -334,7 +338,8 @@ def test_attention_plain_and_causal(dt, B, Sq, Sk, Hq, Hkv, D):
 
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("B,Sq,Sk,Hq,Hkv,D", [(2, 1, 300, 4, 2, 64), (2, 5, 1100, 8, 2, 128), (2, 150, 150, 4, 4, 48),
-                                              (1, 400, 650, 4, 2, 128), (2, 290, 290, 2, 2, 96)])
+                                              (1, 400, 650, 4, 2, 128), (2, 290, 290, 2, 2, 96),
+                                              (28, 150, 150, 4, 4, 48), (5, 290, 290, 2, 2, 96), (4, 700, 900, 2, 2, 64)])
 @pytest.mark.parametrize("shape", ["cap", "slopes", "table", "narrow", "all"])
 def test_attention_shaped_scores(dt, B, Sq, Sk, Hq, Hkv, D, shape):
     q, k, v = qkv(B, Sq, Sk, Hq, Hkv, D, dt)
@@ -351,7 +356,22 @@ def test_attention_shaped_scores(dt, B, Sq, Sk, Hq, Hkv, D, shape):
     check_attention(q, k, v, causal=True, prefix=i32(*range(60, 60 + B)), **kw)
 
 
-@pytest.mark.parametrize("Sq,Sk", [(1, 500), (3, 500), (200, 500), (385, 385)])
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("S,D", [(700, 128), (1100, 48), (1300, 48)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_far_beyond_the_table(dt, S, D, cap, slopes, causal):
+    """A table much narrower than the sequence: most keys take one of its two end values, which
+    differ enough to matter."""
+    q, k, v = qkv(1, S, S, 2, 2, D, dt)
+    table = randn(2, 2 * 20 + 1, dtype=F32, seed=53)
+    table[:, 0], table[:, -1] = 1.5, -1.0
+    check_attention(q, k, v, cap=cap, dist_bias=table, causal=causal,
+                    slopes=torch.tensor([0.002, 0.0], device="cuda") if slopes else None)
+
+
+@pytest.mark.parametrize("Sq,Sk", [(1, 500), (3, 500), (200, 500), (385, 385), (300, 500), (40, 3000)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_lengths_positions_and_empty_rows(Sq, Sk, causal):
     """Lengths of zero and one, past the end and negative; positions before the first key."""
@@ -368,11 +388,12 @@ def test_attention_lengths_positions_and_empty_rows(Sq, Sk, causal):
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("lens", [[300], [1, 2, 3, 250, 44], [128, 128, 44], [100, 5, 170, 3], [40] * 7])
-def test_attention_documents(dt, causal, lens):
+@pytest.mark.parametrize("B,D", [(2, 48), (20, 48), (6, 128)])
+def test_attention_documents(dt, causal, lens, B, D):
     S = sum(lens) + 11
     ids = torch.tensor([i for i, n in enumerate(lens) for _ in range(n)] + [-1] * 11, dtype=torch.int32, device="cuda")
-    q, k, v = qkv(2, S, S, 4, 2, 48, dt)
-    doc = torch.stack([ids, ids.flip(0)]).contiguous()
+    q, k, v = qkv(B, S, S, 4, 2, D, dt)
+    doc = torch.stack([ids, ids.flip(0)]).repeat(B // 2, 1).contiguous()
     y = check_attention(q, k, v, causal=causal, doc_q=doc, doc_k=doc, dist_bias=randn(4, 101, dtype=F32, seed=52))
     assert not y[0, -11:].any() and not y[1, :11].any()
     # a document's rows are what it gives alone
@@ -383,7 +404,7 @@ def test_attention_documents(dt, causal, lens):
 
 def test_attention_documents_in_any_order():
     g = torch.Generator(device="cuda").manual_seed(3)
-    for Sq, Sk in ((1, 300), (9, 200), (330, 330)):
+    for Sq, Sk in ((1, 300), (9, 200), (330, 330), (1000, 1000), (600, 1500)):
         dq = torch.randint(-1, 4, (2, Sq), generator=g, device="cuda", dtype=torch.int32)
         dk = torch.randint(-1, 5, (2, Sk), generator=g, device="cuda", dtype=torch.int32)
         q, k, v = qkv(2, Sq, Sk, 2, 2, 64, F16)
@@ -391,11 +412,11 @@ def test_attention_documents_in_any_order():
         check_attention(q, k, v, doc_q=dq, doc_k=dk, causal=True, prefix=i32(70, 0), k_len=i32(Sk, Sk - 40))
 
 
-@pytest.mark.parametrize("Sq,Sk", [(1, 260), (4, 700), (260, 260)])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 260, 64), (4, 700, 64), (260, 260, 64), (420, 420, 128), (900, 900, 64)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_attention_unseen_keys_may_hold_anything(Sq, Sk, bad):
+def test_attention_unseen_keys_may_hold_anything(Sq, Sk, D, bad):
     """NaN and infinities behind k_len, in another document, and after a causal row's position."""
-    q, k, v = qkv(2, Sq, Sk, 2, 1, 64, F16)
+    q, k, v = qkv(2, Sq, Sk, 2, 1, D, F16)
     k_len = i32(Sk - 37, Sk)
     k[0, Sk - 37:], v[0, Sk - 37:] = bad, bad
     y = check_attention(q, k, v, k_len=k_len)
@@ -406,13 +427,17 @@ def test_attention_unseen_keys_may_hold_anything(Sq, Sk, bad):
     k[:, 20:30], v[:, 20:30] = bad, bad
     check_attention(q, k, v, k_len=k_len, doc_q=doc_q, doc_k=doc_k)
     if Sq == Sk:   # keys after a row's own position
-        q, k, v = qkv(1, Sq, Sk, 2, 1, 64, F16)
+        q, k, v = qkv(2, Sq, Sk, 2, 1, D, F16)
         v[0, 100:] = bad
         y = check_attention(q, k, v, causal=True)
-        assert y[0, :100].isfinite().all() and not y[0, 100:].isfinite().any()
+        assert y[0, :100].isfinite().all() and not y[0, 100:].isfinite().any() and y[1].isfinite().all()
+        q, k, v = qkv(2, Sq, Sk, 2, 1, D, F16)   # a NaN score that is seen makes its rows NaN, no others
+        k[1, 150, 0] = math.nan
+        y = check_attention(q, k, v, causal=True)
+        assert y[1, :150].isfinite().all() and y[1, 150:].isnan().all() and y[0].isfinite().all()
 
 
-@pytest.mark.parametrize("Sq,Sk", [(1, 300), (290, 290)])
+@pytest.mark.parametrize("Sq,Sk", [(1, 300), (290, 290), (1300, 1300)])
 def test_attention_lowest_values_and_hidden_distances(Sq, Sk):
     low = torch.finfo(F32).min
     q, k, v = qkv(1, Sq, Sk, 2, 2, 64, BF16)
@@ -429,7 +454,7 @@ def test_attention_lowest_values_and_hidden_distances(Sq, Sk):
     check_attention(q, k, v, dist_bias=table)
 
 
-@pytest.mark.parametrize("Sq,Sk", [(2, 300), (260, 260)])
+@pytest.mark.parametrize("Sq,Sk", [(2, 300), (260, 260), (1300, 1300)])
 def test_attention_large_scores(Sq, Sk):
     q, k, v = qkv(1, Sq, Sk, 2, 2, 64, BF16)
     check_attention(q * 30, k * 30, v, scale=1.0)
@@ -513,18 +538,20 @@ def _step_ref(x, st):
     return logits_ref(z, history=st["hist"], penalties=st["pen"], allowed=st["allowed"])[0]
 
 
-def test_a_step_of_all_three():
+@pytest.mark.parametrize("B", [2, 30])
+def test_a_step_of_all_three(B):
     """Six roundings to bf16 follow one another, each of relative size 2^-8 at most and spread over
     sums: the 2-norm of the difference stays below their plain sum, 6 * 2^-8 of the result's."""
-    st, x = _step_state()
+    st, x = _step_state(B)
     y, ref = _step(x, st), _step_ref(x, st)
     live = ref > -math.inf
     assert torch.equal(live, y > -math.inf)
     assert ((y.double() - ref)[live].norm() / ref[live].norm()).item() < 6 * 2.0 ** -8
 
 
-def test_streams_and_graph_replays_agree():
-    st, x = _step_state()
+@pytest.mark.parametrize("B", [2, 30])
+def test_streams_and_graph_replays_agree(B):
+    st, x = _step_state(B)
     want = _step(x, st)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

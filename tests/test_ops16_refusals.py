@@ -21,6 +21,7 @@ LINEAR = dict(dtype=1, x=A, ldx=64, w=A, ldw=64, M=4, N=8, K=64, bias=None, act=
     (dict(act=3), "act"), (dict(act=-1), "act"), (dict(x=None), "NULL"), (dict(y=None), "NULL"), (dict(x=A + 2), "aligned"),
     (dict(w=A + 8), "aligned"), (dict(y=A + 1), "aligned"), (dict(bias=A + 2), "aligned"), (dict(ldx=63), "ldx"),
     (dict(ldx=68), "ldx"), (dict(ldw=56), "ldx and ldw"), (dict(ldy=7), "ldy"), (dict(resid=A, ldr=7), "ldy and ldr"),
+    (dict(resid=A, y=A, ldr=8, ldy=16), "in place"),
 ])
 def test_linear_refuses(bad, word):
     from edge_maskgit_b200._lib import lib
