@@ -159,20 +159,25 @@ def embed(tok, pos, tokens, B: int, S: int):
 # ----------------------------------------------------------------- 16-bit operators
 # The checks below look at each tensor's type, device and gradient flag in one condition and
 # explain only what failed: a small call is as long as its host side.
-def _codes():
-    import torch
-    return {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
-
-
-_CODE: dict = {}
+_CODE: dict = {}     # torch dtype -> code, filled with torch's names on the first call
+_torch = None
 # mgc_attention_args; mgc_attention takes its address
 _ATTN_PACK = struct.Struct("8i4Q12q2f2Q2i5Q2Q")
 assert _ATTN_PACK.size == C.sizeof(AttentionArgs)
 
 
+def _load_torch():
+    global _torch, _device, _raw_stream
+    import torch
+    _CODE.update({torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32})
+    _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _torch = torch
+    return torch
+
+
 def _code_of(t, name, f32: bool = False) -> int:
-    if not _CODE:
-        _CODE.update(_codes())
+    if _torch is None:
+        _load_torch()
     code = _CODE.get(getattr(t, "dtype", None))
     if code is None or (code == F32 and not f32):
         raise MgcError(f"{name} must be {'float32, ' if f32 else ''}float16 or bfloat16, not {getattr(t, 'dtype', type(t))}")
@@ -180,7 +185,7 @@ def _code_of(t, name, f32: bool = False) -> int:
 
 
 def _refuse(t, name, dtype, index):
-    import torch
+    torch = _torch or _load_torch()
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index:
         raise MgcError(f"{name} must be a CUDA tensor" + (f" on device {index}" if index >= 0 else ""))
     if t.dtype != dtype:
@@ -217,34 +222,33 @@ def _matrix(t, name, dtype, index):
     return ld
 
 
-def _call(index, what, fn, *args):
-    """Calls the library on torch's current stream of device `index`, made current for the call."""
-    import torch
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, stream)
-    if rc != 0:
-        check(rc, what)
+def _elsewhere(index, what, fn, *args):
+    """Calls the library with device `index` made current, on torch's stream there."""
+    with _torch.cuda.device(index):
+        check(fn(*args, _raw_stream(index)), what)
 
 
 def linear(x, w, bias=None, act: int = 0, resid=None, out=None):
     """y = act(x W^T + bias) + resid in f16 / bf16 (mgc_linear): x [M][K], w [N][K], resid and y
     [M][N], bias f32 [N]; act 0 none, 1 erf-GELU, 2 SiLU; summed in f32, rounded once.  Rows may be
     strided; K and the row strides of x and w are multiples of 8.  `out` may be `resid`."""
-    import torch
-    code = _code_of(x, "x")
+    code = _CODE.get(getattr(x, "dtype", None)) or _code_of(x, "x")
     dt, index = x.dtype, x.get_device()
-    ldx, ldw = _matrix(x, "x", dt, index), _matrix(w, "w", dt, index)
+    if index < 0 or w.dtype is not dt or w.get_device() != index or x.requires_grad or w.requires_grad or \
+            not (x.dim() == w.dim() == 2):
+        _matrix(x, "x", dt, index)
+        _matrix(w, "w", dt, index)
     (M, K), (N, Kw) = x.shape, w.shape
+    (ldx, one_x), (ldw, one_w) = x.stride(), w.stride()
+    if (one_x != 1 or one_w != 1) and K > 1:
+        raise MgcError("the last axes of x and w must be contiguous")
     if Kw != K:
         raise MgcError(f"x has {K} columns, w has {Kw}")
-    bias_p = _vector(bias, "bias", torch.float32, index, (N,)) if bias is not None else None
+    bias_p = _vector(bias, "bias", _torch.float32, index, (N,)) if bias is not None else None
     resid_p, ldr = None, 0
     if resid is not None:
-        resid_p, ldr = resid.data_ptr(), _matrix(resid, "resid", dt, index)
+        ldr = _matrix(resid, "resid", dt, index)
+        resid_p = resid.data_ptr()
         if resid.shape != (M, N):
             raise MgcError(f"resid must have shape {[M, N]}, not {list(resid.shape)}")
     if out is None:
@@ -253,8 +257,12 @@ def linear(x, w, bias=None, act: int = 0, resid=None, out=None):
         ldy = _matrix(out, "out", dt, index)
         if out.shape != (M, N):
             raise MgcError(f"out must have shape {[M, N]}, not {list(out.shape)}")
-    _call(index, "linear", lib.mgc_linear, code, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, bias_p, act, resid_p, ldr,
-          out.data_ptr(), ldy)
+    if _device() != index:
+        _elsewhere(index, "linear", lib.mgc_linear, code, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, bias_p, act,
+                   resid_p, ldr, out.data_ptr(), ldy)
+    elif lib.mgc_linear(code, x.data_ptr(), ldx, w.data_ptr(), ldw, M, N, K, bias_p, act, resid_p, ldr, out.data_ptr(), ldy,
+                        _raw_stream(index)):
+        check(-1, "linear")
     return out
 
 
@@ -281,7 +289,6 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
     over the keys j < k_len[b] that are j <= p or j < prefix[b] if causal, with doc_q[b][i] ==
     doc_k[b][j] >= 0 if given.  A query that sees no key gives zeros.  scale defaults to D ** -0.5;
     slopes f32 [Hq]; prefix, k_len, q_pos int32 [B]; doc_q, doc_k int32 [B][Sq], [B][Sk]."""
-    import torch
     code = _CODE.get(getattr(q, "dtype", None)) or _code_of(q, "q")
     dt, index = q.dtype, q.get_device()
     if index < 0 or not (k.dtype is dt and v.dtype is dt and k.get_device() == index and v.get_device() == index) or \
@@ -295,13 +302,13 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
         raise MgcError("the last axes of q, k and v must be contiguous")
     if k.shape != v.shape or Bk != B or Dk != D:
         raise MgcError(f"k and v must be [{B}][Sk][Hkv][{D}], not {list(k.shape)} and {list(v.shape)}")
-    i32, reach = torch.int32, 0
+    i32, reach = _torch.int32, 0
     slopes_p = table_p = prefix_p = k_len_p = q_pos_p = doc_q_p = doc_k_p = None
     if slopes is not None:
-        slopes_p = _vector(slopes, "slopes", torch.float32, index, (Hq,))
+        slopes_p = _vector(slopes, "slopes", _torch.float32, index, (Hq,))
     if dist_bias is not None:
         reach = dist_bias.shape[-1] // 2
-        table_p = _vector(dist_bias, "dist_bias", torch.float32, index, (Hq, 2 * reach + 1))
+        table_p = _vector(dist_bias, "dist_bias", _torch.float32, index, (Hq, 2 * reach + 1))
     if prefix is not None:
         if not causal:
             raise MgcError("prefix is for causal attention")
@@ -324,20 +331,25 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
             qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os[0], os[1], os[2],
             D ** -0.5 if scale is None else scale, cap, slopes_p or 0, table_p or 0, reach, 0, prefix_p or 0, k_len_p or 0,
             q_pos_p or 0, doc_q_p or 0, doc_k_p or 0)
+    if _device() != index:   # (the split follows the current device's size)
+        with _torch.cuda.device(index):
+            _attention(index, q, head)
+    else:
+        _attention(index, q, head)
+    return out
+
+
+def _attention(index, q, head):
     args = _ATTN_PACK.pack(*head, 0, 0)
     need = C.c_uint64()
-    if torch._C._cuda_getDevice() == index:   # (the split follows the device's size)
-        rc = lib.mgc_attention_workspace(args, C.byref(need))
-    else:
-        with torch.cuda.device(index):
-            rc = lib.mgc_attention_workspace(args, C.byref(need))
+    rc = lib.mgc_attention_workspace(args, C.byref(need))
+    if rc == 0:
+        if need.value:   # from torch's allocator: this stream's (or this capture's) own memory
+            ws = _torch.empty(need.value, dtype=_torch.uint8, device=q.device)
+            args = _ATTN_PACK.pack(*head, ws.data_ptr(), need.value)
+        rc = lib.mgc_attention(args, _raw_stream(index))
     if rc != 0:
         check(rc, "attention")
-    if need.value:   # from torch's allocator: this stream's (or this capture's) own memory
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        args = _ATTN_PACK.pack(*head, ws.data_ptr(), need.value)
-    _call(index, "attention", lib.mgc_attention, args)
-    return out
 
 
 def logits_adjust(logits, history=None, hist_len=None, penalties=None, bias=None, allowed=None, out=None):
@@ -348,12 +360,11 @@ def logits_adjust(logits, history=None, hist_len=None, penalties=None, bias=None
     v % 32 of allowed[v // 32] is 0.  logits f32, f16 or bf16; history int32 [R][L], hist_len int32
     [R], penalties f32 [R][3] = (rep, freq, pres), bias f32 [R][V], allowed int32 [R][(V + 31) // 32].
     One-axis history, penalties, bias or allowed are shared by all rows.  `out` may be `logits`."""
-    import torch
     code = _code_of(logits, "logits", f32=True)
     dt, index = logits.dtype, logits.get_device()
     ld = _matrix(logits, "logits", dt, index)
     R, V = logits.shape
-    i32, f32 = torch.int32, torch.float32
+    i32, f32 = _torch.int32, _torch.float32
 
     def table(t, name, dtype, width):   # (pointer, row stride), 0 = one row for all
         if t.dim() == 1:
@@ -396,8 +407,12 @@ def logits_adjust(logits, history=None, hist_len=None, penalties=None, bias=None
         ld_o = _matrix(out, "out", dt, index)
         if out.shape != logits.shape:
             raise MgcError(f"out must have shape {list(logits.shape)}, not {list(out.shape)}")
-    _call(index, "logits_adjust", lib.mgc_logits_adjust, code, logits.data_ptr(), ld, R, V, hist_p, ld_h, L, len_p, pen_p,
-          ld_p, bias_p, ld_b, allowed_p, ld_a, out.data_ptr(), ld_o)
+    if _device() != index:
+        _elsewhere(index, "logits_adjust", lib.mgc_logits_adjust, code, logits.data_ptr(), ld, R, V, hist_p, ld_h, L, len_p,
+                   pen_p, ld_p, bias_p, ld_b, allowed_p, ld_a, out.data_ptr(), ld_o)
+    elif lib.mgc_logits_adjust(code, logits.data_ptr(), ld, R, V, hist_p, ld_h, L, len_p, pen_p, ld_p, bias_p, ld_b,
+                               allowed_p, ld_a, out.data_ptr(), ld_o, _raw_stream(index)):
+        check(-1, "logits_adjust")
     return out
 
 
