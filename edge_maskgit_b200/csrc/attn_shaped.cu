@@ -125,6 +125,14 @@ Plan plan(const mgc_attention_args& args) {
             p.c.chunk = (int)chunk;
             p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);
             p.c.cluster = p.c.nsplit <= 8;
+            // Few heads and not too many keys: a cluster of 8 blocks of eight warps, one launch (1 row x 4096
+            // keys x 8 heads of 128: 13.2 us a call; by a second kernel 15.2, although its GPU time is
+            // 9.7 against 11.3: the second launch and the workspace cost the host more).
+            if (p.c.nsplit > 8 && a.Sk <= 4096 && heads * 16 <= sms) {
+                p.c.chunk = (int)up64((a.Sk + 7) / 8);
+                p.c.nsplit = (a.Sk + p.c.chunk - 1) / p.c.chunk;
+                p.c.cluster = p.c.wide = 1;
+            }
         }
     }
     p.bytes = p.doc_bytes;

@@ -18,6 +18,7 @@ struct AttnCall {
     int g;                 // query heads per key head
     int nsplit, chunk;     // splits of the key range; keys per split (a multiple of the key tile)
     int cluster;           // few queries: the splits are one cluster, joined in distributed shared memory
+    int wide;              // few queries: eight warps a block instead of four
     float* opart;
     float2* mlpart;
 };

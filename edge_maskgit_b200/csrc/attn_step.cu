@@ -4,7 +4,7 @@
 // Bound by the bytes of k and v, which are read once: the Sq * (Hq / Hkv) query rows that share a
 // key head sit in one 16-row tensor-core tile (mma.sync m16n8k16; with 16 rows or fewer per key the
 // tile is memory-bound by an order of magnitude, so the tcgen05 path with its 128-row tile would
-// add nothing).  The key range is split over CTAs, and inside a CTA over four warps.  Each warp has
+// add nothing).  The key range is split over CTAs, and inside a CTA over four or eight warps.  Each warp has
 // its own ring of 16-key stages filled by cp.async, so the main loop has no CTA-wide barrier; the
 // online softmax keeps (max, sum, output) in registers, and warps and CTAs are joined at the end: up to
 // 8 CTAs are one cluster and join in distributed shared memory, more leave partial results in the
@@ -16,15 +16,16 @@
 namespace mgc {
 namespace {
 
-constexpr int WARPS = 4, KT = 16, STAGES = 3;
+constexpr int KT = 16, STAGES = 3;
 template <int DP> constexpr int row_bytes() { return DP * 2 + 16; }   // odd in 16-byte units: ldmatrix without conflicts
 template <int DP> constexpr int stage_bytes() { return 2 * KT * row_bytes<DP>(); }
-template <int DP> constexpr int ring_bytes() { return WARPS * STAGES * stage_bytes<DP>(); }
+template <int DP, int WARPS> constexpr int ring_bytes() { return WARPS * STAGES * stage_bytes<DP>(); }
 template <int DP> constexpr int join_row() { return DP + 8; }   // floats: eight rows' writes meet no bank twice
-template <int DP> constexpr int join_bytes() { return WARPS * 16 * (join_row<DP>() * 4 + 8); }
+template <int DP, int WARPS> constexpr int join_bytes() { return WARPS * 16 * (join_row<DP>() * 4 + 8); }
 template <int DP> constexpr int part_bytes() { return 16 * (DP * 4 + 8); }   // a CTA's own result, for its cluster
-template <int DP> constexpr int smem_bytes() {
-    return ring_bytes<DP>() > join_bytes<DP>() + part_bytes<DP>() ? ring_bytes<DP>() : join_bytes<DP>() + part_bytes<DP>();
+template <int DP, int WARPS> constexpr int smem_bytes() {
+    constexpr int ring = ring_bytes<DP, WARPS>(), join = join_bytes<DP, WARPS>() + part_bytes<DP>();
+    return ring > join ? ring : join;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -84,7 +85,7 @@ __device__ __forceinline__ void write_row4(const AttnCall& c, int b, int h, int 
 }
 
 // grid: splits x (batch row, key head, 16-row block), splits fastest
-template <bool BF16, int DP>
+template <bool BF16, int DP, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_constant__ AttnCall c) {
     constexpr int RB = row_bytes<DP>(), SB = stage_bytes<DP>(), NK = DP / 16, CH = DP / 8;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
         for (int d = 0; d < DP / 8; d++)
             *reinterpret_cast<float2*>(so + (warp * 16 + qr + 8 * u) * JR + d * 8 + qc) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
     }
-    float* po = reinterpret_cast<float*>(smem + join_bytes<DP>());   // [16][DP]
+    float* po = reinterpret_cast<float*>(smem + join_bytes<DP, WARPS>());   // [16][DP]
     float2* pml = reinterpret_cast<float2*>(po + 16 * DP);            // [16]
     __syncthreads();
     for (int r = warp; r < 16 && blk * 16 + r < rows; r += WARPS) {
@@ -369,20 +370,26 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const __grid_constant
     write_row4<BF16>(c, (int)(bi / a.Sq), (int)(id % a.Hq), (int)(bi % a.Sq), acc, ll);
 }
 
-template <bool BF16, int DP>
-void launch_step(const AttnCall& c, cudaStream_t st) {
+template <bool BF16, int DP, int WARPS>
+void launch_warps(const AttnCall& c, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
-    auto kernel = attn_step_kernel<BF16, DP>;
-    allow_smem(kernel, smem_bytes<DP>(), done);
+    auto kernel = attn_step_kernel<BF16, DP, WARPS>;
+    constexpr int smem = smem_bytes<DP, WARPS>();
+    allow_smem(kernel, smem, done);
     const long long blocks = (long long)c.a.B * c.a.Hkv * ((c.a.Sq * c.g + 15) / 16) * c.nsplit;
     if (blocks > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
     if (c.cluster) {
-        launch_clusters(kernel, (unsigned)blocks, WARPS * 32, smem_bytes<DP>(), c.nsplit, st, c);
+        launch_clusters(kernel, (unsigned)blocks, WARPS * 32, smem, c.nsplit, st, c);
         return;
     }
     ++g_launch_count;
-    const cudaError_t e = launch_k(kernel, dim3((unsigned)blocks), dim3(WARPS * 32), smem_bytes<DP>(), st, c);
+    const cudaError_t e = launch_k(kernel, dim3((unsigned)blocks), dim3(WARPS * 32), smem, st, c);
     if (e != cudaSuccess) throw std::runtime_error(std::string("launch failed: ") + cudaGetErrorString(e));
+}
+template <bool BF16, int DP>
+void launch_step(const AttnCall& c, cudaStream_t st) {
+    if (c.wide) launch_warps<BF16, DP, 8>(c, st);
+    else launch_warps<BF16, DP, 4>(c, st);
 }
 
 template <bool BF16>
