@@ -162,7 +162,7 @@ __device__ __forceinline__ void max32(float (&hi)[4], const uint32_t* s) {
         hi[(j >> 1) & 3] = max3_nan(hi[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
 }
 
-// 32 columns of a row's output in TMEM, times a power of two.
+// 32 columns of a row's output in TMEM, times f.
 __device__ __forceinline__ void scale_o(uint32_t taddr, float f) {
     uint32_t v[32];
     tmem_ld32(taddr, v);
@@ -450,11 +450,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         x.k0 = 0.999997882f * x.cap2 * x.c1;
         x.k1 = -0.332985124f * x.cap2 * x.c1 * x.c1 * x.c1;
         x.k2 = 0.124804431f * x.cap2 * x.c1 * x.c1 * x.c1 * x.c1 * x.c1;
-        // Probabilities are 2^(t - base).  base is a whole number, set at the first scores to SHIFT below
-        // their maximum, and again only when a score passes it by SLACK: what was computed before is
-        // then scaled by a power of two, exactly.  So no pass over the tile has to find its maximum
-        // first.  In f16 probabilities go up to 2^15, which it holds, and its smallest normal number
-        // is 2^-17 of the row's maximum; bf16 has room for more.
+        // Probabilities are 2^(t - base).  base is set at the first scores to SHIFT below their maximum,
+        // whose probability is then a power of two and rounds to itself, and again only when a score
+        // passes it by SLACK: the sum and the output so far are then scaled, in f32.  So no pass over the
+        // tile has to find its maximum first.  In f16 probabilities go up to 2^15, which it holds, and its
+        // smallest normal number is 2^-17 of the row's maximum; bf16 has room for more.
         constexpr float SHIFT = 3.0f, SLACK = BF16 ? 40.0f : 15.0f;
 
         // bias window and documents of key tile kt: fetched a tile ahead
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 if (move) {
                     float alpha = 1.0f;
                     if (set) {
-                        const float nb = ceilf(mx) - SHIFT;
+                        const float nb = mx - SHIFT;
                         if (!fresh) alpha = ex2_approx(base - nb);
                         l *= alpha;
                         base = nb;
