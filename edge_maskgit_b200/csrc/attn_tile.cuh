@@ -682,11 +682,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     probs([&](uint64_t t, int j) {
                         return fma2(t, c2, pack2(fmaf((float)j, x.lin_b, la), fmaf((float)(j + 1), x.lin_b, la)));
                     });
-                } else if (!(MODE & CAP) && raw) {
-                    const uint64_t la2 = pack2(x.lin_a - base, x.lin_a - base);
-                    probs([&](uint64_t t, int) { return fma2(t, c2, la2); });
-                } else {
-                    probs([&](uint64_t t, int) { return add2(t, nb2); });
+                } else if (MODE == 0) {
+                    probs([&](uint64_t t, int) { return fma2(t, c2, nb2); });
+                } else {   // raw scores, or t already: one form
+                    const float k = raw ? x.c1 : 1.0f, off = (raw ? x.lin_a : 0.0f) - base;
+                    const uint64_t k2 = pack2(k, k), off2 = pack2(off, off);
+                    probs([&](uint64_t t, int) { return fma2(t, k2, off2); });
                 }
                 float e0, e1, e2, e3;
                 unpack2(add2(sum2[0], sum2[1]), e0, e1);
