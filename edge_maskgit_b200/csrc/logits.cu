@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kThreads, 3) logits_adjust_kernel(const LogitA
     const int lead = (int)((reinterpret_cast<uintptr_t>(zrow) & 15) / E::SIZE);
     const bool out_vec = ((reinterpret_cast<uintptr_t>(zrow) ^ reinterpret_cast<uintptr_t>(orow)) & 15) == 0;
     const int t0 = c * chunk - lead;   // token of the chunk's first value (may be < 0); V + chunk < 2^31
+    if (t0 >= a.V) return;   // (chunks are counted for the longest lead: a row with less may not fill the last)
     const float* brow = BIAS ? a.bias + r * a.ld_bias : nullptr;
 
     auto seg_at = [&](int k) { return (k * kWarps + warp) * SEG; };   // segment k's place in the chunk
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(kThreads, 3) logits_adjust_kernel(const LogitA
         __syncthreads();
         const int32_t* h = a.hist + r * a.ld_hist;
         const int first = max(t0, 0);
-        const unsigned span = (unsigned)(min(t0 + chunk, a.V) - first);   // > 0
+        const unsigned span = (unsigned)(min(t0 + chunk, a.V) - first);   // > 0: t0 < V
         auto count = [&](int tok) {
             if ((unsigned)tok - (unsigned)first < span) {   // (a negative number is a large one)
                 atomicAdd(s_count + (tok - t0), 1u);   // integers: the order does not matter

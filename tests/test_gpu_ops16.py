@@ -177,6 +177,21 @@ def test_logits_all(dt, R, V, L):
                  bias=randn(R, V, dtype=F32, seed=23), allowed=ints(-2 ** 31, 2 ** 31 - 1, R, words, seed=24))
 
 
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("V", [2045, 2046, 2047, 2048, 4089, 4093, 4095, 4096, 8189, 8191, 8192])
+@pytest.mark.parametrize("R", [6, 400])
+def test_logits_rows_that_end_at_a_chunks_border(dt, V, R):
+    """A row may fill its last chunk exactly, pass it by its lead, or leave it empty."""
+    kw = dict(history=ints(-2, V + 2, R, 9, seed=81), penalties=torch.tensor([1.3, 0.4, 0.2], device="cuda"),
+              bias=randn(V, dtype=F32, seed=82), allowed=ints(-2 ** 31, 2 ** 31 - 1, (V + 31) // 32, seed=83))
+    z = randn(R, V, dtype=dt, seed=84, std=3.0)
+    from edge_maskgit_b200 import runtime as rt
+    y = rt.logits_adjust(z, **kw)
+    rows = list(range(min(R, 8))) + [R - 1]
+    pick = dict(kw, history=kw["history"][rows])
+    within(y[rows], *logits_ref(z[rows], **pick))
+
+
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("hist", [False, True])
 @pytest.mark.parametrize("bias", [False, True])
