@@ -46,7 +46,8 @@ __device__ __forceinline__ float gelu16(float x) {
     p = fmaf(p, t, 0.107331982f);
     p = fmaf(p, t, 0.103501627f);
     const float h = ex2_approx(a * a * -0.7213475204f) * (p * t);
-    return fmaf(0.5f, x + fabsf(x), -(a * h));   // (x + |x|: a NaN stays one)
+    const float half = 0.5f * x;
+    return fmaf(-a, h, half + fabsf(half));   // (max(x, 0) with a NaN that stays one; x + |x| would overflow)
 }
 __device__ __forceinline__ float silu16(float x) {
     float r;
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(ls::THREADS) linear_split_kernel(const __grid_
         __syncwarp();
         cluster_sync_all();
         if (warp >= 2 && ok && n < a.N) {
-constexpr int G = BN == 16 ? 2 : 8;   // columns in flight: remote reads take a microsecond
+            constexpr int G = BN == 16 ? 2 : 8;   // columns in flight: remote reads take a microsecond
             const int c0 = cols * rank / split, c1 = cols * (rank + 1) / split;   // this CTA's columns
 #pragma unroll 1
             for (int c = c0; c < c1; c += G) {

@@ -94,6 +94,19 @@ def test_linear_epilogue(dt, act, M, N, use_bias, use_resid):
                  resid=randn(M, N, dtype=dt, seed=6) if use_resid else None)
 
 
+@pytest.mark.parametrize("act", [1, 2])
+@pytest.mark.parametrize("M,N", [(3, 64), (700, 2304), (8200, 2304)])
+def test_linear_activation_near_the_largest_float(act, M, N):
+    """Sums between half of float32's largest value and the largest: the activation is the value itself
+    (or -0), not infinity.  One term of K = 8 is not 0, so the sum is exact."""
+    from edge_maskgit_b200 import runtime as rt
+    x, w = torch.zeros(M, 8, device="cuda", dtype=BF16), torch.zeros(N, 8, device="cuda", dtype=BF16)
+    x[:, 0] = 2.0 ** 64
+    w[0::2, 0], w[1::2, 0] = 1.5 * 2.0 ** 63, -1.5 * 2.0 ** 63
+    y = rt.linear(x, w, act=act)
+    assert torch.all(y[:, 0::2] == 1.5 * 2.0 ** 127) and torch.all(y[:, 1::2] == 0)
+
+
 @pytest.mark.parametrize("M,N", [(7, 300), (2000, 2056)])
 def test_linear_strided_rows_and_in_place_residual(M, N):
     K = 136
@@ -369,6 +382,16 @@ def test_attention_shaped_scores(dt, B, Sq, Sk, Hq, Hkv, D, shape):
         kw.update(dist_bias=randn(Hq, 2 * 3 + 1, dtype=F32, seed=51, std=2.0))
     check_attention(q, k, v, **kw)
     check_attention(q, k, v, causal=True, prefix=i32(*range(60, 60 + B)), **kw)
+
+
+@pytest.mark.parametrize("S,D", [(40, 64), (700, 64), (700, 128)])
+@pytest.mark.parametrize("cap,scale", [(2.0 ** -10, 2.0 ** 10), (2.0 ** 10, 0.125), (2.0 ** 10, 200.0), (0.0, 2.0 ** 100)])
+def test_attention_constants_at_their_bounds(S, D, cap, scale):
+    q, k, v = qkv(1, S, S, 4, 2, D, F16, seed=66)
+    if scale > 1e3:   # scores of 0 and of one size: each is either nothing or far past the cap
+        q, k = torch.zeros_like(q), torch.zeros_like(k)
+        q[..., 0], k[:, S // 2:, :, 0] = 1.0, -1.0
+    check_attention(q, k, v, cap=cap, scale=scale)
 
 
 @pytest.mark.parametrize("dt", [F16, BF16])
