@@ -41,8 +41,11 @@ void check(const mgc_attention_args& a) {
     need(a.Hkv > 0 && a.Hq > 0 && a.Hq % a.Hkv == 0, "Hq must be a positive multiple of Hkv");
     need(a.D >= 8 && a.D <= 128 && a.D % 8 == 0, "D must be a multiple of 8 from 8 to 128");
     need(a.causal == 0 || a.causal == 1, "causal must be 0 or 1");
-    need(std::isfinite(a.scale), "scale must be finite");
-    need(a.cap >= 0.0f && std::isfinite(a.cap), "cap must be finite and not negative");
+    // Capped scores carry an absolute error of up to 2^-20 cap, at 1024 what one rounding step of an f16
+    // result is; and the constants of the cap, (scale / cap)^5 cap at most, have to be finite.
+    need(std::fabs(a.scale) <= 0x1p100f, "scale must be at most 2^100");
+    need(a.cap == 0.0f || (a.cap >= 0x1p-10f && a.cap <= 0x1p10f), "cap must be 0 or from 2^-10 to 2^10");
+    need(a.cap == 0.0f || std::fabs(a.scale) <= 0x1p20f * a.cap, "scale must be at most 2^20 cap");
     need(a.dist_range >= 0 && a.dist_range <= (1 << 30), "dist_range must be from 0 to 2^30");
     need((a.doc_q != nullptr) == (a.doc_k != nullptr), "doc_q and doc_k are given together");
     need(a.reserved == 0, "reserved must be 0");

@@ -288,7 +288,7 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
         s += dist_bias[h][clamp(j - p, -R, R) + R]     (dist_bias f32 [Hq][2 R + 1])
     over the keys j < k_len[b] that are j <= p or j < prefix[b] if causal, with doc_q[b][i] ==
     doc_k[b][j] >= 0 if given.  A query that sees no key gives zeros.  scale defaults to D ** -0.5;
-    slopes f32 [Hq]; prefix, k_len, q_pos int32 [B]; doc_q, doc_k int32 [B][Sq], [B][Sk]."""
+    cap is 0 or from 2^-10 to 2^10; slopes f32 [Hq]; prefix, k_len, q_pos int32 [B]; doc_q, doc_k int32 [B][Sq], [B][Sk]."""
     code = _CODE.get(getattr(q, "dtype", None)) or _code_of(q, "q")
     dt, index = q.dtype, q.get_device()
     if index < 0 or not (k.dtype is dt and v.dtype is dt and k.get_device() == index and v.get_device() == index) or \

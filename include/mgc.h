@@ -147,8 +147,8 @@ typedef struct mgc_attention_args {
                                    repeats (not in out) */
     int64_t v_stride[3];
     int64_t out_stride[3];
-    float scale;
-    float cap;                  /* 0 = none */
+    float scale;                /* |scale| at most 2^100, and 2^20 cap */
+    float cap;                  /* 0 = none, or from 2^-10 to 2^10 */
     const float* slopes;        /* dev [Hq] or NULL */
     const float* dist_bias;     /* dev [Hq][2 * dist_range + 1] or NULL */
     int32_t dist_range;         /* >= 0 */

@@ -87,6 +87,17 @@ def test_attention_refuses_sizes(bad, word):
         assert rc == -1 and word in _err(lib)
 
 
+@pytest.mark.parametrize("bad,word", [
+    (dict(cap=2.0 ** -11), "cap"), (dict(cap=2.0 ** 11), "cap"), (dict(scale=2.0 ** 101), "scale"),
+    (dict(scale=-2.0 ** 101), "scale"), (dict(scale=2.0 ** 13, cap=2.0 ** -8), "scale must be at most 2^20 cap"),
+])
+def test_attention_refuses_constants_out_of_range(bad, word):
+    """A cap far above 1024 would carry its rounding into the scores; a scale far above the cap overflows."""
+    from edge_maskgit_b200._lib import lib
+    need = C.c_uint64()
+    assert lib.mgc_attention_workspace(C.byref(_attn(**bad)), C.byref(need)) == -1 and word in _err(lib)
+
+
 def test_null_structs_are_refused():
     from edge_maskgit_b200._lib import lib
     assert lib.mgc_attention(None, None) == -1 and "NULL" in _err(lib)
