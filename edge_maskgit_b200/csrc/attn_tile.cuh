@@ -47,6 +47,11 @@ struct TileCall {
     int kmul[3], vmul[3], qmul[3];   // 0 where a stride is 0 (batch, -, head): the map has one entry there
 };
 
+// Where a tile's bias is linear in the key, its part that all keys share joins the base: exponents are then
+// s c1 + (bias - base), and the scores must not be lost in the rounding of bias or base.  Up to this size
+// of the bias (in base 2) that rounding is below 2^-3; larger ones are added to each score.
+constexpr float LINEAR_MAX = 1048576.0f;
+
 // What the softmax of one row needs of one key tile.
 struct RowTile {
     float c1;              // no cap: scale in base 2 (sign in `flip`); cap: scale / cap
@@ -487,9 +492,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             for (next = i + 1; next < n && !mine(next);) next++;
             // All of the tile's distances beyond the table's range on one side: one bias for all.  (Then they
             // have one sign too, so the tile is linear and does not look at the window.  Capped scores
-            // do: for them the window is always filled.)
+            // do: for them the window is always filled.)  A bias that would absorb the scores, the type's
+            // lowest value say, has to be added to each of them: it takes the window.
             const int dist_lo = kt * KT - (rb.pos0 + q0 + w * QT) - 127, dist_hi = dist_lo + 254;
-            const bool flat = (MODE & TABLE) && !(MODE & CAP) && (dist_lo >= sh.range || dist_hi <= -sh.range);
+            const bool flat = (MODE & TABLE) && !(MODE & CAP) && (dist_lo >= sh.range || dist_hi <= -sh.range) &&
+                              (fabsf(pre_b[0]) <= LINEAR_MAX || pre_b[0] == -INFINITY);
             if (((MODE & TABLE) && !flat) || a.doc_k) {
                 if ((MODE & TABLE) && !flat) {   // four copies, each shifted by one entry: every row reads aligned vectors
 #pragma unroll
@@ -509,7 +516,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             bool linear = false;
             if (MODE & (SLOPE | TABLE)) {
                 linear = !(MODE & TABLE) || flat;
-                if (MODE & SLOPE) linear = linear && __all_sync(0xffffffffu, x.d0 >= 0.0f || x.d0 <= -127.0f);
+                if (MODE & SLOPE)
+                    linear = linear && __all_sync(0xffffffffu, (x.d0 >= 0.0f || x.d0 <= -127.0f) &&
+                                                                   fabsf(x.slope2) * (fabsf(x.d0) + 127.0f) <= LINEAR_MAX);
                 x.lin_b = x.d0 >= 0.0f ? -x.slope2 : x.slope2;
                 x.lin_a = ((MODE & SLOPE) ? x.lin_b * x.d0 : 0.0f) + (flat ? bias2(pre_b[0]) : 0.0f);
             }

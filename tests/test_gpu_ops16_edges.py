@@ -1,0 +1,79 @@
+"""GPU: the 16-bit operators where they can go wrong at the ends of their ranges: the lowest bias, values near
+the largest, probabilities far below a row's maximum, padding documents, far positions, workspaces.
+
+Tolerances as in test_gpu_ops16: half a step for each rounding (probabilities, result) and n 2^-22 for sums of
+n terms, here with the size of a score taken over the keys whose weight is not 0."""
+import math
+
+import pytest
+
+from test_gpu_ops16 import BF16, F16, F32, U22, half_step, qkv, within
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    yield torch.device("cuda:0")
+    from edge_maskgit_b200 import runtime as rt
+    torch.cuda.synchronize()
+    assert rt.device_error() == 0
+
+
+def scores_ref(q, k, v, bias, seen, scale=None):
+    """(out, tolerance) in 64 bits of softmax(scale q.k + bias) v over the seen keys; bias and seen [Hq][Sq][Sk], equal heads."""
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    Sk, fin = k.shape[1], torch.finfo(q.dtype)
+    qq, kk, vv = (t[0].double().transpose(0, 1) for t in (q, k, v))
+    s = torch.where(seen, qq @ kk.mT * scale + bias, -math.inf)
+    m = s.amax(-1, keepdim=True)
+    w = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
+    w = w / torch.where(m == -math.inf, 1.0, w.sum(-1, keepdim=True))
+    out, mag = w @ vv, w @ vv.abs()
+    err = (q.shape[-1] + 4) * U22 * (qq.abs() @ kk.abs().mT) * abs(scale) + 4 * U22 * s.abs()
+    # (a score that its bias absorbs is the bias itself, here and in 32 bits: no error)
+    e_s = torch.where((w > 0) & (s != bias), err, 0.0).amax(-1, keepdim=True) + 8 * U22
+    tol = (half_step(q.dtype) + 2 * e_s + (Sk + 8) * U22) * mag
+    tol = tol + half_step(q.dtype) * (out.abs() + tol) + fin.smallest_normal * fin.eps
+    return out.transpose(0, 1)[None], tol.transpose(0, 1)[None]
+
+
+# ---------------------------------------------------------------------------- lowest biases
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,Sk,reach", [(1, 300, 40), (40, 300, 40), (700, 700, 100), (1300, 1300, 300), (300, 2000, 1)])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_attention_lowest_bias_everywhere(dt, D, Sq, Sk, reach, slopes):
+    """Every score is absorbed by the lowest bias: a uniform row, however large the scores are, in tiles whose
+    distances lie inside the table and in those beyond it."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 2, 2, D, dt)
+    table = torch.full((2, 2 * reach + 1), torch.finfo(F32).min, device="cuda")
+    for causal in (False, True):
+        seen = torch.ones(Sq, Sk, dtype=torch.bool, device="cuda")
+        if causal:
+            seen = seen.tril(Sk - Sq)
+        y = rt.attention(q, k, v, scale=4.0, dist_bias=table, causal=causal,
+                         slopes=torch.tensor([0.01, 0.0], device="cuda") if slopes else None)
+        within(y, *scores_ref(q, k, v, torch.finfo(F32).min, seen, scale=4.0))
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,Sk", [(1, 300), (40, 300), (700, 700), (1300, 1300)])
+def test_attention_lowest_bias_as_a_window(dt, D, Sq, Sk):
+    """The lowest value outside a window of distances: it hides a key wherever another is inside."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 2, 2, D, dt)
+    reach = 300
+    table = torch.full((2, 2 * reach + 1), torch.finfo(F32).min, device="cuda")
+    table[0, reach - 20:reach + 1] = 0.5
+    table[1, reach + 250:] = -0.5   # far keys only: rows near the end see lowest biases alone
+    j, p = torch.arange(Sk, device="cuda")[None], Sk - Sq + torch.arange(Sq, device="cuda")[:, None]
+    bias = table.double()[:, (j - p).clamp(-reach, reach) + reach]
+    y = rt.attention(q, k, v, scale=3.0, dist_bias=table)
+    within(y, *scores_ref(q, k, v, bias, torch.ones_like(bias, dtype=torch.bool), scale=3.0))
