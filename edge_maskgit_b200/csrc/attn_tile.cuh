@@ -47,9 +47,11 @@ struct TileCall {
     int kmul[3], vmul[3], qmul[3];   // 0 where a stride is 0 (batch, -, head): the map has one entry there
 };
 
-// Where a tile's bias is linear in the key, its part that all keys share joins the base: exponents are then
-// s c1 + (bias - base), and the scores must not be lost in the rounding of bias or base.  Up to this size
-// of the bias (in base 2) that rounding is below 2^-3; larger ones are added to each score.
+// A tile whose bias is linear in the key (or that has none) forms its exponents in one step, s c1 + (bias - base),
+// with one rounding at the end, while base and bias were rounded on their own.  Up to this size of the bias
+// and of the row's maximum (in base 2) those roundings are below 2^-3.  Beyond it a lowest bias would
+// lose the scores, and a maximum of 2^27 could lie 16 above its own base, past f16's largest value: such a
+// tile forms t = s c1 + bias of each key first, and t minus the base is exact where it matters.
 constexpr float LINEAR_MAX = 1048576.0f;
 
 // What the softmax of one row needs of one key tile.
@@ -623,6 +625,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 }
                 float mx = max3_nan(max3_nan(hi[0], hi[1], hi[2]), hi[3], hi[3]);
                 if (raw && !(MODE & SLOPE) && mx != -INFINITY) mx = fmaf(mx, x.c1, x.lin_a);
+                if (!(MODE & CAP) && raw && __any_sync(0xffffffffu, fabsf(mx) > LINEAR_MAX && mx != -INFINITY)) {
+                    raw = false;   // scores of that size round like their maximum
+#pragma unroll
+                    for (int j = 0; j < 128; j++)
+                        s[j] = __float_as_uint(fmaf(__uint_as_float(s[j]), x.c1, fmaf((float)j, x.lin_b, x.lin_a)));
+                }
                 if (MODE == CAP) {
                     const float low = fminf(fminf(lo_s[0], lo_s[1]), fminf(lo_s[2], lo_s[3]));
                     raw = !masked && __all_sync(0xffffffffu, fmaxf(mx, -low) * fabsf(x.c1) <= CAP_RAW && mx == mx);
@@ -691,8 +699,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     probs([&](uint64_t t, int j) {
                         return fma2(t, c2, pack2(fmaf((float)j, x.lin_b, la), fmaf((float)(j + 1), x.lin_b, la)));
                     });
-                } else if (MODE == 0) {
-                    probs([&](uint64_t t, int) { return fma2(t, c2, nb2); });
                 } else {   // raw scores, or t already: one form
                     const float k = raw ? x.c1 : 1.0f, off = (raw ? x.lin_a : 0.0f) - base;
                     const uint64_t k2 = pack2(k, k), off2 = pack2(off, off);

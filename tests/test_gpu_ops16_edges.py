@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_gpu_ops16 import BF16, F16, F32, U22, half_step, qkv, within
+from test_gpu_ops16 import BF16, F16, F32, U22, half_step, qkv, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,29 @@ def test_attention_lowest_bias_as_a_window(dt, D, Sq, Sk):
     bias = table.double()[:, (j - p).clamp(-reach, reach) + reach]
     y = rt.attention(q, k, v, scale=3.0, dist_bias=table)
     within(y, *scores_ref(q, k, v, bias, torch.ones_like(bias, dtype=torch.bool), scale=3.0))
+
+
+# -------------------------------------------------------------------------------- large scores
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 200, 64), (40, 200, 64), (200, 200, 64), (2000, 200, 64), (2000, 200, 128), (400, 250, 128)])
+@pytest.mark.parametrize("scale", [2.0 ** 10, -2.0 ** 16, 2.0 ** 21, 2.0 ** 28, 2.0 ** 60])
+@pytest.mark.parametrize("shape", ["plain", "causal", "table", "slopes"])
+def test_attention_very_large_scores(dt, Sq, Sk, D, scale, shape):
+    """Scores that differ by 2^10 and more: each row is the value of its largest seen score."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 4, 4, D, dt)
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    order = torch.randperm(Sk, generator=torch.Generator().manual_seed(7)).cuda()
+    q[..., 0], k[..., 0] = 1.0, (order - Sk // 3).to(dt)[None, :, None]   # whole numbers below 256: exact in bf16
+    kw = {"causal": dict(causal=True), "table": dict(dist_bias=randn(4, 41, dtype=F32, seed=5)),
+          "slopes": dict(slopes=torch.tensor([0.5, 0.1, 0.01, 0.0], device="cuda"))}.get(shape, {})
+    s = (order - Sk // 3).double() * scale
+    p = Sk - Sq + torch.arange(Sq, device="cuda")[:, None]
+    seen = torch.arange(Sk, device="cuda")[None] <= p if shape == "causal" else torch.ones(Sq, Sk, dtype=torch.bool, device="cuda")
+    best = torch.where(seen, s, -math.inf).argmax(1)
+    want = torch.where(seen.any(1)[:, None, None], v[0, best], 0.0)
+    y = rt.attention(q, k, v, scale=scale, **kw)
+    # two roundings: the one probability p of the row, relative to the sum's unrounded p, and the result:
+    # (1 + eps / 2)^2 - 1, and the sums' few 2^-22
+    h = half_step(dt)
+    within(y, want.double()[None], (2 * h + h * h + 8 * U22) * want.double().abs()[None])
