@@ -75,10 +75,15 @@ __device__ __forceinline__ RowBounds row_bounds(const mgc_attention_args& a, int
 // length, and causally at most p or inside the prefix (not causal: prefix = Sk).
 __device__ __forceinline__ int key_end(const RowBounds& r, int p) { return min(r.len, max(p + 1, r.prefix)); }
 
+// A result that the row may not have: NaN, or in bf16 an infinity (values up to 2^127 can pass the
+// largest float in a sum of unnormalised products; f16's cannot).
+template <bool BF16>
+__device__ __forceinline__ bool suspect(float x) { return BF16 ? !isfinite(x) : isnan(x); }
 // One row, exactly as the formulas have it, touching seen keys only, by one warp; o = this lane's
 // dims d = lane + 32 u.  The kernels multiply a whole tile of v by probabilities that are 0 at
-// unseen keys; a NaN or infinity that v holds there turns the row into NaN.  A row whose result is
-// NaN is therefore recomputed here: it stays NaN if a seen key made it so.
+// unseen keys; a NaN or infinity that v holds there turns the row into NaN.  A row with a suspect
+// result is therefore recomputed here: it stays NaN or infinite if a seen key made it so.  o is the
+// average so far, not a sum, so it never exceeds the largest value.
 template <bool BF16>
 __device__ __noinline__ void exact_row(const mgc_attention_args& a, int g, int b, int h, int i, float (&o)[4]) {
     const int lane = threadIdx.x & 31;
@@ -106,19 +111,21 @@ __device__ __noinline__ void exact_row(const mgc_attention_args& a, int g, int b
         const unsigned seen = __ballot_sync(0xffffffffu, !(t == -INFINITY));
         float ls = pj;
         for (int k = 16; k; k >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, k);
-        l = l * alpha + ls;
-        for (int u = 0; u < 4; u++) o[u] *= alpha;
+        const float before = l * alpha;
+        l = before + ls;
         m = mn;
+        if (l == 0.0f) continue;   // nothing seen yet
+        const float inv = 1.0f / l;
+        for (int u = 0; u < 4; u++) o[u] *= before * inv;
         for (int k = 0; k < 32; k++) {
             if (!(seen >> k & 1)) continue;
-            const float pk = __shfl_sync(0xffffffffu, pj, k);
+            const float pk = __shfl_sync(0xffffffffu, pj, k) * inv;
             for (int u = 0; u < 4; u++) {
                 const int d = lane + 32 * u;
                 if (d < a.D) o[u] = fmaf(pk, load16<BF16>(a.v, vo + (j0 + k) * a.v_stride[1] + d), o[u]);
             }
         }
     }
-    for (int u = 0; u < 4; u++) o[u] = l == 0.0f ? 0.0f : o[u] / l;
 }
 
 // Launches of the two kernels; the caller has checked the arguments.

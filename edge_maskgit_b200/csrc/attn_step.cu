@@ -55,13 +55,13 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(copy ? 16 : 0) : "memory");
 }
 
-// Writes one finished row (o = dims lane + 32 u), repairing a NaN.
+// Writes one finished row (o = dims lane + 32 u), repairing a suspect one.
 template <bool BF16>
 __device__ __forceinline__ void write_row(const AttnCall& c, int b, int h, int i, float (&o)[4]) {
     const int lane = threadIdx.x & 31;
     bool bad = false;
 #pragma unroll
-    for (int u = 0; u < 4; u++) bad |= lane + 32 * u < c.a.D && isnan(o[u]);
+    for (int u = 0; u < 4; u++) bad |= lane + 32 * u < c.a.D && suspect<BF16>(o[u]);
     if (__any_sync(0xffffffffu, bad)) exact_row<BF16>(c.a, c.g, b, h, i, o);
     const long long at = b * c.a.out_stride[0] + i * c.a.out_stride[1] + h * c.a.out_stride[2];
 #pragma unroll
@@ -74,7 +74,7 @@ template <bool BF16>
 __device__ __forceinline__ void write_row4(const AttnCall& c, int b, int h, int i, float4 o, float l) {
     const int lane = threadIdx.x & 31;
     const bool dims = lane * 4 < c.a.D;
-    if (__any_sync(0xffffffffu, dims && (isnan(o.x) || isnan(o.y) || isnan(o.z) || isnan(o.w) || isnan(l)))) {
+    if (__any_sync(0xffffffffu, dims && (suspect<BF16>(o.x) || suspect<BF16>(o.y) || suspect<BF16>(o.z) || suspect<BF16>(o.w) || isnan(l)))) {
         float nan[4] = {NAN, NAN, NAN, NAN};
         write_row<BF16>(c, b, h, i, nan);
         return;

@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
                     const float v = any ? __uint_as_float(o[e]) : 0.0f;
-                    bad |= d + e < a.D && isnan(v);
+                    bad |= d + e < a.D && suspect<BF16>(v);
                     o[e] = __float_as_uint(c.nsplit > 1 ? v : v * inv);
                 }
 #pragma unroll
@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 }
                 __syncwarp();
             }
-            bad = (bad || isnan(l)) && live && c.nsplit == 1;   // (split: the join looks for NaN)
+            bad = (bad || isnan(l)) && live && c.nsplit == 1;   // (split: the join looks for it)
             unsigned todo = __ballot_sync(0xffffffffu, bad);
             while (todo) {
                 const int k = __ffs(todo) - 1;

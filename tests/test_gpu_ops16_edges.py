@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_gpu_ops16 import BF16, F16, F32, U22, half_step, qkv, randn, within
+from test_gpu_ops16 import BF16, F16, F32, U22, attention_ref, half_step, qkv, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -77,6 +77,23 @@ def test_attention_lowest_bias_as_a_window(dt, D, Sq, Sk):
     bias = table.double()[:, (j - p).clamp(-reach, reach) + reach]
     y = rt.attention(q, k, v, scale=3.0, dist_bias=table)
     within(y, *scores_ref(q, k, v, bias, torch.ones_like(bias, dtype=torch.bool), scale=3.0))
+
+
+# --------------------------------------------------------------------- values near the largest
+@pytest.mark.parametrize("Sq,Sk", [(1, 5), (1, 300), (1, 9000), (3, 700), (40, 300), (300, 300), (700, 3000), (64, 9000)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_values_near_the_largest(Sq, Sk, D, causal):
+    """Averages of values up to 2^127.9 are finite, also where their sum is not."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 4, 2, D, BF16)
+    unit = 1.0 + v.float().abs().clamp(max=2.9) * 0.33   # 1 .. 1.957
+    sign = torch.ones(2, device="cuda")
+    sign[1] = -1.0
+    small = (unit * sign[None, None, :, None]).to(BF16)
+    ref, tol = attention_ref(q, k, small, causal=causal, scale=0.5)
+    y = rt.attention(q, k, (small.float() * 2.0 ** 127).to(BF16), causal=causal, scale=0.5)
+    within(y.double() * 2.0 ** -127, ref, tol)
 
 
 # -------------------------------------------------------------------------------- large scores
