@@ -88,6 +88,10 @@ __device__ __forceinline__ void write_row4(const AttnCall& c, int b, int h, int 
 template <bool BF16, int DP, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_constant__ AttnCall c) {
     constexpr int RB = row_bytes<DP>(), SB = stage_bytes<DP>(), NK = DP / 16, CH = DP / 8;
+    // Probabilities are 2^(t - base), with the base LIFT below the row's maximum.  In f16 they then go up to
+    // 2^15, and those that are 2^-29 of the largest still have all their bits (a sum of many small ones behind
+    // one large is right); bf16 needs no lift.  m below is this base.
+    constexpr int LIFT = BF16 ? 0 : 15;
     extern __shared__ __align__(16) uint8_t smem[];
     griddep_wait();
     griddep_launch();
@@ -207,7 +211,8 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
         for (int u = 0; u < 2; u++) {
             mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
             mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
-            const float mn = fmaxf(m[u], mx[u]);
+            // (rounded up: p never passes 2^LIFT)
+            const float mn = fmaxf(m[u], LIFT ? __fadd_ru(mx[u], -(float)LIFT) : mx[u]);
             base[u] = mn == -INFINITY ? 0.0f : mn;   // nothing seen yet: p = 2^-inf = 0
             alpha[u] = ex2_approx(m[u] - base[u]);
             m[u] = mn;

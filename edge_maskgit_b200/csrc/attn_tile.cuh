@@ -461,8 +461,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         // whose probability is then a power of two and rounds to itself, and again only when a score
         // passes it by SLACK: the sum and the output so far are then scaled, in f32.  So no pass over the
         // tile has to find its maximum first.  In f16 probabilities go up to 2^15, which it holds, and its
-        // smallest normal number is 2^-17 of the row's maximum; bf16 has room for more.
-        constexpr float SHIFT = 3.0f, SLACK = BF16 ? 40.0f : 15.0f;
+        // smallest normal number is 2^-25 of the row's maximum or less (a sum of many small ones behind one
+        // large is right); bf16 has room for more.  (base is rounded up: no score lies more than SHIFT above it.)
+        constexpr float SHIFT = BF16 ? 3.0f : 11.0f, SLACK = BF16 ? 40.0f : 15.0f;
 
         // bias window and documents of key tile kt: fetched a tile ahead
         float pre_b[2] = {0.0f, 0.0f};
@@ -656,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 if (move) {
                     float alpha = 1.0f;
                     if (set) {
-                        const float nb = mx - SHIFT;
+                        const float nb = __fadd_ru(mx, -SHIFT);
                         if (!fresh) alpha = ex2_approx(base - nb);
                         l *= alpha;
                         base = nb;

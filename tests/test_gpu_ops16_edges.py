@@ -96,6 +96,23 @@ def test_attention_values_near_the_largest(Sq, Sk, D, causal):
     within(y.double() * 2.0 ** -127, ref, tol)
 
 
+# ------------------------------------------------------------- probabilities far below the maximum
+@pytest.mark.parametrize("Sq,Sk", [(1, 300), (1, 3000), (1, 16385), (40, 300), (40, 16385), (300, 5000)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("gap", [13.0, 14.0, 15.0, 16.0, 17.0])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+def test_attention_many_keys_far_below_one(Sq, Sk, D, gap, where):
+    """One key takes the row's weight and has a value of 0: what is left is the many keys 13 to 17 below it."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 2, 2, D, F16)
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    v = v.abs() + 0.5
+    at = {"first": 0, "middle": Sk // 2, "last": Sk - 1}[where]
+    q[..., 0], k[:, at, :, 0], v[:, at] = 1.0, gap, 0.0
+    ref, tol = attention_ref(q, k, v, scale=1.0)
+    within(rt.attention(q, k, v, scale=1.0), ref, tol)
+
+
 # -------------------------------------------------------------------------------- large scores
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("Sq,Sk,D", [(1, 200, 64), (40, 200, 64), (200, 200, 64), (2000, 200, 64), (2000, 200, 128), (400, 250, 128)])
