@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
 #pragma unroll
                 for (int u = 0; u < 2; u++) pre_b[u] = __ldg(sh.table + max(-sh.range, min(sh.range, d0 + r + 128 * u)));
             }
-            if (a.doc_k) {   // (keys past the length get a number that no query has)
-                pre_d = kt * KT + r < rb.len ? __ldg(a.doc_k + (long long)b * a.Sk + kt * KT + r) : -1;
+            if (a.doc_k) {   // (padding, and keys past the length, get one number, and a padding query another)
+                pre_d = kt * KT + r < rb.len ? max(-1, __ldg(a.doc_k + (long long)b * a.Sk + kt * KT + r)) : -1;
                 pre_r = __ldg(tc.doc_range + (long long)b * nkt + kt);
             }
         };

@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_gpu_ops16 import BF16, F16, F32, U22, attention_ref, half_step, qkv, randn, within
+from test_gpu_ops16 import BF16, F16, F32, U22, attention_ref, half_step, ints, qkv, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -111,6 +111,19 @@ def test_attention_many_keys_far_below_one(Sq, Sk, D, gap, where):
     q[..., 0], k[:, at, :, 0], v[:, at] = 1.0, gap, 0.0
     ref, tol = attention_ref(q, k, v, scale=1.0)
     within(rt.attention(q, k, v, scale=1.0), ref, tol)
+
+
+# ------------------------------------------------------------------------------- documents
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 300, 64), (40, 300, 64), (900, 900, 64), (900, 900, 128), (600, 1500, 48)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_padding_of_any_negative_number(Sq, Sk, D, causal):
+    """A query with a negative document number sees nothing, whatever negative numbers the keys have."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(2, Sq, Sk, 2, 2, D, F16)
+    dq, dk = ints(-4, 3, 2, Sq, seed=100), ints(-4, 3, 2, Sk, seed=101)
+    y = rt.attention(q, k, v, doc_q=dq, doc_k=dk, causal=causal)
+    assert not y[dq < 0].any()
+    within(y, *attention_ref(q, k, v, doc_q=dq, doc_k=dk, causal=causal))
 
 
 # -------------------------------------------------------------------------------- large scores
