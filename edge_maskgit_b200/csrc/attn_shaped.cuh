@@ -55,9 +55,9 @@ __device__ __forceinline__ float capped(float s, float c1, float cap2) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return fmaf(-2.0f * cap2, r, cap2);
 }
-__device__ __forceinline__ float shaped(float s, const ScoreShape& f, int dist) {
+__device__ __forceinline__ float shaped(float s, const ScoreShape& f, int dist, int slope_dist) {
     float t = f.cap2 > 0.0f ? capped(s, f.c1, f.cap2) : s * f.c1;
-    t = fmaf(-f.slope2, fabsf((float)dist), t);
+    t = fmaf(-f.slope2, fabsf((float)slope_dist), t);
     if (f.table) t += bias2(__ldg(f.table + max(-f.range, min(f.range, dist))));
     return t;
 }
@@ -75,6 +75,11 @@ __device__ __forceinline__ RowBounds row_bounds(const mgc_attention_args& a, int
 // length, and causally at most p or inside the prefix (not causal: prefix = Sk).
 __device__ __forceinline__ int key_end(const RowBounds& r, int p) { return min(r.len, max(p + 1, r.prefix)); }
 
+// The position that slopes count distances from.  A query before the first or behind the last key has the same
+// -slope |p - nearest key| in all its scores, which the softmax does not see: counted from the nearest key,
+// the distances that differ keep their bits, however far the query is.
+__device__ __forceinline__ int slope_pos(const RowBounds& r, int p) { return max(0, min(p, r.len - 1)); }
+
 // A result that the row may not have: NaN, or in bf16 an infinity (values up to 2^127 can pass the
 // largest float in a sum of unnormalised products; f16's cannot).
 template <bool BF16>
@@ -89,7 +94,7 @@ __device__ __noinline__ void exact_row(const mgc_attention_args& a, int g, int b
     const int lane = threadIdx.x & 31;
     const RowBounds rb = row_bounds(a, b);
     const ScoreShape sh = score_shape(a, h);
-    const int p = rb.pos0 + i, end = key_end(rb, p);
+    const int p = rb.pos0 + i, ps = slope_pos(rb, p), end = key_end(rb, p);
     const long long hk = h / g;
     const long long qo = b * a.q_stride[0] + i * a.q_stride[1] + h * a.q_stride[2];
     const long long ko = b * a.k_stride[0] + hk * a.k_stride[2], vo = b * a.v_stride[0] + hk * a.v_stride[2];
@@ -102,7 +107,7 @@ __device__ __noinline__ void exact_row(const mgc_attention_args& a, int g, int b
         if (j < end && (!a.doc_q || (doc >= 0 && __ldg(a.doc_k + (long long)b * a.Sk + j) == doc))) {
             float s = 0.0f;
             for (int d = 0; d < a.D; d++) s = fmaf(load16<BF16>(a.q, qo + d), load16<BF16>(a.k, ko + j * a.k_stride[1] + d), s);
-            t = shaped(s, sh, j - p);
+            t = shaped(s, sh, j - p, j - ps);
         }
         float mx = t;   // NaN scores reach l through ex2
         for (int k = 16; k; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));

@@ -192,7 +192,10 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
         };
         if (a.cap > 0.0f) each([&](float& x, int, int) { x = capped(x, s0.c1, s0.cap2); });
         else each([&](float& x, int, int) { x *= s0.c1; });
-        if (a.slopes) each([&](float& x, int u, int j) { x = fmaf(u ? -s1.slope2 : -s0.slope2, fabsf((float)(j - pos[u])), x); });
+        if (a.slopes)
+            each([&](float& x, int u, int j) {
+                x = fmaf(u ? -s1.slope2 : -s0.slope2, fabsf((float)(j - slope_pos(rb, pos[u]))), x);
+            });
         if (a.dist_bias)
             each([&](float& x, int u, int j) {
                 x += bias2(__ldg((u ? s1.table : s0.table) + max(-s0.range, min(s0.range, j - pos[u]))));

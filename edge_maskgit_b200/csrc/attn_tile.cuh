@@ -59,7 +59,7 @@ struct RowTile {
     float c1;              // no cap: scale in base 2 (sign in `flip`); cap: scale / cap
     uint32_t flip;
     float cap2, slope2;
-    float d0;              // distance of the tile's key 0
+    float d0;              // distance of the tile's key 0, as slopes count it
     float lin_a, lin_b;    // the bias of key j where it is linear: lin_a + lin_b * j
     const float* win;      // bias of key j at win[j], 16-byte aligned
     int lim;               // keys below the row's end
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 if (a.doc_k) sdoc[buf * 128 + r] = pre_d;
                 named_bar_sync(bar_id, 128);
             }
-            x.d0 = (float)(kt * KT - p);
+            x.d0 = (float)(kt * KT - slope_pos(rb, p));
             x.lin_a = x.lin_b = 0.0f;
             bool linear = false;
             if (MODE & (SLOPE | TABLE)) {

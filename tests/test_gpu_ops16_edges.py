@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_gpu_ops16 import BF16, F16, F32, U22, attention_ref, half_step, ints, qkv, randn, within
+from test_gpu_ops16 import BF16, F16, F32, U22, attention_ref, half_step, i32, ints, qkv, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -124,6 +124,22 @@ def test_attention_padding_of_any_negative_number(Sq, Sk, D, causal):
     y = rt.attention(q, k, v, doc_q=dq, doc_k=dk, causal=causal)
     assert not y[dq < 0].any()
     within(y, *attention_ref(q, k, v, doc_q=dq, doc_k=dk, causal=causal))
+
+
+# ---------------------------------------------------------------------------- far positions
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 300, 64), (1, 9000, 128), (40, 300, 64), (700, 700, 64), (700, 700, 128)])
+@pytest.mark.parametrize("far", [10 ** 5, 10 ** 6, 2 ** 29 - 10 ** 4, -10 ** 6])
+def test_attention_slopes_of_far_positions(dt, Sq, Sk, D, far):
+    """Slopes fall off by distance, however far the first key is: a constant of the row takes no part."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 2, 2, D, dt)
+    slopes = torch.tensor([0.4, 0.01], device="cuda")
+    p = far + torch.arange(Sq, device="cuda")[:, None]
+    j = torch.arange(Sk, device="cuda")[None]
+    near = -slopes.double()[:, None, None] * ((p - j).abs() - (p - p.clamp(0, Sk - 1)).abs())   # less the row's constant
+    ref, tol = scores_ref(q, k, v, near, torch.ones_like(near, dtype=torch.bool))
+    within(rt.attention(q, k, v, slopes=slopes, q_pos=i32(far)), ref, tol)
 
 
 # -------------------------------------------------------------------------------- large scores
