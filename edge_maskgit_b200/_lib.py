@@ -58,6 +58,7 @@ _SIGS = {
     "mgc_linear": (I, [I, P, I64, P, I64, I, I, I, P, I, P, I64, P, I64, P]),
     "mgc_attention_workspace": (I, [P, P]),   # AttentionArgs (by reference, or packed bytes), uint64
     "mgc_attention": (I, [P, P]),
+    "mgc_selftest_attention_gives_up": (I, [P, P]),
     "mgc_logits_adjust": (I, [I, P, I64, I, I, P, I64, I, P, P, I64, P, I64, P, I64, P, I64, P]),
     "mgc_generate_with": (I, [P, I, P, P, I, F, C.POINTER(LogitControls), P]),
     "mgc_runtime_create": (I, [C.c_char_p, I, I, C.POINTER(P)]),

@@ -154,7 +154,7 @@ CUtensorMap operand_map(const void* p, bool bf16, int D, int S, int H, int B, co
     return make_map16(p, bf16, 4, dims, strides, box);
 }
 
-void run_tile(Plan& p, cudaStream_t st) {
+void run_tile(Plan& p, cudaStream_t st, bool gives_up = false) {
     const mgc_attention_args& a = p.c.a;
     const bool bf16 = a.dtype == MGC_BF16;
     if (a.doc_k) {
@@ -171,8 +171,19 @@ void run_tile(Plan& p, cudaStream_t st) {
     const CUtensorMap mq = operand_map(a.q, bf16, a.D, a.Sq, a.Hq, a.B, a.q_stride);
     const CUtensorMap mk = operand_map(a.k, bf16, a.D, a.Sk, a.Hkv, a.B, a.k_stride);
     const CUtensorMap mv = operand_map(a.v, bf16, a.D, a.Sk, a.Hkv, a.B, a.v_stride);
+    if (gives_up) return at::launch_tile_gives_up(mq, mk, mv, p.t, st);
     (bf16 ? (a.D <= 64 ? at::launch_tile_bf16_64 : at::launch_tile_bf16_128)
           : (a.D <= 64 ? at::launch_tile_f16_64 : at::launch_tile_f16_128))(mq, mk, mv, p.t, st);
+}
+
+void place_workspace(Plan& p) {
+    if (!p.bytes) return;
+    const mgc_attention_args& a = p.c.a;
+    if (!a.workspace || ((uintptr_t)a.workspace & 15) || a.workspace_bytes < p.bytes)
+        throw std::invalid_argument("workspace must be 16-byte aligned and hold mgc_attention_workspace() bytes");
+    uint8_t* ws = reinterpret_cast<uint8_t*>(a.workspace);
+    p.c.opart = reinterpret_cast<float*>(ws + p.doc_bytes);
+    p.c.mlpart = reinterpret_cast<float2*>(ws + p.doc_bytes + p.opart_bytes);
 }
 
 }  // namespace
@@ -195,17 +206,25 @@ int mgc_attention(const mgc_attention_args* args, void* stream) {
         Plan p = plan(*args);
         if (args->B == 0 || args->Sq == 0) return;
         check_pointers(*args);
-        if (p.bytes) {
-            if (!args->workspace || ((uintptr_t)args->workspace & 15) || args->workspace_bytes < p.bytes)
-                throw std::invalid_argument("workspace must be 16-byte aligned and hold mgc_attention_workspace() bytes");
-            uint8_t* ws = reinterpret_cast<uint8_t*>(args->workspace);
-            p.c.opart = reinterpret_cast<float*>(ws + p.doc_bytes);
-            p.c.mlpart = reinterpret_cast<float2*>(ws + p.doc_bytes + p.opart_bytes);
-        }
+        place_workspace(p);
         const cudaStream_t st = (cudaStream_t)stream;
         if (p.tile) run_tile(p, st);
         else launch_attn_step(p.c, st);
         if (p.c.nsplit > 1 && !p.c.cluster) launch_attn_combine(p.c, st);
+    });
+}
+
+int mgc_selftest_attention_gives_up(const mgc_attention_args* args, void* stream) {
+    return guarded("mgc_selftest_attention_gives_up", [&] {
+        if (!args) throw std::invalid_argument("args must not be NULL");
+        Plan p = plan(*args);
+        if (!p.tile || args->dtype != MGC_F16 || args->D > 64 || !args->dist_bias || args->cap != 0.0f || args->slopes)
+            throw std::invalid_argument("takes calls of the tile kernel in f16, heads of up to 64, a distance table only");
+        check_pointers(*args);
+        place_workspace(p);
+        run_tile(p, (cudaStream_t)stream, true);
+        const cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
+        if (e != cudaSuccess) throw std::runtime_error(cudaGetErrorString(e));
     });
 }
 

@@ -179,7 +179,8 @@ __device__ __forceinline__ void scale_o(uint32_t taddr, float f) {
     tmem_st32(taddr, v);
 }
 
-template <bool BF16, int DP, int MODE>
+// GIVE_UP: a self-test, in which one warp of each block acts as if its wait for a tile's second scores had run out.
+template <bool BF16, int DP, int MODE, bool GIVE_UP = false>
 __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_constant__ CUtensorMap mq,
                                                                const __grid_constant__ CUtensorMap mk,
                                                                const __grid_constant__ CUtensorMap mv,
@@ -202,8 +203,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     uint64_t* p_full = s_full + 2;         // [2] P is in TMEM (4 warps)
     uint64_t* o_full = p_full + 2;         // [2] a product with P is done
     uint64_t* s_free = o_full + 2;         // [2] S was read (4 warps; SEP)
-    uint64_t* p_half = s_free + 2;           // [2] the first half of P is in TMEM (4 warps)
-    uint32_t* tmem_slot = (uint32_t*)(p_half + 2);
+    uint64_t* p_half = s_free + 2;         // [2] the first half of P is in TMEM (4 warps)
+    uint64_t* drained = p_half + 2;        // every product is done
+    uint32_t* tmem_slot = (uint32_t*)(drained + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     int* range = (int*)(tmem_slot + 2);    // lo0, lo1, hi0, hi1, then a tile's lowest / highest document
 
@@ -282,6 +284,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         for (int i = 0; i < NST; i++) {
             mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1); mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
         }
+        mbar_init(drained, 1);
         *abort_flag = 0;
         mbar_fence_init();
         if (!a.doc_q) first_copies();   // under the rest of the set-up
@@ -331,21 +334,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     if (warp == 8) {
         // ---------------------------------------------------------------- copies
         if (lane == 0 && n > 0) {
-            bool ok = true;
-            int i = min(n, NST);   // (the first ring is under way)
+            int i = min(n, NST), ks = i, vs = i;   // (the first ring is under way); copies of K and V requested
             for (; i < n; i++) {
                 const int par = (i / NST - 1) & 1;
-                if (!(ok = mbar_wait(k_empty + i % NST, par, abort_flag, 51, tc.dev_error))) break;
+                if (!mbar_wait(k_empty + i % NST, par, abort_flag, 51, tc.dev_error)) break;
                 copy_k(i);
-                if (!(ok = mbar_wait(v_empty + i % NST, par, abort_flag, 52, tc.dev_error))) break;
+                ks++;
+                if (!mbar_wait(v_empty + i % NST, par, abort_flag, 52, tc.dev_error)) break;
                 copy_v(i);
+                vs++;
             }
-            if (!ok) {   // gave up: let the copies in flight land (tile i may have K only)
-                volatile int never = 0;
-                for (int w = 0; w < 2; w++) if (on[w]) mbar_wait(q_full + w, 0, &never, 53, tc.dev_error);
-                for (int t = max(0, i - NST); t <= i; t++) mbar_wait(k_full + t % NST, (t / NST) & 1, &never, 53, tc.dev_error);
-                for (int t = max(0, i - NST); t < i; t++) mbar_wait(v_full + t % NST, (t / NST) & 1, &never, 53, tc.dev_error);
-            }
+            // The block must not end with copies under way.  They have landed where all of them were used; after
+            // a wait that gave up, here or in another warp, some may not have been.
+            volatile int never = 0;
+            for (int w = 0; w < 2; w++) if (on[w]) mbar_wait(q_full + w, 0, &never, 53, tc.dev_error);
+            for (int t = max(0, ks - NST); t < ks; t++) mbar_wait(k_full + t % NST, (t / NST) & 1, &never, 53, tc.dev_error);
+            for (int t = max(0, vs - NST); t < vs; t++) mbar_wait(v_full + t % NST, (t / NST) & 1, &never, 53, tc.dev_error);
         }
     } else if (warp == 9) {
         // ---------------------------------------------------------------- products
@@ -427,6 +431,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 st = st1;
                 par = par1;
             }
+            if (lead) {   // the TMEM is freed behind the last product, also after a wait that gave up
+                volatile int never = 0;
+                mma_commit(drained);
+                mbar_wait(drained, 0, &never, 65, tc.dev_error);
+            }
             __syncwarp();
         }
     }
@@ -480,6 +489,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 pre_r = __ldg(tc.doc_range + (long long)b * nkt + kt);
             }
         };
+        // All of the tile's distances beyond the table's range on one side: one bias for all.  (Then they
+        // have one sign too, so the tile is linear and does not look at the window.  Capped scores
+        // do: for them the window is always filled.)  A bias that would absorb the scores, the type's
+        // lowest value say, has to be added to each of them: it takes the window.
+        auto is_flat = [&](int kt) {
+            const int dist_lo = kt * KT - (rb.pos0 + q0 + w * QT) - 127, dist_hi = dist_lo + 254;
+            return (MODE & TABLE) && !(MODE & CAP) && (dist_lo >= sh.range || dist_hi <= -sh.range) &&
+                   (fabsf(pre_b[0]) <= LINEAR_MAX || pre_b[0] == -INFINITY);
+        };
         float base = 0.0f, l = 0.0f;
         bool fresh = true, ok = true;   // fresh: the row has seen nothing yet, base is not set
         // (selected, not indexed by w: arrays would go to local memory)
@@ -493,13 +511,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         for (int next; it < n_w; i = next, it++) {
             const int kt = order(i), buf = it & 1;
             for (next = i + 1; next < n && !mine(next);) next++;
-            // All of the tile's distances beyond the table's range on one side: one bias for all.  (Then they
-            // have one sign too, so the tile is linear and does not look at the window.  Capped scores
-            // do: for them the window is always filled.)  A bias that would absorb the scores, the type's
-            // lowest value say, has to be added to each of them: it takes the window.
-            const int dist_lo = kt * KT - (rb.pos0 + q0 + w * QT) - 127, dist_hi = dist_lo + 254;
-            const bool flat = (MODE & TABLE) && !(MODE & CAP) && (dist_lo >= sh.range || dist_hi <= -sh.range) &&
-                              (fabsf(pre_b[0]) <= LINEAR_MAX || pre_b[0] == -INFINITY);
+            const bool flat = is_flat(kt);
             if (((MODE & TABLE) && !flat) || a.doc_k) {
                 if ((MODE & TABLE) && !flat) {   // four copies, each shifted by one entry: every row reads aligned vectors
 #pragma unroll
@@ -540,6 +552,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             if (((MODE & TABLE) || a.doc_k) && next < n) fetch(order(next));
 
             ok = __all_sync(0xffffffffu, mbar_wait(s_full + w, it & 1, abort_flag, 58, tc.dev_error));
+            if (GIVE_UP && it == 1 && warp == 1) {
+                if (lane == 0) {
+                    *abort_flag = 58;
+                    atomicExch(tc.dev_error, 58);
+                }
+                ok = false;
+            }
             if (!ok) break;
             tc_fence_after();
             // keys behind the row's length are not in the tensor maps' bounds: v may hold NaN there
@@ -716,6 +735,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + w);
         }
+        // A warp whose wait gave up still meets the tile's other warps at its remaining steps: one of them may
+        // see the scores that it waits for before it sees the flag, and nothing bounds the wait at a meeting.
+        if (!ok && ((MODE & TABLE) || a.doc_k)) {
+            auto meets = [&](int kt) {
+                if (a.doc_k) return true;
+                fetch(kt);
+                return !is_flat(kt);
+            };
+#pragma unroll 1
+            while (++it < n_w) {
+                for (i++; !mine(i);) i++;
+                if (meets(order(i))) named_bar_sync(bar_id, 128);
+            }
+        }
         // ---------------------------------------------------------------- output
         if (ok && n_w > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full + w, (n_w - 1) & 1, abort_flag, 60, tc.dev_error));
         tc_fence_after();
@@ -782,10 +815,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
     }
 }
 
-template <bool BF16, int DP, int MODE>
+template <bool BF16, int DP, int MODE, bool GIVE_UP = false>
 void launch_tile(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TileCall& t, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
-    auto kernel = attn_tile_kernel<BF16, DP, MODE>;
+    auto kernel = attn_tile_kernel<BF16, DP, MODE, GIVE_UP>;
     allow_smem(kernel, smem<DP>(), done);
     const long long grid = (long long)t.qblocks * t.c.a.B * t.c.a.Hq * t.c.nsplit;
     if (grid > 0x7fffffffLL) throw std::runtime_error("too many rows for one launch");
@@ -814,6 +847,7 @@ void launch_tile_f16_64(const CUtensorMap&, const CUtensorMap&, const CUtensorMa
 void launch_tile_f16_128(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);
 void launch_tile_bf16_64(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);
 void launch_tile_bf16_128(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);
+void launch_tile_gives_up(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const TileCall&, cudaStream_t);   // f16, up to 64, a table
 
 }  // namespace at
 }  // namespace mgc

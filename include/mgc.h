@@ -165,6 +165,11 @@ typedef struct mgc_attention_args {
 /* Bytes of workspace the call needs (0 = none); reads the sizes and which pointers are NULL. */
 int mgc_attention_workspace(const mgc_attention_args* args, uint64_t* bytes);
 int mgc_attention(const mgc_attention_args* args, void* stream);
+/* Self-test of what mgc_attention does when a bounded wait gives up (see mgc_selftest_wait_timeout): one
+ * warp of each block leaves at its second key tile, as if its wait had run out.  The call ends (it syncs
+ * `stream`), mgc_device_error() then returns 58, out is undefined and later calls run as ever.  Takes calls
+ * of 32 or more queries in f16 with D <= 64 and dist_bias, without cap and slopes. */
+int mgc_selftest_attention_gives_up(const mgc_attention_args* args, void* stream);
 
 /* Adjusts logits before a draw.  Row r of logits [R][V] (dtype MGC_F32, MGC_F16 or MGC_BF16):
  *   z = z > 0 ? z / rep : z * rep   and   z -= freq * c + pres   for a token that the row's history

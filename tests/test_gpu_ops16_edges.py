@@ -166,3 +166,32 @@ def test_attention_very_large_scores(dt, Sq, Sk, D, scale, shape):
     # (1 + eps / 2)^2 - 1, and the sums' few 2^-22
     h = half_step(dt)
     within(y, want.double()[None], (2 * h + h * h + 8 * U22) * want.double().abs()[None])
+
+
+# ------------------------------------------------------------------------- waits that give up
+@pytest.mark.parametrize("S,B,documents", [(700, 3, False), (700, 3, True), (1300, 1, False), (1300, 1, True)])
+def test_attention_ends_when_a_wait_gives_up(S, B, documents):
+    """One warp leaves at its second key tile as if its wait had run out: the others, which would meet it at the
+    next bias window, end too, the error is reported and later calls are right."""
+    import ctypes as C
+    from edge_maskgit_b200 import runtime as rt
+    from edge_maskgit_b200._lib import AttentionArgs, lib
+    q, k, v = qkv(B, S, S, 4, 4, 64, F16)
+    kw = dict(dist_bias=randn(4, 2 * 200 + 1, dtype=F32, seed=110))
+    if documents:
+        kw["doc_q"] = kw["doc_k"] = torch.arange(S, device="cuda", dtype=torch.int32).div(300, rounding_mode="floor").int().repeat(B, 1)
+    want = rt.attention(q, k, v, **kw)
+    out = torch.empty_like(q)
+    a = AttentionArgs(dtype=1, B=B, Sq=S, Sk=S, Hq=4, Hkv=4, D=64, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(),
+                      out=out.data_ptr(), scale=0.125, dist_range=200, **{n: t.data_ptr() for n, t in kw.items()})
+    a.q_stride[:] = a.k_stride[:] = a.v_stride[:] = a.out_stride[:] = q.stride()[:3]
+    need = C.c_uint64()
+    assert lib.mgc_attention_workspace(C.byref(a), C.byref(need)) == 0
+    ws = torch.empty(max(need.value, 16), dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+    torch.cuda.synchronize()
+    assert lib.mgc_selftest_attention_gives_up(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    assert rt.device_error() == 58
+    assert torch.equal(rt.attention(q, k, v, **kw), want)
+    torch.cuda.synchronize()
+    assert rt.device_error() == 0
