@@ -142,6 +142,56 @@ def test_attention_slopes_of_far_positions(dt, Sq, Sk, D, far):
     within(rt.attention(q, k, v, slopes=slopes, q_pos=i32(far)), ref, tol)
 
 
+# -------------------------------------------------------------------------------- workspaces
+def workspace(q, k, **kw):
+    """Bytes that a call of these shapes asks for."""
+    import ctypes as C
+    from edge_maskgit_b200._lib import AttentionArgs, lib
+    B, Sq, Hq, D = q.shape
+    a = AttentionArgs(dtype=1 if q.dtype == F16 else 30, B=B, Sq=Sq, Sk=k.shape[1], Hq=Hq, Hkv=k.shape[2], D=D, scale=1.0, **kw)
+    a.q_stride[:] = a.out_stride[:] = q.stride()[:3]
+    a.k_stride[:] = a.v_stride[:] = k.stride()[:3]
+    need = C.c_uint64()
+    assert lib.mgc_attention_workspace(C.byref(a), C.byref(need)) == 0
+    return need.value
+
+
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hkv,D", [(2, 1, 9000, 8, 2, 64), (1, 4, 20000, 4, 1, 128), (1, 128, 4000, 2, 2, 64),
+                                              (1, 200, 3000, 4, 2, 128)])
+def test_attention_workspaces_of_calls_that_overlap(B, Sq, Sk, Hq, Hkv, D):
+    """Partial results belong to their call: captured calls that are replayed at the same time do not share them."""
+    from edge_maskgit_b200 import runtime as rt
+    calls = []
+    for seed in (90, 95, 99):
+        q, k, v = qkv(B, Sq, Sk, Hq, Hkv, D, F16, seed=seed)
+        assert workspace(q, k) >= B * Sq * Hq * 2 * (4 * D + 8)   # two ranges of keys or more
+        want = rt.attention(q, k, v)
+        within(want, *attention_ref(q, k, v))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = rt.attention(q, k, v)
+        calls.append((g, out, want, (q, k, v)))
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (g, *_), s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for g, out, want, _ in calls:
+        assert torch.equal(out, want)
+    # the same without graphs, calls of one after another on three streams
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for _ in range(10):
+        for (_, _, want, qkv_), s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                outs.append((rt.attention(*qkv_), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y, want in outs)
+
+
 # -------------------------------------------------------------------------------- large scores
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("Sq,Sk,D", [(1, 200, 64), (40, 200, 64), (200, 200, 64), (2000, 200, 64), (2000, 200, 128), (400, 250, 128)])
