@@ -115,15 +115,16 @@ Plan plan(const mgc_attention_args& args) {
     } else {
         const long long heads = (long long)a.B * a.Hkv * ((rows + 15) / 16);
         // As many ranges of keys as run at once (two blocks an SM with large heads, three with small ones),
-        // of 128 keys at least.  Long ones of several rows are cut to 1024 keys (at most 32 ranges), so
-        // that rows of unequal length balance, unless there are several rounds of blocks anyway.  Up to
+        // of 128 keys at least.  Long ones of several rows are cut to 1024 keys, or to 32 ranges where those
+        // are longer, so that rows of unequal length balance, unless there are several rounds of blocks anyway.  Up to
         // 8 ranges are one cluster and join in one launch (4 rows x 4096 keys x 8 heads of 128: 17.5 us,
         // by a second kernel 20; clusters of 16 took 35).
         const long long slots = (long long)sms * (a.D > 64 ? 2 : 3);
         const long long n = std::max<long long>(1, slots / heads);
         auto up64 = [](long long x) { return (x + 63) / 64 * 64; };
         long long chunk = std::max<long long>(128, up64((a.Sk + n - 1) / n));
-        if (chunk > 2048 && a.B > 1 && heads < 4 * slots) chunk = std::max<long long>(1024, up64((a.Sk + 31) / 32));
+        if (chunk > 2048 && a.B > 1 && heads < 4 * slots)
+            chunk = std::min(chunk, std::max<long long>(1024, up64((a.Sk + 31) / 32)));
         if (a.Sk > chunk) {
             p.c.chunk = (int)chunk;
             p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);

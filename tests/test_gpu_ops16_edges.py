@@ -192,6 +192,18 @@ def test_attention_workspaces_of_calls_that_overlap(B, Sq, Sk, Hq, Hkv, D):
     assert all(torch.equal(y, want) for y, want in outs)
 
 
+# ------------------------------------------------------------------------------ long caches
+@pytest.mark.parametrize("B,Hkv,Sk", [(2, 1, 400000), (2, 2, 262144), (3, 1, 150000), (1, 1, 400000)])
+def test_attention_long_caches_of_few_heads_fill_the_gpu(B, Hkv, Sk):
+    """A long cache is cut into as many ranges of keys as there are multiprocessors, and more than 32 of them join."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(B, 1, Sk, 4 * Hkv, Hkv, 128, BF16)
+    ranges = workspace(q, k) // (B * 4 * Hkv * (4 * 128 + 8))
+    assert ranges * B * Hkv >= torch.cuda.get_device_properties(0).multi_processor_count
+    y = rt.attention(q, k, v, k_len=i32(*[Sk - 1000 * b for b in range(B)]))
+    within(y, *attention_ref(q, k, v, k_len=i32(*[Sk - 1000 * b for b in range(B)])))
+
+
 # -------------------------------------------------------------------------------- large scores
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("Sq,Sk,D", [(1, 200, 64), (40, 200, 64), (200, 200, 64), (2000, 200, 64), (2000, 200, 128), (400, 250, 128)])
