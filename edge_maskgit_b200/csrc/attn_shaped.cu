@@ -129,10 +129,16 @@ Plan plan(const mgc_attention_args& args) {
             p.c.chunk = (int)chunk;
             p.c.nsplit = (int)((a.Sk + chunk - 1) / chunk);
             p.c.cluster = p.c.nsplit <= 8;
-            // Few heads and not too many keys: a cluster of 8 blocks of eight warps, one launch (1 row x 4096
-            // keys x 8 heads of 128: 13.2 us a call; by a second kernel 15.2, although its GPU time is
-            // 9.7 against 11.3: the second launch and the workspace cost the host more).
-            if (p.c.nsplit > 8 && a.Sk <= 4096 && heads * 16 <= sms) {
+            // Few heads and not too many keys: a cluster of 8 blocks of eight warps, one launch and no workspace,
+            // which saves the host 3 to 5 us a call and costs the GPU up to 3 us.  Its GPU time is about
+            // 6.2 us + 7.3 ps * keys * (D + 32); it is taken where calls gain at least what graph replays lose.
+            // One row, 1 to 8 heads, call (GPU) in us, against two launches:
+            //   heads of 128: 1100 keys 9.9 (7.7) / 14.8 (6.9), 2000 10.3 (8.4) / 14.8 (7.0), 4096 12.6 (11.1) /
+            //   14.9 (8.3), 6000 16.4 (13.7) / 14.8 (11.2), 8192 18.6 (16.3) / 15.2 (11.6)
+            //   heads of 64: 2000 9.9 (6.8) / 14.8 (6.3), 4096 10.3 (8.4) / 14.8 (7.3), 6000 12.8 (10.0) / 14.9 (10.5),
+            //   8192 13.5 (11.5) / 14.9 (10.0)
+            // (16 heads, two rounds of such clusters: 2000 keys 14.5 (12.4) / 14.8 (7.2))
+            if (p.c.nsplit > 8 && (long long)a.Sk * (a.D + 32) <= 655360 && heads * 16 <= sms) {
                 p.c.chunk = (int)up64((a.Sk + 7) / 8);
                 p.c.nsplit = (a.Sk + p.c.chunk - 1) / p.c.chunk;
                 p.c.cluster = p.c.wide = 1;

@@ -257,3 +257,15 @@ def test_attention_ends_when_a_wait_gives_up(S, B, documents):
     assert torch.equal(rt.attention(q, k, v, **kw), want)
     torch.cuda.synchronize()
     assert rt.device_error() == 0
+
+
+# ------------------------------------------------------------------------ the rules' borders
+@pytest.mark.parametrize("B,Sk,Hq,Hkv,D", [(1, 4096, 8, 2, 128), (1, 4097, 8, 2, 128), (1, 6826, 4, 1, 64), (2, 6827, 4, 1, 64),
+                                           (1, 13653, 4, 4, 16), (1, 13654, 4, 4, 16), (1, 16384, 9, 9, 8), (1, 5000, 10, 10, 48)])
+@pytest.mark.parametrize("Sq", [1, 3])
+def test_attention_steps_on_both_sides_of_a_cluster(B, Sq, Sk, Hq, Hkv, D):
+    """Key ranges that join inside a cluster, and those that join through the workspace."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(B, Sq, Sk, Hq, Hkv, D, F16)
+    kw = dict(k_len=i32(*[Sk - 700 * b for b in range(B)]), causal=True)
+    within(rt.attention(q, k, v, **kw), *attention_ref(q, k, v, **kw))
