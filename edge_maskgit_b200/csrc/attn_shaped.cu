@@ -88,10 +88,13 @@ Plan plan(const mgc_attention_args& args) {
     const int rows = a.Sq * p.c.g, sms = current_sms();
     // A position stride of 0 (one key repeated) has no tensor map; the other kernel takes any.
     const bool maps = a.Sk > 0 && (a.Sq == 1 || a.q_stride[1] > 0) && (a.Sk == 1 || (a.k_stride[1] > 0 && a.v_stride[1] > 0));
-    // The other kernel also serves small problems (its set-up is a third of the tiles'): blocks of 16
-    // rows times keys, measured as the two take equal time: 1 x 257 x 16 heads of 48 (70 thousand) 8.0
-    // against 10.3 us, 4 x 257 (280 thousand) 19.0 / 19.6, 1 x 513 x 16 of 64 (271 thousand) 20.0 / 13.7;
-    // 1 x 128 x 32 heads of 128 over 8 (33 thousand) 7.7 / 7.9, 1 x 300 (180 thousand) 28.2 / 12.2.
+    // The other kernel also serves small problems (its set-up is a third of the tiles'): blocks of 16 rows times
+    // keys, about where the two take equal time in a graph.  Over 334 shapes (32 to 1000 queries, 40 to 4000
+    // keys, 1 to 16 rows, 4 to 32 heads of 48 to 128) the chosen ones take 2 % more in all than the better
+    // of the two each time: 1 x 257 x 16 heads of 48 (70 thousand) 8.0 against 10.3 us, 4 x 257 (280 thousand) 19.0 / 19.6, 1 x
+    // 513 x 16 of 64 (271 thousand) 20.0 / 13.7; 1 x 128 x 32 heads of 128 over 8 (33 thousand) 7.7 / 7.9, 1 x 300 (180
+    // thousand) 28.2 / 12.2.  It is furthest off for many short rows (16 x 128 x 8 of 64, 131 thousand: 14.6 / 7.4, the
+    // first is taken) and for 32 queries of many rows (16 x 32 x 2000 keys x 16 of 48: 40.6 / 60.2, the second is).
     const long long block_keys = (long long)a.B * a.Hkv * ((rows + 15) / 16) * a.Sk;
     p.tile = maps && a.Sq >= 32 && block_keys > (a.D <= 64 ? 160000 : 32000);
     if (p.tile) {
