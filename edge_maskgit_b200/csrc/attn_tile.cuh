@@ -71,7 +71,7 @@ struct RowTile {
 // 2.2e-6: scores well below their cap, the usual case, take four FP32 operations a pair.
 constexpr float CAP_RAW = 1.0f / 3.0f;
 
-// cap tanh(u) in base 2 for |u| <= 1: u (c0 + c1 u^2 + ...), fitted here to a relative error of 5.2e-7
+// cap tanh(u) in base 2 for |u| <= 1: u (c0 + c1 u^2 + ...), fitted here; as stored, relative error 6.9e-7
 // (times the cap: an error of that size in the exponent).  A score within the cap, the usual case,
 // then takes no MUFU operation; tanh from its definition would take two beside the one of 2^x.
 __device__ __forceinline__ uint64_t capped_poly(uint64_t u, uint64_t cap2) {

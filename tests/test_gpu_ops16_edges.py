@@ -204,6 +204,21 @@ def test_attention_long_caches_of_few_heads_fill_the_gpu(B, Hkv, Sk):
     within(y, *attention_ref(q, k, v, k_len=i32(*[Sk - 1000 * b for b in range(B)])))
 
 
+# ------------------------------------------------------------------------------------- GELU
+@pytest.mark.parametrize("M,N", [(1, 64), (300, 2025), (2048, 2304), (4100, 2025)])
+def test_linear_gelu_keeps_small_results(M, N):
+    """Sums from -13 to 0 that are exact: results down to 2^-123, relative to themselves.  The exponent of the
+    Gaussian, up to 122 in base 2, takes three roundings of 2^-24 (1.6e-5 of the result at most); the rest a few 1e-6."""
+    from edge_maskgit_b200 import runtime as rt
+    x, w = torch.zeros(M, 8, device="cuda", dtype=BF16), torch.zeros(N, 8, device="cuda", dtype=BF16)
+    w[:, 0] = -torch.linspace(0.0, 13.0, N, device="cuda").to(BF16)
+    x[:, 0] = 1.0
+    y = rt.linear(x, w, act=1)
+    s = w[:, 0].double().expand(M, N)
+    ref = s * 0.5 * torch.erfc(-s * math.sqrt(0.5))
+    within(y, ref, (half_step(BF16) + 2e-5) * ref.abs())
+
+
 # -------------------------------------------------------------------------------- large scores
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("Sq,Sk,D", [(1, 200, 64), (40, 200, 64), (200, 200, 64), (2000, 200, 64), (2000, 200, 128), (400, 250, 128)])
