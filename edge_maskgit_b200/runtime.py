@@ -167,12 +167,23 @@ assert _ATTN_PACK.size == C.sizeof(AttentionArgs)
 
 
 def _load_torch():
-    global _torch, _device, _raw_stream
+    global _torch, _device, _raw_stream, _forward_ad, _is_tracing
     import torch
+    import torch.autograd.forward_ad as _forward_ad
     _CODE.update({torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32})
-    _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _device, _raw_stream, _is_tracing = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch._C._is_tracing
     _torch = torch
     return torch
+
+
+def _only_values(**tensors):
+    """Refuses what would be lost: these operators read their arguments' memory, so a forward-mode
+    tangent does not pass through them, and a trace would hold an output that nothing fills."""
+    if _is_tracing():
+        raise MgcError("this operator cannot be recorded by torch.jit.trace")
+    for name, t in tensors.items():
+        if isinstance(t, _torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise MgcError(f"{name} carries a forward-mode tangent, which this operator does not pass on")
 
 
 def _code_of(t, name, f32: bool = False) -> int:
@@ -233,6 +244,8 @@ def linear(x, w, bias=None, act: int = 0, resid=None, out=None):
     [M][N], bias f32 [N]; act 0 none, 1 erf-GELU, 2 SiLU; summed in f32, rounded once.  Rows may be
     strided; K and the row strides of x and w are multiples of 8.  `out` may be `resid`."""
     code = _CODE.get(getattr(x, "dtype", None)) or _code_of(x, "x")
+    if _forward_ad._current_level >= 0 or _is_tracing():
+        _only_values(x=x, w=w, bias=bias, resid=resid, out=out)
     dt, index = x.dtype, x.get_device()
     if index < 0 or w.dtype is not dt or w.get_device() != index or x.requires_grad or w.requires_grad or \
             not (x.dim() == w.dim() == 2):
@@ -290,6 +303,8 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
     doc_k[b][j] >= 0 if given.  A query that sees no key gives zeros.  scale defaults to D ** -0.5;
     cap is 0 or from 2^-10 to 2^10; slopes f32 [Hq]; prefix, k_len, q_pos int32 [B]; doc_q, doc_k int32 [B][Sq], [B][Sk]."""
     code = _CODE.get(getattr(q, "dtype", None)) or _code_of(q, "q")
+    if _forward_ad._current_level >= 0 or _is_tracing():
+        _only_values(q=q, k=k, v=v, slopes=slopes, dist_bias=dist_bias, out=out)
     dt, index = q.dtype, q.get_device()
     if index < 0 or not (k.dtype is dt and v.dtype is dt and k.get_device() == index and v.get_device() == index) or \
             q.requires_grad or k.requires_grad or v.requires_grad or not (q.dim() == k.dim() == v.dim() == 4):
@@ -361,6 +376,8 @@ def logits_adjust(logits, history=None, hist_len=None, penalties=None, bias=None
     [R], penalties f32 [R][3] = (rep, freq, pres), bias f32 [R][V], allowed int32 [R][(V + 31) // 32].
     One-axis history, penalties, bias or allowed are shared by all rows.  `out` may be `logits`."""
     code = _code_of(logits, "logits", f32=True)
+    if _forward_ad._current_level >= 0 or _is_tracing():
+        _only_values(logits=logits, penalties=penalties, bias=bias, out=out)
     dt, index = logits.dtype, logits.get_device()
     ld = _matrix(logits, "logits", dt, index)
     R, V = logits.shape
