@@ -257,6 +257,8 @@ def linear(x, w, bias=None, act: int = 0, resid=None, out=None):
         raise MgcError("the last axes of x and w must be contiguous")
     if Kw != K:
         raise MgcError(f"x has {K} columns, w has {Kw}")
+    if (M | N | K) >> 31:   # (ctypes would keep the low 32 bits)
+        raise MgcError(f"linear: sizes must be below 2^31, not {[M, N, K]}")
     bias_p = _vector(bias, "bias", _torch.float32, index, (N,)) if bias is not None else None
     resid_p, ldr = None, 0
     if resid is not None:
@@ -355,7 +357,10 @@ def attention(q, k, v, scale: float | None = None, cap: float = 0.0, slopes=None
 
 
 def _attention(index, q, head):
-    args = _ATTN_PACK.pack(*head, 0, 0)
+    try:
+        args = _ATTN_PACK.pack(*head, 0, 0)
+    except (struct.error, OverflowError) as e:   # beyond what the call's struct holds
+        raise MgcError(f"attention: a size, scale or cap is out of range ({e})") from None
     need = C.c_uint64()
     rc = lib.mgc_attention_workspace(args, C.byref(need))
     if rc == 0:
@@ -418,6 +423,8 @@ def logits_adjust(logits, history=None, hist_len=None, penalties=None, bias=None
         bias_p, ld_b = table(bias, "bias", f32, V)
     if allowed is not None:
         allowed_p, ld_a = table(allowed, "allowed", i32, (V + 31) // 32)
+    if (R | V | L) >> 31:   # (ctypes would keep the low 32 bits)
+        raise MgcError(f"logits_adjust: sizes must be below 2^31, not {[R, V, L]}")
     if out is None:
         out, ld_o = logits.new_empty((R, V)), V
     else:

@@ -284,3 +284,25 @@ def test_attention_steps_on_both_sides_of_a_cluster(B, Sq, Sk, Hq, Hkv, D):
     q, k, v = qkv(B, Sq, Sk, Hq, Hkv, D, F16)
     kw = dict(k_len=i32(*[Sk - 700 * b for b in range(B)]), causal=True)
     within(rt.attention(q, k, v, **kw), *attention_ref(q, k, v, **kw))
+
+
+# --------------------------------------------------------------------------- beyond the types
+def test_python_forms_refuse_what_the_c_types_cannot_hold():
+    """Sizes of 2^31 and more (rows that repeat, so that they need no memory), constants beyond float32."""
+    from edge_maskgit_b200 import runtime as rt
+    many = 2 ** 32 + 1   # its low 32 bits are 1
+    x, w = randn(1, 64, dtype=F16, seed=1), randn(8, 64, dtype=F16, seed=2)
+    y = torch.zeros(1, 8, dtype=F16, device="cuda")
+    z = randn(1, 8, dtype=F32, seed=3)
+    h, pen = ints(0, 8, 1, seed=4), torch.ones(3, device="cuda")
+    q, k, v = qkv(1, 3, 5, 2, 2, 64, F16)
+    for bad in (lambda: rt.linear(x.expand(many, 64), w, out=y.expand(many, 8)),
+                lambda: rt.linear(x, w[:1].expand(many, 64), out=y[:, :1].expand(1, many)),
+                lambda: rt.logits_adjust(z.expand(many, 8), out=z.clone().expand(many, 8)),
+                lambda: rt.logits_adjust(z, history=h.expand(many), penalties=pen),
+                lambda: rt.attention(q, k[:, :1].expand(1, many, 2, 64), v[:, :1].expand(1, many, 2, 64)),
+                lambda: rt.attention(q, k, v, scale=1e300), lambda: rt.attention(q, k, v, scale=-1e39),
+                lambda: rt.attention(q, k, v, cap=1e39), lambda: rt.attention(q, k, v, scale=math.nan)):
+        with pytest.raises(rt.MgcError):
+            bad()
+    assert not y.any()
