@@ -512,6 +512,8 @@ extern "C" int mgc_linear(int dtype, const void* x, int64_t ldx, const void* w, 
         auto need = [](bool ok, const char* m) { if (!ok) throw std::invalid_argument(m); };
         need(dtype == MGC_F16 || dtype == MGC_BF16, "dtype must be F16 or BF16");
         need(M >= 0 && N >= 0, "negative size");
+        // (tiles and k steps are counted up to the next multiple of 256 and one more, in 32 bits)
+        need(M <= 0x7ffffc00 && N <= 0x7ffffc00 && K <= 0x7ffffc00, "M, N and K must be at most 2^31 - 1024");
         need(K > 0 && K % 8 == 0, "K must be a positive multiple of 8");
         need(act >= 0 && act <= 2, "act must be 0 (none), 1 (GELU) or 2 (SiLU)");
         if (M == 0 || N == 0) return;

@@ -117,7 +117,8 @@ int mgc_embed(const float* tok_embd_dev, int vocab, const float* pos_embd_dev, i
  * rounded once.  x [M][K], w [N][K], resid and y [M][N] are all `dtype` (MGC_F16 or MGC_BF16),
  * bias f32; bias / resid may be NULL; act 0 none, 1 erf-GELU, 2 SiLU.  ld* are row strides in
  * elements.  K, ldx and ldw must be multiples of 8, x and w 16-byte aligned; N, ldr and ldy may
- * be odd.  y may be the buffer of resid (same stride), not of x or w.  M = 0 or N = 0 is a no-op. */
+ * be odd.  y may be the buffer of resid (same stride), not of x or w.  M, N and K are at most
+ * 2^31 - 1024; M = 0 or N = 0 is a no-op. */
 int mgc_linear(int dtype, const void* x_dev, int64_t ldx, const void* w_dev, int64_t ldw, int M, int N, int K,
                const float* bias_dev, int act, const void* resid_dev, int64_t ldr, void* y_dev, int64_t ldy,
                void* stream);
