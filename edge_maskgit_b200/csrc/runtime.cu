@@ -952,6 +952,10 @@ struct ControlBuffers {
                 if (!(c->repetition > 0.0f) || !std::isfinite(c->repetition) || !std::isfinite(c->frequency) ||
                     !std::isfinite(c->presence))
                     throw Err("mgc_generate_with: repetition must be positive and all penalties finite");
+                // a logit that a penalty takes to infinity would leave a draw without probabilities
+                if (c->repetition < 0x1p-60f || c->repetition > 0x1p60f || std::fabs(c->frequency) > 0x1p60f ||
+                    std::fabs(c->presence) > 0x1p60f)
+                    throw Err("mgc_generate_with: repetition must be from 2^-60 to 2^60, frequency and presence at most 2^60");
                 const float p[3] = {c->repetition, c->frequency, c->presence};
                 pen = dupload(p, 3);
             }

@@ -242,8 +242,9 @@ int mgc_generate(mgc_runtime* rt, int B, const int32_t* class_ids, const uint64_
 /* mgc_generate with its logits adjusted (mgc_logits_adjust) before every draw (controls NULL: not
  * adjusted).  All host pointers. */
 typedef struct mgc_logit_controls {
-    float repetition, frequency, presence;   /* against the codes an image already holds; 1, 0, 0 = none */
-    const float* bias;                       /* [codebook] added to every position's logits, or NULL */
+    float repetition, frequency, presence;   /* against the codes an image already holds; 1, 0, 0 = none;
+                                                repetition from 2^-60 to 2^60, the others at most 2^60 */
+    const float* bias;                       /* [codebook], finite, added to every position's logits, or NULL */
     const uint32_t* allowed;                 /* [allowed_rows][(codebook + 31) / 32] bit masks, or NULL */
     int32_t allowed_rows;                    /* 1: one mask for every position; n_tokens: one each (a
                                                 region's own codes).  Each must allow a code. */
