@@ -944,7 +944,17 @@ struct ControlBuffers {
     int words = 0;
     bool per_position = false;
 
-    ControlBuffers(const mgc_logit_controls* c, int CB, int S) {
+    // On the runtime's own stream: a copy on another one may still be under way when its kernels run (the
+    // call returns once the host's bytes are staged).
+    template <class T>
+    static T* upload(const T* h, size_t n, cudaStream_t st) {
+        T* d = dalloc<T>(n);
+        const cudaError_t e = cudaMemcpyAsync(d, h, n * sizeof(T), cudaMemcpyHostToDevice, st);
+        if (e != cudaSuccess) { cudaFree(d); CK(e); }
+        return d;
+    }
+
+    ControlBuffers(const mgc_logit_controls* c, int CB, int S, cudaStream_t st) {
         if (!c) return;
         try {
             words = (CB + 31) / 32;
@@ -957,12 +967,12 @@ struct ControlBuffers {
                     std::fabs(c->presence) > 0x1p60f)
                     throw Err("mgc_generate_with: repetition must be from 2^-60 to 2^60, frequency and presence at most 2^60");
                 const float p[3] = {c->repetition, c->frequency, c->presence};
-                pen = dupload(p, 3);
+                pen = upload(p, 3, st);
             }
             if (c->bias) {
                 for (int v = 0; v < CB; v++)
                     if (!std::isfinite(c->bias[v])) throw Err("mgc_generate_with: bias must be finite (forbid codes with allowed)");
-                bias = dupload(c->bias, CB);
+                bias = upload(c->bias, CB, st);
             }
             if (c->allowed) {
                 if (c->allowed_rows != 1 && c->allowed_rows != S - 1)
@@ -980,7 +990,7 @@ struct ControlBuffers {
                     }
                     if (!any) throw Err("mgc_generate_with: a row of allowed allows no code");
                 }
-                allowed = dupload(m.data(), m.size());
+                allowed = upload(m.data(), m.size(), st);
             }
         } catch (...) { release(); throw; }
     }
@@ -1024,7 +1034,7 @@ static void generate_impl(mgc_runtime* rt, int B, const int32_t* class_ids, cons
         const size_t R = (size_t)B * S;
         CK(cudaSetDevice(rt->device));
         ensure_attn_scratch(rt, B, S);
-        ControlBuffers ctl(controls, CB, S);
+        ControlBuffers ctl(controls, CB, S, rt->st);
         for (int step = 0; step < steps; step++) {
             // forward on the device; the logits stay there (no read-back)
             std::memcpy(rt->h_tokens, tokens.data(), sizeof(int32_t) * R);
