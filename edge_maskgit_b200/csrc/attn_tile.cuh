@@ -489,14 +489,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 pre_r = __ldg(tc.doc_range + (long long)b * nkt + kt);
             }
         };
-        // All of the tile's distances beyond the table's range on one side: one bias for all.  (Then they
-        // have one sign too, so the tile is linear and does not look at the window.  Capped scores
-        // do: for them the window is always filled.)  A bias that would absorb the scores, the type's
-        // lowest value say, has to be added to each of them: it takes the window.
+        // All of the tile's distances beyond the table's range on one side: one bias for all, and the window is
+        // neither filled nor looked at, so the tile has to be linear for each of its rows: no caps, slopes that
+        // count from one side, and a bias that does not absorb the scores (the type's lowest value, say).
         auto is_flat = [&](int kt) {
             const int dist_lo = kt * KT - (rb.pos0 + q0 + w * QT) - 127, dist_hi = dist_lo + 254;
-            return (MODE & TABLE) && !(MODE & CAP) && (dist_lo >= sh.range || dist_hi <= -sh.range) &&
-                   (fabsf(pre_b[0]) <= LINEAR_MAX || pre_b[0] == -INFINITY);
+            bool flat = (MODE & TABLE) && !(MODE & CAP) && (dist_lo >= sh.range || dist_hi <= -sh.range) &&
+                        (fabsf(pre_b[0]) <= LINEAR_MAX || pre_b[0] == -INFINITY);
+            if ((MODE & SLOPE) && (MODE & TABLE) && flat) {
+                const int first = slope_pos(rb, rb.pos0 + q0 + w * QT), last = slope_pos(rb, rb.pos0 + min(q0 + w * QT + QT, a.Sq) - 1);
+                const int k0 = kt * KT, far = max(abs(k0 - first), abs(k0 - last)) + 127;
+                flat = (k0 >= last || k0 + 127 <= first) && fabsf(x.slope2) * (float)far <= LINEAR_MAX;
+            }
+            return flat;
         };
         float base = 0.0f, l = 0.0f;
         bool fresh = true, ok = true;   // fresh: the row has seen nothing yet, base is not set
@@ -530,10 +535,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
             x.lin_a = x.lin_b = 0.0f;
             bool linear = false;
             if (MODE & (SLOPE | TABLE)) {
-                linear = !(MODE & TABLE) || flat;
-                if (MODE & SLOPE)
-                    linear = linear && __all_sync(0xffffffffu, (x.d0 >= 0.0f || x.d0 <= -127.0f) &&
-                                                                   fabsf(x.slope2) * (fabsf(x.d0) + 127.0f) <= LINEAR_MAX);
+                linear = flat;
+                if (!(MODE & TABLE))
+                    linear = __all_sync(0xffffffffu, (x.d0 >= 0.0f || x.d0 <= -127.0f) &&
+                                                         fabsf(x.slope2) * (fabsf(x.d0) + 127.0f) <= LINEAR_MAX);
                 x.lin_b = x.d0 >= 0.0f ? -x.slope2 : x.slope2;
                 x.lin_a = ((MODE & SLOPE) ? x.lin_b * x.d0 : 0.0f) + (flat ? bias2(pre_b[0]) : 0.0f);
             }

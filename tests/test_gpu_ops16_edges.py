@@ -306,3 +306,26 @@ def test_python_forms_refuse_what_the_c_types_cannot_hold():
         with pytest.raises(rt.MgcError):
             bad()
     assert not y.any()
+
+
+# -------------------------------------------------------------------------- slopes with a table
+@pytest.mark.parametrize("dt,D", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("S,k_len,pos", [(40, 40, 0), (462, 462, 0), (462, 300, 100), (700, 500, 400), (922, 922, -300), (922, 600, 10 ** 5),
+                                         (922, 130, 5000), (1300, 1290, -10 ** 4)])
+@pytest.mark.parametrize("reach", [0, 1, 5, 40, 300])
+@pytest.mark.parametrize("slope", [0.3, 30.0, 3e5])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_slopes_with_a_table(dt, D, S, k_len, pos, reach, slope, causal):
+    """Both biases by distance, where the table's counts from the query and the slopes' from the nearest key."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, S, S, 2, 2, D, dt)
+    table = randn(2, 2 * reach + 1, dtype=F32, seed=120)
+    slopes = torch.tensor([slope, slope / 64], device="cuda")
+    p, j = pos + torch.arange(S, device="cuda")[:, None], torch.arange(S, device="cuda")[None]
+    bias = table.double()[:, (j - p).clamp(-reach, reach) + reach]
+    bias = bias - slopes.double()[:, None, None] * ((p - j).abs() - (p - p.clamp(0, k_len - 1)).abs())
+    seen = (j < k_len).expand(S, S)
+    if causal:
+        seen = seen & (j <= p)
+    y = rt.attention(q, k, v, slopes=slopes, dist_bias=table, k_len=i32(k_len), q_pos=i32(pos), causal=causal)
+    within(y, *scores_ref(q, k, v, bias, seen.expand(2, S, S)))
