@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                     }
                 }
                 s_is_read();
-                const bool set = fresh ? mx != -INFINITY : mx > base + SLACK;
+                const bool set = fresh ? mx != -INFINITY : mx - base > SLACK;   // (base + SLACK could round up)
                 const bool move = __any_sync(0xffffffffu, set);
                 wait_product();
                 if (move) {

@@ -329,3 +329,22 @@ def test_attention_slopes_with_a_table(dt, D, S, k_len, pos, reach, slope, causa
         seen = seen & (j <= p)
     y = rt.attention(q, k, v, slopes=slopes, dist_bias=table, k_len=i32(k_len), q_pos=i32(pos), causal=causal)
     within(y, *scores_ref(q, k, v, bias, seen.expand(2, S, S)))
+
+
+# ------------------------------------------------------------------------ biases of any size
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 900, 64), (40, 300, 64), (700, 700, 64), (700, 900, 128)])
+@pytest.mark.parametrize("bias", [1e5, 1e7, 5e7, 9e7, 1.2e8, 1.5e8, 1.8e8, 3e8, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+def test_attention_common_biases_of_any_size(dt, Sq, Sk, D, bias, sign, cap):
+    """One bias for all keys takes bits of the scores, down to a uniform row, but a result stays an average."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 2, 2, D, dt)
+    y = rt.attention(q, k, v, scale=2.0, cap=cap, dist_bias=torch.full((2, 1), sign * bias, device="cuda"))
+    top, low = v.double().amax(1, keepdim=True), v.double().amin(1, keepdim=True)
+    slack = 4 * half_step(dt) * v.double().abs().amax(1, keepdim=True)
+    assert y.isfinite().all() and (y.double() <= top + slack).all() and (y.double() >= low - slack).all()
+    if bias >= 1e12:
+        mean, mag = v.double().mean(1, keepdim=True), v.double().abs().mean(1, keepdim=True)
+        within(y, mean.expand_as(y), (half_step(dt) * (mean.abs() + mag) + (Sk + 8) * U22 * mag + 2.0 ** -24).expand_as(y))
