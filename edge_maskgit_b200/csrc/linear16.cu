@@ -49,10 +49,12 @@ __device__ __forceinline__ float gelu16(float x) {
     const float half = 0.5f * x;
     return fmaf(-a, h, half + fabsf(half));   // (max(x, 0) with a NaN that stays one; x + |x| would overflow)
 }
+// x / (1 + e^-x), from e^-|x| so that nothing overflows: small results keep their precision too.
 __device__ __forceinline__ float silu16(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_approx(x * -1.4426950409f)));
-    return x * r;
+    float e, r;   // (e may be subnormal: no flush)
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(fabsf(x) * -1.4426950409f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return x * (x < 0.0f ? e : 1.0f) * r;
 }
 __device__ __forceinline__ float act16(float v, int a) { return a == 1 ? gelu16(v) : a == 2 ? silu16(v) : v; }
 template <int N>

@@ -348,3 +348,18 @@ def test_attention_common_biases_of_any_size(dt, Sq, Sk, D, bias, sign, cap):
     if bias >= 1e12:
         mean, mag = v.double().mean(1, keepdim=True), v.double().abs().mean(1, keepdim=True)
         within(y, mean.expand_as(y), (half_step(dt) * (mean.abs() + mag) + (Sk + 8) * U22 * mag + 2.0 ** -24).expand_as(y))
+
+
+# --------------------------------------------------------------------------------- SiLU
+@pytest.mark.parametrize("M,N", [(1, 64), (300, 2025), (2048, 2304), (4100, 2025)])
+def test_linear_silu_keeps_small_results(M, N):
+    """Sums from -90 to 0 that are exact: results down to 2^-123, relative to themselves.  The exponential's exponent, up to
+    130 in base 2, takes two roundings of 2^-24 (1.1e-5 of the result at most); the rest a few 1e-6."""
+    from edge_maskgit_b200 import runtime as rt
+    x, w = torch.zeros(M, 8, device="cuda", dtype=BF16), torch.zeros(N, 8, device="cuda", dtype=BF16)
+    w[:, 0] = -torch.linspace(0.0, 90.0, N, device="cuda").to(BF16)
+    x[:, 0] = 1.0
+    y = rt.linear(x, w, act=2)
+    s = w[:, 0].double().expand(M, N)
+    ref = s * torch.sigmoid(s)
+    within(y, ref, (half_step(BF16) + 2e-5) * ref.abs())
