@@ -55,33 +55,37 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(copy ? 16 : 0) : "memory");
 }
 
-// Writes one finished row (o = dims lane + 32 u), repairing a suspect one.
+// Writes one finished row (o = dims lane + 32 u, l their sum of probabilities), and puts suspect results right.
 template <bool BF16>
-__device__ __forceinline__ void write_row(const AttnCall& c, int b, int h, int i, float (&o)[4]) {
+__device__ __forceinline__ void write_row(const AttnCall& c, int b, int h, int i, const float (&o)[4], float l) {
     const int lane = threadIdx.x & 31;
+    const long long at = b * c.a.out_stride[0] + i * c.a.out_stride[1] + h * c.a.out_stride[2];
     bool bad = false;
 #pragma unroll
-    for (int u = 0; u < 4; u++) bad |= lane + 32 * u < c.a.D && suspect<BF16>(o[u]);
-    if (__any_sync(0xffffffffu, bad)) exact_row<BF16>(c.a, c.g, b, h, i, o);
-    const long long at = b * c.a.out_stride[0] + i * c.a.out_stride[1] + h * c.a.out_stride[2];
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-        if (lane + 32 * u < c.a.D) store16<BF16>(c.a.out, at + lane + 32 * u, o[u]);
+    for (int u = 0; u < 4; u++) {
+        if (lane + 32 * u >= c.a.D) continue;
+        bad |= suspect<BF16>(o[u]);
+        store16<BF16>(c.a.out, at + lane + 32 * u, o[u]);
+    }
+    if (__any_sync(0xffffffffu, bad) && !isnan(l)) {
+        __syncwarp();
+        repair_row<BF16>(c.a, c.g, b, h, i);
+    }
 }
 
-// The same from sums of unnormalised values: o = dims 4 lane .. 4 lane + 3, l their sum of probabilities.
+// The same from sums of unnormalised values: o = dims 4 lane .. 4 lane + 3.
 template <bool BF16>
 __device__ __forceinline__ void write_row4(const AttnCall& c, int b, int h, int i, float4 o, float l) {
     const int lane = threadIdx.x & 31;
     const bool dims = lane * 4 < c.a.D;
-    if (__any_sync(0xffffffffu, dims && (suspect<BF16>(o.x) || suspect<BF16>(o.y) || suspect<BF16>(o.z) || suspect<BF16>(o.w) || isnan(l)))) {
-        float nan[4] = {NAN, NAN, NAN, NAN};
-        write_row<BF16>(c, b, h, i, nan);
-        return;
-    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t* dst = reinterpret_cast<uint16_t*>(c.a.out) + b * c.a.out_stride[0] + i * c.a.out_stride[1] + h * c.a.out_stride[2];
     if (dims) reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<BF16>(o.x * inv, o.y * inv), pack16<BF16>(o.z * inv, o.w * inv));
+    const bool bad = dims && (suspect<BF16>(o.x) || suspect<BF16>(o.y) || suspect<BF16>(o.z) || suspect<BF16>(o.w));
+    if (__any_sync(0xffffffffu, bad) && !isnan(l)) {
+        __syncwarp();
+        repair_row<BF16>(c.a, c.g, b, h, i);
+    }
 }
 
 // grid: splits x (batch row, key head, 16-row block), splits fastest
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(WARPS * 32) attn_step_kernel(const __grid_cons
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
             for (int u = 0; u < 4; u++) acc[u] = ll == 0.0f ? 0.0f : acc[u] * inv;
-            write_row<BF16>(c, b, h, i, acc);
+            write_row<BF16>(c, b, h, i, acc, ll);
         } else {
             const long long all = (long long)a.B * a.Sq * a.Hq;
             const long long id = split * all + ((long long)b * a.Sq + i) * a.Hq + h;

@@ -796,19 +796,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 }
                 __syncwarp();
             }
-            bad = (bad || isnan(l)) && live && c.nsplit == 1;   // (split: the join looks for it)
-            unsigned todo = __ballot_sync(0xffffffffu, bad);
-            while (todo) {
-                const int k = __ffs(todo) - 1;
-                todo &= todo - 1;
-                const int bad_i = q0 + w * QT + (warp & 3) * 32 + k;
-                float o[4];
-                exact_row<BF16>(a, c.g, b, h, bad_i, o);
-                const long long at = b * a.out_stride[0] + bad_i * a.out_stride[1] + h * a.out_stride[2];
-#pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (lane + 32 * u < a.D) store16<BF16>(a.out, at + lane + 32 * u, o[u]);
-            }
+            bad = bad && !isnan(l) && live && c.nsplit == 1;   // (split: the join looks for it)
+            for (unsigned todo = __ballot_sync(0xffffffffu, bad); todo; todo &= todo - 1)
+                repair_row<BF16>(a, c.g, b, h, q0 + w * QT + (warp & 3) * 32 + __ffs(todo) - 1);
         }
     }
     __syncwarp();

@@ -363,3 +363,62 @@ def test_linear_silu_keeps_small_results(M, N):
     s = w[:, 0].double().expand(M, N)
     ref = s * torch.sigmoid(s)
     within(y, ref, (half_step(BF16) + 2e-5) * ref.abs())
+
+
+# ------------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 300, 64), (1, 9000, 128), (3, 700, 48), (40, 300, 64), (500, 500, 64), (500, 700, 128), (128, 4000, 64)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_one_bad_dim_leaves_the_others(dt, Sq, Sk, D, bad):
+    """A NaN or infinity in one dim of a seen key's v: that dim is it, every other bit is as without it."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, Sq, Sk, 4, 2, D, dt)
+    p = Sk - Sq + torch.arange(Sq, device="cuda")
+    for at in (0, Sk // 3, Sk - 1):
+        want = rt.attention(q, k, v, causal=True)
+        w = v.clone()
+        w[0, at, 1, 5] = bad
+        y = rt.attention(q, k, w, causal=True)
+        sees = p >= at
+        hit = y[0, sees][:, 2:, 5]
+        assert hit.isnan().all() if math.isnan(bad) else (hit == bad).all()
+        want[0, sees.nonzero()[:, 0][:, None], torch.arange(2, 4, device="cuda")[None], 5] = 0.0
+        y[0, sees.nonzero()[:, 0][:, None], torch.arange(2, 4, device="cuda")[None], 5] = 0.0
+        # rows that do not see it, in a tile that holds it, have that one dim computed in another order
+        near = 2 * half_step(dt) * v.abs().max().item()
+        assert (y[..., 5] - want[..., 5]).abs().max().item() <= near
+        y[..., 5] = want[..., 5] = 0.0
+        assert torch.equal(y, want)
+
+
+def test_attention_infinities_of_small_weight_and_of_both_signs():
+    from edge_maskgit_b200 import runtime as rt
+    for Sq, Sk, D, dt in ((1, 400, 64, F16), (300, 400, 64, F16), (300, 400, 128, BF16), (1, 9000, 64, BF16)):
+        q, k, v = qkv(1, Sq, Sk, 2, 2, D, dt)
+        q, k = torch.zeros_like(q), torch.zeros_like(k)
+        q[..., 0], k[:, 7, :, 0] = 1.0, 100.0   # key 7 has all but e^-100 of the weight
+        v[0, 9, 0, 3], v[0, 9, 1, 3], v[0, 11, 1, 3], v[0, 9, 1, 4] = math.inf, math.inf, -math.inf, -math.inf
+        y = rt.attention(q, k, v, scale=1.0)
+        assert (y[:, :, 0, 3] == math.inf).all() and y[:, :, 1, 3].isnan().all() and (y[:, :, 1, 4] == -math.inf).all()
+        assert y[:, :, :, 5:].isfinite().all()
+        table = torch.zeros(2, 2 * Sk + 1, device="cuda")
+        pos = Sk - 1 if Sq == 1 else 0
+        if Sq == 1:   # a score of -inf hides a key, whatever its value
+            table[:, 9 - pos + Sk] = table[:, 11 - pos + Sk] = -math.inf
+            assert rt.attention(q, k, v, scale=1.0, dist_bias=table).isfinite().all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_a_nan_that_all_rows_see_costs_little(bad):
+    """It took 350 ms where every row was computed again."""
+    from edge_maskgit_b200 import runtime as rt
+    q, k, v = qkv(1, 4096, 4096, 32, 8, 128, BF16)
+    v[0, 100] = bad
+    rt.attention(q, k, v, causal=True)
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    e[0].record()
+    y = rt.attention(q, k, v, causal=True)
+    e[1].record()
+    torch.cuda.synchronize()
+    assert not y[0, 100:].isfinite().any() and y[0, :100].isfinite().all()
+    assert e[0].elapsed_time(e[1]) < 60.0
