@@ -650,12 +650,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 }
                 float mx = max3_nan(max3_nan(hi[0], hi[1], hi[2]), hi[3], hi[3]);
                 if (raw && !(MODE & SLOPE) && mx != -INFINITY) mx = fmaf(mx, x.c1, x.lin_a);
-                if (!(MODE & CAP) && raw && __any_sync(0xffffffffu, fabsf(mx) > LINEAR_MAX && mx != -INFINITY)) {
-                    raw = false;   // scores of that size round like their maximum
-#pragma unroll
-                    for (int j = 0; j < 128; j++)
-                        s[j] = __float_as_uint(fmaf(__uint_as_float(s[j]), x.c1, fmaf((float)j, x.lin_b, x.lin_a)));
-                }
                 if (MODE == CAP) {
                     const float low = fminf(fminf(lo_s[0], lo_s[1]), fminf(lo_s[2], lo_s[3]));
                     raw = !masked && __all_sync(0xffffffffu, fmaxf(mx, -low) * fabsf(x.c1) <= CAP_RAW && mx == mx);
@@ -676,9 +670,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
                 }
                 s_is_read();
                 const bool set = fresh ? mx != -INFINITY : mx - base > SLACK;   // (base + SLACK could round up)
-                const bool move = __any_sync(0xffffffffu, set);
+                const bool large = !(MODE & CAP) && raw && fabsf(mx) > LINEAR_MAX && mx != -INFINITY;
+                const bool move = __any_sync(0xffffffffu, set || large);
                 wait_product();
                 if (move) {
+                    if (!(MODE & CAP) && __any_sync(0xffffffffu, large)) {
+                        raw = false;   // scores of that size round like their maximum
+#pragma unroll
+                        for (int j = 0; j < 128; j++)
+                            s[j] = __float_as_uint(fmaf(__uint_as_float(s[j]), x.c1, fmaf((float)j, x.lin_b, x.lin_a)));
+                    }
                     float alpha = 1.0f;
                     if (set) {
                         const float nb = __fadd_ru(mx, -SHIFT);
