@@ -602,6 +602,8 @@ class CudaRuntime:
         cls = np.ascontiguousarray(class_ids, dtype=np.int32)
         sd = np.ascontiguousarray(seeds, dtype=np.uint64)
         B = cls.shape[0]
+        if sd.size < B:
+            raise MgcError(f"generate: {B} images need a seed each, not {sd.size}")
         out = np.empty((B, self.hparams.n_tokens + 1), np.int32)
         if controls is None:
             check(lib.mgc_generate(self._h, B, _ptr(cls), _ptr(sd), steps, temperature, _ptr(out)), "generate")
@@ -617,6 +619,8 @@ class CudaRuntime:
         cls = np.ascontiguousarray(class_ids, np.int32)
         sd = np.ascontiguousarray(seeds, np.uint64)
         B, R = len(cls), vq.resolution
+        if sd.size < B:
+            raise MgcError(f"generate_images: {B} images need a seed each, not {sd.size}")
         rgb = np.empty((B, R, R, 3), np.uint8)
         tok = np.empty((B, self.hparams.n_tokens + 1), np.int32)
         check(lib.mgc_generate_images(self._h, vq._h, B, _ptr(cls), _ptr(sd), steps, temperature, _ptr(rgb),

@@ -43,3 +43,14 @@ def test_forbidden_codes_stay_out_at_the_bounds(model, at, bias):
     allowed[[11, 12, hp.codebook_size // 2]] = True
     got = model.generate(*ARGS, controls=rt.LogitControls(allowed=allowed, bias=np.full(hp.codebook_size, bias, np.float32), **at))
     assert allowed[got[:, 1:]].all()
+
+
+@pytest.mark.parametrize("seeds", [[], [1, 2]])
+def test_a_seed_for_each_image(model, seeds):
+    """Fewer seeds than images were read past their end."""
+    from types import SimpleNamespace
+    from edge_maskgit_b200 import runtime as rt
+    for call in (lambda: model.generate([3, 7, 100], seeds), lambda: model.generate([3, 7, 100], seeds, controls=rt.LogitControls(presence=1.0)),
+                 lambda: model.generate_images(SimpleNamespace(resolution=16, _h=None), [3, 7, 100], seeds)):
+        with pytest.raises(rt.MgcError, match="a seed each"):
+            call()
