@@ -466,7 +466,8 @@ class OpProfile:   # include/mg-opencl.hpp:17-21
 class LogitControls:
     """What generate() does to the logits of the codes before each draw (mgc_logit_controls):
     penalties against the codes an image already holds, a bias [codebook], and allowed codes as
-    truth values [codebook] or, one row per grid cell, [n_tokens][codebook]."""
+    truth values [codebook] or, one row per grid cell, [n_tokens][codebook].  The bias is finite,
+    repetition from 2^-60 to 2^60, frequency and presence at most 2^60."""
     repetition: float = 1.0
     frequency: float = 0.0
     presence: float = 0.0

@@ -132,7 +132,8 @@ int mgc_linear(int dtype, const void* x_dev, int64_t ldx, const void* w_dev, int
  *   and its score is not -inf (a -inf in dist_bias hides a distance).
  * out = softmax(s) . v over the seen keys, and zeros for a query that sees none.  What k and v
  * hold at unseen keys, NaN included, does not reach the result, and keys from k_len[b] on are not
- * used at all.  Scores, softmax statistics and sums are f32; probabilities are rounded to dtype
+ * used at all (a row that shares a 128-key tile with a masked NaN or infinity is computed a second time,
+ * slowly).  Scores, softmax statistics and sums are f32; probabilities are rounded to dtype
  * for the product with v, as is the result. */
 typedef struct mgc_attention_args {
     int32_t dtype;              /* MGC_F16 or MGC_BF16: q, k, v and out */
