@@ -12,7 +12,7 @@ namespace mgc {
 constexpr float ATTN_LOG2E = 1.4426950408889634f;
 
 // The call, as the kernels get it.  Partial results (nsplit > 1), per split and row
-// (b * Sq + i) * Hq + h: the unnormalised output f32 [D], then (row max in base 2, sum).
+// (b * Sq + i) * Hq + h: the unnormalised output f32 [D], then (base, sum): probabilities are 2^(t - base).
 struct AttnCall {
     mgc_attention_args a;
     int g;                 // query heads per key head
