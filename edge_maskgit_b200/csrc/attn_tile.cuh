@@ -744,15 +744,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tile_kernel(const __grid_cons
         // A warp whose wait gave up still meets the tile's other warps at its remaining steps: one of them may
         // see the scores that it waits for before it sees the flag, and nothing bounds the wait at a meeting.
         if (!ok && ((MODE & TABLE) || a.doc_k)) {
-            auto meets = [&](int kt) {
-                if (a.doc_k) return true;
-                fetch(kt);
-                return !is_flat(kt);
-            };
 #pragma unroll 1
             while (++it < n_w) {
-                for (i++; !mine(i);) i++;
-                if (meets(order(i))) named_bar_sync(bar_id, 128);
+                bool meet = true;   // (with documents, at each step)
+                if ((MODE & TABLE) && !a.doc_k) {
+                    for (i++; !mine(i);) i++;
+                    fetch(order(i));
+                    meet = !is_flat(order(i));
+                }
+                if (meet) named_bar_sync(bar_id, 128);
             }
         }
         // ---------------------------------------------------------------- output
